@@ -600,6 +600,102 @@ int myl_attention_int(myl_ctx* ctx, const int16_t* q, int64_t q_len, const int16
                       int64_t score_mult, uint8_t score_shift, const int16_t* exp_lut,
                       int64_t exp_len, uint8_t lut_shift, uint8_t prob_frac_bits, int16_t* out);
 
+/* --- Serving many requests that share a prompt ---------------------------------------
+ * No counterpart in the reference, which runs one sequence; each operator is
+ * composed of its primitives, so every result is one exact integer.
+ *
+ * Attention plan: the constants of attention_int (attention.rs:42-94) and of
+ * the rescale to the output projection's input (model.rs:563-567):
+ * score = i32(rne(dot * score_mult, score_shift)), exp_lut / lut_shift /
+ * prob_frac_bits of softmax_int, out_shift = v_frac - attn_out_frac in
+ * [-31, 30]. Limits: prob_frac_bits <= 15, exp_lut[0] > 0 and no negative entry,
+ * entries times 2^prob_frac_bits inside i32. */
+typedef struct myl_attn_plan myl_attn_plan;
+int myl_attn_plan_create(myl_ctx* ctx, int64_t score_mult, uint8_t score_shift,
+                         const int16_t* exp_lut, int64_t exp_len, uint8_t lut_shift,
+                         uint8_t prob_frac_bits, int out_shift, myl_attn_plan** out);
+int myl_attn_plan_release(myl_ctx* ctx, myl_attn_plan* plan);
+/* A prefix shared by a batch: keys and values of `positions` positions, device
+ * pointers, element (head g, position j, dim d) at g * head_stride +
+ * j * pos_stride + d. They are laid out once as byte planes (the int16 arrays
+ * may be freed afterwards); the call synchronises `stream`. head_dim: a
+ * multiple of 8 up to 248. positions may be 0. */
+typedef struct myl_prefix myl_prefix;
+int myl_prefix_create(myl_ctx* ctx, const int16_t* k, const int16_t* v, int64_t positions,
+                      int64_t num_kv_heads, int64_t head_dim, int64_t pos_stride,
+                      int64_t head_stride, void* stream, myl_prefix** out);
+int myl_prefix_release(myl_ctx* ctx, myl_prefix* prefix);
+int64_t myl_prefix_positions(const myl_prefix* prefix);
+/* Attention of T new tokens of each of `batch` requests (rotated queries
+ * q [batch * T][ldq], head h at h * head_dim) over the prefix and the
+ * request's own suffix cache (element (b, g, j, d) at b * seq_stride +
+ * g * head_stride + j * pos_stride + d, j < suffix_cap). lens[b] (device) is
+ * the number of suffix entries including the T new ones: token t sees the
+ * prefix and suffix entries 0 .. lens[b] - T + t (none if that is negative).
+ * out [batch * T][ldo] int16; a row that sees no key gives zeros. A length
+ * outside [0, suffix_cap] is clamped and reported as MYL_ERR_DEVICE at the next
+ * synchronising call. q, k_suffix and v_suffix are 16-byte aligned, strides
+ * multiples of 8 elements. Equal to attention_int over the concatenated keys. */
+int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_prefix* prefix,
+                             const int16_t* q, int64_t batch, int64_t T, int64_t num_heads,
+                             int64_t ldq, const int16_t* k_suffix, const int16_t* v_suffix,
+                             int64_t suffix_cap, int64_t seq_stride, int64_t head_stride,
+                             int64_t pos_stride, const int32_t* lens, int16_t* out, int64_t ldo,
+                             void* stream);
+
+/* Low-rank adapters of one projection (host arrays): A [num][rank][in_features],
+ * B [num][out_features][rank] int8 with one shift per row (a_shifts
+ * [num][rank], b_shifts [num][out_features]):
+ *   h = clamp_i16(rescale(dot(A[a][i], x), a_shifts + act_frac, h_frac))
+ *   y = clamp_i16(linear(x) + clamp_i16(rescale(dot(B[a][n], h), b_shifts + h_frac, out_frac)))
+ * with the primitives of linear.rs:43-70 and :132-145; linear(x) is
+ * myl_linear_dev of the same weight and requant plan (bias included). An
+ * adapter of a smaller rank is padded with zero rows and columns. rank <= 256. */
+typedef struct myl_adapters myl_adapters;
+int myl_adapters_register(myl_ctx* ctx, int64_t num, int64_t rank, int64_t in_features,
+                          int64_t out_features, const int8_t* A, const uint8_t* a_shifts,
+                          const int8_t* B, const uint8_t* b_shifts, uint8_t act_frac,
+                          uint8_t h_frac, uint8_t out_frac, myl_adapters** out);
+int myl_adapters_release(myl_ctx* ctx, myl_adapters* adapters);
+/* y [M][ldy] int16 = the projection of x [M][ldx] with row m's adapter ids[m]
+ * (device; -1: none). An id outside [-1, num) counts as none and is reported as
+ * MYL_ERR_DEVICE at the next synchronising call. int8 weights with an int16
+ * requant only. y must not overlap x. */
+int myl_linear_adapters_dev(myl_ctx* ctx, const myl_weight* w, const myl_requant* rq,
+                            const myl_adapters* adapters, const int16_t* x, int64_t M, int64_t ldx,
+                            const int32_t* ids, int16_t* y, int64_t ldy, void* stream);
+
+/* Verification of drafted tokens (speculative sampling on integer weights).
+ * A logit row has the weights w_j = exp_lut[((max - l_j) * temp_mult) >>
+ * temp_shift] (0 past the table; the difference saturates at 2^31 - 1) and
+ * their sum S: temp_mult / 2^temp_shift maps logit units to the table's grid,
+ * divided by the temperature. For request b, positions i = 0, 1, ... with
+ * drafted token x = tokens[b][i], target weights w and draft weights z (one-hot
+ * at x when draft is NULL), and the halves u = rand[b][i] >> 32 and
+ * u' = rand[b][i] & 0xFFFFFFFF:
+ *   i < counts[b] and u * z_x * S_w < 2^32 * w_x * S_z: x is accepted, go on;
+ *   i < counts[b] otherwise: the token is drawn from max(w_j S_z - z_j S_w, 0)
+ *   (from w_j if that is 0 everywhere); i = counts[b]: it is drawn from w_j,
+ * as the lowest index whose inclusive sum exceeds floor(u' * total / 2^32).
+ * accepted[b] = number of accepted tokens n; out_tokens[b] = the n accepted
+ * tokens, the drawn one, then -1. Logits are device int32, row (b, i) at
+ * b * seq_stride + i * pos_stride (target: drafted + 1 rows, draft: drafted);
+ * tokens [batch][drafted], counts [batch] (NULL: drafted), rand
+ * [batch][drafted + 1], out_tokens [batch][drafted + 1] contiguous. A drafted
+ * token outside the vocabulary counts as having no weight, a count outside
+ * [0, drafted] is clamped; both are reported as MYL_ERR_DEVICE at the next
+ * synchronising call. Limits: vocab times the largest table entry below 2^32,
+ * drafted <= 1024. */
+typedef struct myl_verifier myl_verifier;
+int myl_verifier_create(myl_ctx* ctx, const int16_t* exp_lut, int64_t exp_len, uint32_t temp_mult,
+                        uint8_t temp_shift, myl_verifier** out);
+int myl_verifier_release(myl_ctx* ctx, myl_verifier* verifier);
+int myl_verify_dev(myl_ctx* ctx, const myl_verifier* verifier, const int32_t* target,
+                   int64_t target_seq_stride, int64_t target_pos_stride, const int32_t* draft,
+                   int64_t draft_seq_stride, int64_t draft_pos_stride, int64_t batch,
+                   int64_t drafted, int64_t vocab, const int32_t* tokens, const int32_t* counts,
+                   const uint64_t* rand, int32_t* accepted, int32_t* out_tokens, void* stream);
+
 /* --- Allocation-free variant ------------------------------------------------------
  * No counterpart in the reference: its CPU path never allocates device memory.
  *

@@ -458,6 +458,10 @@ class Weight:
             self.ctx.handle, self._h, rq.handle, _p(x), M, x.stride(0), _p(y), y.stride(0),
             _stream_ptr(stream)))
 
+    def linear_adapters_dev(self, rq: "Requant", adapters, x, ids, y, stream=None) -> None:
+        """linear_dev plus row m's low-rank adapter ids[m] (-1: none), see Adapters."""
+        linear_adapters_dev(self, rq, adapters, x, ids, y, stream)
+
     def linear_planes_dev(self, rq, xhi, xlo, M: int, y, stream=None) -> None:
         """Tensor-core GEMM from byte planes; rq=None stores int64 accumulators."""
         _check("myl_linear_planes_dev", load_library().myl_linear_planes_dev(
@@ -918,6 +922,9 @@ def _stream_ptr(stream) -> int | None:
         return int(stream.cuda_stream) or None
     return int(stream) or None
 
+
+from .serving import (Adapters, AttentionPlan, DraftVerifier, Prefix,  # noqa: E402,F401
+                      linear_adapters_dev)
 
 # ---- the reference's free functions ---------------------------------------------
 

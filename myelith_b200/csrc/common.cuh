@@ -30,6 +30,8 @@ enum DeviceError : int {
   DEV_WAIT_PEER = 0x106,      // a peer rank did not reach an exchange barrier in time
   DEV_BAD_EXPERT = 0x201,     // an expert id outside the experts this object holds
   DEV_BAD_TOKEN = 0x202,      // a token id outside the vocabulary (device-side ids)
+  DEV_BAD_LENGTH = 0x203,     // a device-side length outside its capacity
+  DEV_BAD_ADAPTER = 0x204,    // an adapter id outside the registered adapters
 };
 
 // Epilogue modes.

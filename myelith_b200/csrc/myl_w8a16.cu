@@ -134,7 +134,7 @@ struct myl_ctx {
   int pdl = 0;         // launch with programmatic stream serialization (the forward's chains)
   int64_t launches = 0;
   PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-  DevBuf x, y, rq, planes, part, h, hplanes, moe, xsum, crc;
+  DevBuf x, y, rq, planes, part, h, hplanes, moe, xsum, crc, pfx, ad_h, vfy;
   // Host-pointer calls on page-locked memory: copy-in and copy-out streams
   // and one event pair per chunk.
   cudaStream_t s_in = nullptr, s_out = nullptr;
@@ -748,7 +748,9 @@ static int check_device_error(myl_ctx* ctx) {
     return fail(MYL_ERR_DEVICE, "kernel reported error 0x%x (%s)", e,
                 e == DEV_BAD_EXPERT  ? "an expert id outside this object's experts"
                 : e == DEV_BAD_TOKEN ? "a token id outside the vocabulary"
-                                     : "a bounded wait ran out");
+                : e == DEV_BAD_LENGTH  ? "a length outside its capacity"
+                : e == DEV_BAD_ADAPTER ? "an adapter id outside the registered adapters"
+                                       : "a bounded wait ran out");
   }
   return MYL_OK;
 }
@@ -889,7 +891,7 @@ int myl_destroy(myl_ctx* ctx) {
   for (auto& kv : ctx->backend_cache) myl_weight_release(ctx, kv.second);
   ctx->backend_cache.clear();
   for (DevBuf* b : {&ctx->x, &ctx->y, &ctx->rq, &ctx->planes, &ctx->part, &ctx->h, &ctx->hplanes,
-                    &ctx->moe, &ctx->xsum, &ctx->crc})
+                    &ctx->moe, &ctx->xsum, &ctx->crc, &ctx->pfx, &ctx->ad_h, &ctx->vfy})
     if (b->p) cudaFree(b->p);
   if (ctx->d_err) cudaFree(ctx->d_err);
   if (ctx->h_err) cudaFreeHost(ctx->h_err);
@@ -2790,3 +2792,4 @@ int myl_wire_unpack_tokens(const int16_t* values, uint64_t n_values, uint32_t* t
 }  // extern "C"
 
 #include "model.cuh"
+#include "serving.cuh"

@@ -1,0 +1,447 @@
+// serving.cuh — host side of the operators for serving many requests that
+// share a prompt (myl_attn_plan_*, myl_prefix_*, myl_adapters_*,
+// myl_linear_adapters_dev, myl_verify_*), included by myl_w8a16.cu after the
+// linear code and the forward.
+
+#include "adapters.cuh"
+#include "prefix.cuh"
+#include "verify.cuh"
+
+struct myl_attn_plan {
+  int16_t* d_lut = nullptr;
+  int64_t exp_len = 0;
+  int32_t exp_max = 0;
+  int64_t score_mult = 0;
+  int score_shift = 0, lut_shift = 0, prob_frac = 0, out_shift = 0;
+  std::vector<void*> allocs;
+};
+
+struct myl_prefix {
+  int64_t P = 0, Pp = 0, nkv = 0, hd = 0;
+  uint8_t *kh = nullptr, *kl = nullptr, *vth = nullptr, *vtl = nullptr;
+  std::vector<void*> allocs;
+};
+
+struct myl_adapters {
+  int64_t num = 0, rank = 0, K = 0, N = 0, lda = 0, ldb = 0;
+  int8_t *A = nullptr, *B = nullptr, *sa = nullptr, *sb = nullptr;
+  std::vector<void*> allocs;
+};
+
+struct myl_verifier {
+  int16_t* d_lut = nullptr;
+  int64_t len = 0;
+  int32_t max = 0;
+  uint32_t mult = 0;
+  int shift = 0;
+  std::vector<void*> allocs;
+};
+
+namespace {
+
+// An exponential table whose row sums stay positive: entry 0 (the row
+// maximum's) positive, none negative.
+int check_exp_lut(const int16_t* lut, int64_t len, int32_t* mx) {
+  if (len <= 0 || len > (int64_t(1) << 31) - 1) return fail(MYL_ERR_SHAPE, "exp table of %lld entries", (long long)len);
+  *mx = 0;
+  for (int64_t i = 0; i < len; ++i) {
+    if (lut[i] < 0) return fail(MYL_ERR_UNSUPPORTED, "negative exp table entry %lld", (long long)i);
+    *mx = std::max<int32_t>(*mx, lut[i]);
+  }
+  if (lut[0] <= 0) return fail(MYL_ERR_UNSUPPORTED, "exp table entry 0 must be positive");
+  return MYL_OK;
+}
+
+template <typename T>
+void free_handle(myl_ctx* ctx, T* h) {
+  if (ctx) {
+    cudaSetDevice(ctx->device);
+    cudaStreamSynchronize(ctx->stream);
+  }
+  for (void* p : h->allocs) cudaFree(p);
+  (void)cudaGetLastError();  // a failed allocation is reported once, by the call that made it
+  delete h;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int attn_plan_build(myl_attn_plan* pl, int64_t score_mult, uint8_t score_shift, const int16_t* exp_lut,
+                    int64_t exp_len, uint8_t lut_shift, uint8_t prob_frac, int out_shift) {
+  if (score_shift > 62 || lut_shift > 31 || out_shift < -31 || out_shift > 30)
+    return fail(MYL_ERR_OVERFLOW, "attention shifts (%u, %u, %d)", unsigned(score_shift), unsigned(lut_shift), out_shift);
+  if (prob_frac > 15)
+    return fail(MYL_ERR_UNSUPPORTED, "prob_frac_bits %u: at most 15 (probabilities are 16-bit operands)",
+                unsigned(prob_frac));
+  TRY(check_exp_lut(exp_lut, exp_len, &pl->exp_max));
+  if ((int64_t(pl->exp_max) << prob_frac) > INT32_MAX)
+    return fail(MYL_ERR_OVERFLOW, "exp table values times 2^prob_frac_bits overflow i32");
+  pl->exp_len = exp_len;
+  pl->score_mult = score_mult;
+  pl->score_shift = score_shift;
+  pl->lut_shift = lut_shift;
+  pl->prob_frac = prob_frac;
+  pl->out_shift = out_shift;
+  return dev_upload(pl->allocs, &pl->d_lut, exp_lut, size_t(exp_len));
+}
+
+int prefix_build(myl_ctx* ctx, myl_prefix* pf, const int16_t* k, const int16_t* v, int64_t pos_stride,
+                 int64_t head_stride, cudaStream_t st) {
+  const size_t n = size_t(pf->nkv) * size_t(pf->Pp) * size_t(pf->hd);
+  TRY(dev_alloc(pf->allocs, &pf->kh, n));
+  TRY(dev_alloc(pf->allocs, &pf->kl, n));
+  TRY(dev_alloc(pf->allocs, &pf->vth, n));
+  TRY(dev_alloc(pf->allocs, &pf->vtl, n));
+  if (pf->P > 0) {
+    const dim3 grid(unsigned(pf->Pp / 32), unsigned((pf->hd + 31) / 32), unsigned(pf->nkv));
+    prefix_planes_kernel<<<grid, 256, 0, st>>>(k, v, pf->P, pf->Pp, int(pf->hd), pos_stride, head_stride, pf->kh,
+                                               pf->kl, pf->vth, pf->vtl);
+    CUDA_TRY(cudaGetLastError());
+    ctx->launches++;
+  }
+  CUDA_TRY(cudaStreamSynchronize(st));
+  return MYL_OK;
+}
+
+// The attention of `p` (pointers, shapes and plan filled in) with the
+// context's workspace, which the caller holds.
+int run_prefix_attention(myl_ctx* ctx, PrefixParams& p, cudaStream_t st) {
+  const int64_t rows = int64_t(p.nkv) * p.R;
+  p.lds = p.Pp + ((p.S + 31) & ~31);
+  const size_t o_max = size_t(rows) * size_t(p.hd) * 8, o_sum = o_max + size_t(rows) * 4,
+               o_sc = (o_sum + size_t(rows) * 4 + 255) & ~size_t(255);
+  TRY(ensure(ctx->pfx, o_sc + size_t(rows) * size_t(p.lds) * 4));
+  uint8_t* ws = static_cast<uint8_t*>(ctx->pfx.p);
+  p.acc = reinterpret_cast<unsigned long long*>(ws);
+  p.rowmax = reinterpret_cast<unsigned*>(ws + o_max);
+  p.rowsum = reinterpret_cast<int32_t*>(ws + o_sum);
+  p.scores = reinterpret_cast<int32_t*>(ws + o_sc);
+  p.err = ctx->d_err;
+  const unsigned flat = unsigned(std::min<int64_t>((rows * p.hd + 255) / 256, int64_t(ctx->num_sms) * 8));
+  {
+    LaunchCfg lc(ctx, dim3(flat), dim3(256), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, prefix_init_kernel, p, rows));
+    ctx->launches++;
+  }
+  if (p.P > 0 || p.S > 0) {
+    const unsigned gy = unsigned(p.nkv * ((p.R + PFX_ROWS - 1) / PFX_ROWS));
+    if (gy > 65535u) return fail(MYL_ERR_UNSUPPORTED, "%d query rows per KV head", p.R);
+    const int nb1 = (p.P + PFX_SKEYS - 1) / PFX_SKEYS, t1 = (p.S + PFX_SKEYS - 1) / PFX_SKEYS;
+    LaunchCfg l1(ctx, dim3(unsigned(nb1 + p.B * t1), gy), dim3(PFX_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_scores_kernel, p, nb1, t1));
+    LaunchCfg l2(ctx, dim3(unsigned(rows)), dim3(PFX_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_sum_kernel, p));
+    const int nb3 = (p.P + PFX_VKEYS - 1) / PFX_VKEYS, t3 = (p.S + PFX_VKEYS - 1) / PFX_VKEYS;
+    LaunchCfg l3(ctx, dim3(unsigned(nb3 + p.B * t3), gy), dim3(PFX_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_values_kernel, p, nb3, t3));
+    ctx->launches += 3;
+  }
+  LaunchCfg l4(ctx, dim3(flat), dim3(256), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l4.cfg, prefix_finish_kernel, p, rows));
+  ctx->launches++;
+  return MYL_OK;
+}
+
+void prefix_params(PrefixParams& p, const myl_attn_plan* pl, const myl_prefix* pf) {
+  p.nkv = int(pf->nkv);
+  p.hd = int(pf->hd);
+  p.kh = pf->kh;
+  p.kl = pf->kl;
+  p.vth = pf->vth;
+  p.vtl = pf->vtl;
+  p.P = int(pf->P);
+  p.Pp = int(pf->Pp);
+  p.score_mult = pl->score_mult;
+  p.score_shift = pl->score_shift;
+  p.exp_lut = pl->d_lut;
+  p.exp_len = int32_t(pl->exp_len);
+  p.lut_shift = pl->lut_shift;
+  p.prob_frac = pl->prob_frac;
+  p.out_shift = pl->out_shift;
+}
+
+// y (int16, the projection's output) += the rows' adapters; the workspace is held.
+int run_adapter_shrink(myl_ctx* ctx, const myl_adapters* ad, AdapterParams& p, const int16_t* x, int64_t M,
+                       int64_t ldx, const int32_t* ids, cudaStream_t st) {
+  TRY(ensure(ctx->ad_h, size_t(M) * size_t(ad->ldb) * 2));
+  p = AdapterParams{ad->A, ad->B, ad->sa, ad->sb, int(ad->num), int(ad->rank), ad->K, ad->N, ad->lda, int(ad->ldb),
+                    ids, M, static_cast<int16_t*>(ctx->ad_h.p), ctx->d_err};
+  const int aligned = aligned16(x) && ldx % 8 == 0;
+  const unsigned blocks = unsigned(std::min<int64_t>((M * ad->ldb + 7) / 8, int64_t(ctx->num_sms) * 64));
+  LaunchCfg lc(ctx, dim3(blocks), dim3(256), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_shrink_kernel, x, ldx, aligned, p));
+  ctx->launches++;
+  return MYL_OK;
+}
+
+int run_adapter_expand(myl_ctx* ctx, const AdapterParams& p, int16_t* y, int64_t ldy, cudaStream_t st) {
+  LaunchCfg lc(ctx, dim3(unsigned((p.N + 255) / 256), unsigned(std::min<int64_t>(p.M, 65535))), dim3(256), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_expand_kernel, p, y, ldy));
+  ctx->launches++;
+  return MYL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int myl_attn_plan_create(myl_ctx* ctx, int64_t score_mult, uint8_t score_shift, const int16_t* exp_lut,
+                         int64_t exp_len, uint8_t lut_shift, uint8_t prob_frac_bits, int out_shift,
+                         myl_attn_plan** out) {
+  if (!ctx || !exp_lut || !out) return fail(MYL_ERR_ARG, "null argument");
+  *out = nullptr;
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  myl_attn_plan* pl = new myl_attn_plan();
+  const int rc =
+      attn_plan_build(pl, score_mult, score_shift, exp_lut, exp_len, lut_shift, prob_frac_bits, out_shift);
+  if (rc != MYL_OK) {
+    free_handle(ctx, pl);
+    return rc;
+  }
+  *out = pl;
+  return MYL_OK;
+}
+
+int myl_attn_plan_release(myl_ctx* ctx, myl_attn_plan* plan) {
+  if (plan) free_handle(ctx, plan);
+  return MYL_OK;
+}
+
+int myl_prefix_create(myl_ctx* ctx, const int16_t* k, const int16_t* v, int64_t positions, int64_t num_kv_heads,
+                      int64_t head_dim, int64_t pos_stride, int64_t head_stride, void* stream, myl_prefix** out) {
+  if (!ctx || !out || (positions > 0 && (!k || !v))) return fail(MYL_ERR_ARG, "null argument");
+  *out = nullptr;
+  if (positions < 0 || num_kv_heads <= 0 || head_dim <= 0 || pos_stride < head_dim || head_stride < 0)
+    return fail(MYL_ERR_SHAPE, "prefix of %lld positions, %lld heads of %lld", (long long)positions,
+                (long long)num_kv_heads, (long long)head_dim);
+  if (head_dim % 8 || head_dim > PFX_MAX_HD)
+    return fail(MYL_ERR_UNSUPPORTED, "head_dim %lld: a multiple of 8 up to %d", (long long)head_dim, PFX_MAX_HD);
+  if (positions > (1 << 30) || num_kv_heads > 65535)
+    return fail(MYL_ERR_UNSUPPORTED, "prefix beyond 2^30 positions or 65535 heads");
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  myl_prefix* pf = new myl_prefix();
+  pf->P = positions;
+  pf->Pp = (positions + PFX_PAD - 1) / PFX_PAD * PFX_PAD;
+  pf->nkv = num_kv_heads;
+  pf->hd = head_dim;
+  const int rc = prefix_build(ctx, pf, k, v, pos_stride, head_stride, static_cast<cudaStream_t>(stream));
+  if (rc != MYL_OK) {
+    free_handle(ctx, pf);
+    return rc;
+  }
+  *out = pf;
+  return MYL_OK;
+}
+
+int myl_prefix_release(myl_ctx* ctx, myl_prefix* prefix) {
+  if (prefix) free_handle(ctx, prefix);
+  return MYL_OK;
+}
+
+int64_t myl_prefix_positions(const myl_prefix* prefix) { return prefix ? prefix->P : -1; }
+
+int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_prefix* prefix, const int16_t* q,
+                             int64_t batch, int64_t T, int64_t num_heads, int64_t ldq, const int16_t* k_suffix,
+                             const int16_t* v_suffix, int64_t suffix_cap, int64_t seq_stride, int64_t head_stride,
+                             int64_t pos_stride, const int32_t* lens, int16_t* out, int64_t ldo, void* stream) {
+  if (!ctx || !plan || !prefix) return fail(MYL_ERR_ARG, "null argument");
+  if (batch < 0 || T < 0 || suffix_cap < 0) return fail(MYL_ERR_SHAPE, "negative batch, T or suffix capacity");
+  if (batch == 0 || T == 0) return MYL_OK;
+  if (!q || !out || !lens || (suffix_cap > 0 && (!k_suffix || !v_suffix))) return fail(MYL_ERR_ARG, "null argument");
+  const int64_t nkv = prefix->nkv, hd = prefix->hd;
+  if (num_heads <= 0 || num_heads % nkv)
+    return fail(MYL_ERR_SHAPE, "%lld query heads over %lld KV heads", (long long)num_heads, (long long)nkv);
+  if (ldq < num_heads * hd || ldo < num_heads * hd || (suffix_cap > 0 && (pos_stride < hd || head_stride < 0 || seq_stride < 0)))
+    return fail(MYL_ERR_SHAPE, "row or cache strides shorter than a row");
+  if (!aligned16(q) || ldq % 8 || (suffix_cap > 0 && (!aligned16(k_suffix) || pos_stride % 8 || head_stride % 8 || seq_stride % 8)))
+    return fail(MYL_ERR_UNSUPPORTED, "queries and suffix keys must lie on 16-byte boundaries (strides in multiples of 8)");
+  const int64_t keys = prefix->P + suffix_cap;
+  // softmax.rs:46: the i32 sum of up to `keys` exponentials
+  if (keys > INT32_MAX / 2 || int64_t(plan->exp_max) * keys > INT32_MAX)
+    return fail(MYL_ERR_OVERFLOW, "%lld keys overflow the softmax's i32 sum", (long long)keys);
+  const int64_t R = batch * T * (num_heads / nkv);
+  if (R > (1 << 24) || nkv * R > INT32_MAX || batch > 65535)
+    return fail(MYL_ERR_UNSUPPORTED, "%lld query rows in one call", (long long)(nkv * R));
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  PrefixParams p{};
+  prefix_params(p, plan, prefix);
+  p.q = q;
+  p.ldq = ldq;
+  p.B = int(batch);
+  p.T = int(T);
+  p.nq = int(num_heads);
+  p.G = int(num_heads / nkv);
+  p.R = int(R);
+  p.ks = k_suffix;
+  p.vs = v_suffix;
+  p.seq_stride = seq_stride;
+  p.head_stride = head_stride;
+  p.pos_stride = pos_stride;
+  p.S = int(suffix_cap);
+  p.lens = lens;
+  p.out = out;
+  p.ldo = ldo;
+  TRY(ws_acquire(ctx, st));
+  {
+    PdlScope pdl(ctx);
+    TRY(run_prefix_attention(ctx, p, st));
+  }
+  return ws_release(ctx, st);
+}
+
+int myl_adapters_register(myl_ctx* ctx, int64_t num, int64_t rank, int64_t in_features, int64_t out_features,
+                          const int8_t* A, const uint8_t* a_shifts, const int8_t* B, const uint8_t* b_shifts,
+                          uint8_t act_frac, uint8_t h_frac, uint8_t out_frac, myl_adapters** out) {
+  if (!ctx || !A || !a_shifts || !B || !b_shifts || !out) return fail(MYL_ERR_ARG, "null argument");
+  *out = nullptr;
+  if (num <= 0 || rank <= 0 || in_features <= 0 || out_features <= 0)
+    return fail(MYL_ERR_SHAPE, "adapters: %lld of rank %lld over [%lld][%lld]", (long long)num, (long long)rank,
+                (long long)out_features, (long long)in_features);
+  if (rank > 256 || num > (1 << 20) || in_features > (int64_t(1) << 31) || out_features > (int64_t(1) << 31))
+    return fail(MYL_ERR_UNSUPPORTED, "adapters: rank at most 256, at most 2^20 adapters");
+  std::vector<int8_t> sa, sb;
+  try {
+    sa.resize(size_t(num * rank));
+    sb.resize(size_t(num * out_features));
+  } catch (const std::exception&) {
+    return fail(MYL_ERR_UNSUPPORTED, "out of host memory for %lld adapters", (long long)num);
+  }
+  for (size_t i = 0; i < sa.size(); ++i) TRY(signed_total_shift(a_shifts[i], act_frac, h_frac, &sa[i]));
+  for (size_t i = 0; i < sb.size(); ++i) TRY(signed_total_shift(b_shifts[i], h_frac, out_frac, &sb[i]));
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  myl_adapters* ad = new myl_adapters();
+  ad->num = num;
+  ad->rank = rank;
+  ad->K = in_features;
+  ad->N = out_features;
+  ad->lda = round_up16(in_features);
+  ad->ldb = round_up16(rank);
+  auto upload = [&](int8_t** d, const int8_t* h, int64_t rows, int64_t cols, int64_t ld) -> int {
+    TRY(dev_alloc(ad->allocs, d, size_t(rows * ld)));
+    CUDA_TRY(cudaMemset(*d, 0, size_t(rows * ld)));
+    CUDA_TRY(cudaMemcpy2D(*d, size_t(ld), h, size_t(cols), size_t(cols), size_t(rows), cudaMemcpyHostToDevice));
+    return MYL_OK;
+  };
+  int rc = upload(&ad->A, A, num * rank, in_features, ad->lda);
+  if (rc == MYL_OK) rc = upload(&ad->B, B, num * out_features, rank, ad->ldb);
+  if (rc == MYL_OK) rc = dev_upload(ad->allocs, &ad->sa, sa.data(), sa.size());
+  if (rc == MYL_OK) rc = dev_upload(ad->allocs, &ad->sb, sb.data(), sb.size());
+  if (rc != MYL_OK) {
+    free_handle(ctx, ad);
+    return rc;
+  }
+  *out = ad;
+  return MYL_OK;
+}
+
+int myl_adapters_release(myl_ctx* ctx, myl_adapters* adapters) {
+  if (adapters) free_handle(ctx, adapters);
+  return MYL_OK;
+}
+
+int myl_linear_adapters_dev(myl_ctx* ctx, const myl_weight* w, const myl_requant* rq, const myl_adapters* ad,
+                            const int16_t* x, int64_t M, int64_t ldx, const int32_t* ids, int16_t* y, int64_t ldy,
+                            void* stream) {
+  if (!ctx || !w || !rq || !ad || (M > 0 && (!x || !y || !ids))) return fail(MYL_ERR_ARG, "null argument");
+  if (w->w16 || rq->mode == MYL_RQ_SHIFT_I32)
+    return fail(MYL_ERR_ARG, "adapters take an int8 weight with an int16 requant");
+  if (rq->N != w->N) return fail(MYL_ERR_SHAPE, "requant has %lld channels, weight %lld", (long long)rq->N, (long long)w->N);
+  if (ad->K != w->K || ad->N != w->N)
+    return fail(MYL_ERR_SHAPE, "adapters are [%lld][%lld], the weight [%lld][%lld]", (long long)ad->N, (long long)ad->K,
+                (long long)w->N, (long long)w->K);
+  if (M < 0 || ldx < w->K || ldy < w->N) return fail(MYL_ERR_SHAPE, "bad M/ldx/ldy");
+  if (M == 0) return MYL_OK;
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TRY(ws_acquire(ctx, st));
+  {
+    PdlScope pdl(ctx);
+    AdapterParams p;
+    TRY(run_adapter_shrink(ctx, ad, p, x, M, ldx, ids, st));
+    TRY(dispatch_linear(ctx, w, x, M, ldx, make_ep(rq, y, ldy), st));
+    TRY(run_adapter_expand(ctx, p, y, ldy, st));
+  }
+  return ws_release(ctx, st);
+}
+
+int myl_verifier_create(myl_ctx* ctx, const int16_t* exp_lut, int64_t exp_len, uint32_t temp_mult,
+                        uint8_t temp_shift, myl_verifier** out) {
+  if (!ctx || !exp_lut || !out) return fail(MYL_ERR_ARG, "null argument");
+  *out = nullptr;
+  if (temp_shift > 62) return fail(MYL_ERR_OVERFLOW, "temperature shift %u", unsigned(temp_shift));
+  if (temp_mult == 0) return fail(MYL_ERR_ARG, "temperature multiplier 0");
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  myl_verifier* v = new myl_verifier();
+  v->len = exp_len;
+  v->mult = temp_mult;
+  v->shift = temp_shift;
+  int rc = check_exp_lut(exp_lut, exp_len, &v->max);
+  if (rc == MYL_OK) rc = dev_upload(v->allocs, &v->d_lut, exp_lut, size_t(exp_len));
+  if (rc != MYL_OK) {
+    free_handle(ctx, v);
+    return rc;
+  }
+  *out = v;
+  return MYL_OK;
+}
+
+int myl_verifier_release(myl_ctx* ctx, myl_verifier* verifier) {
+  if (verifier) free_handle(ctx, verifier);
+  return MYL_OK;
+}
+
+int myl_verify_dev(myl_ctx* ctx, const myl_verifier* v, const int32_t* target, int64_t target_seq_stride,
+                   int64_t target_pos_stride, const int32_t* draft, int64_t draft_seq_stride, int64_t draft_pos_stride,
+                   int64_t batch, int64_t drafted, int64_t vocab, const int32_t* tokens, const int32_t* counts,
+                   const uint64_t* rand, int32_t* accepted, int32_t* out_tokens, void* stream) {
+  if (!ctx || !v) return fail(MYL_ERR_ARG, "null argument");
+  if (batch < 0 || drafted < 0 || vocab <= 0) return fail(MYL_ERR_SHAPE, "batch, drafted or vocab");
+  if (batch == 0) return MYL_OK;
+  if (!target || !rand || !accepted || !out_tokens || (drafted > 0 && !tokens)) return fail(MYL_ERR_ARG, "null argument");
+  if ((drafted > 0 && target_pos_stride < vocab) || target_seq_stride < 0 ||
+      (draft && (draft_pos_stride < vocab || draft_seq_stride < 0)))
+    return fail(MYL_ERR_SHAPE, "logit rows shorter than the vocabulary");
+  // weights sums below 2^32, so that products of two fit 64 bits
+  if (int64_t(v->max) * vocab >= (int64_t(1) << 32))
+    return fail(MYL_ERR_OVERFLOW, "%lld table weights of up to %d overflow 32 bits", (long long)vocab, v->max);
+  if (drafted > 1024 || batch > (1 << 20)) return fail(MYL_ERR_UNSUPPORTED, "at most 1024 drafted tokens, 2^20 requests");
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (drafted == 0) draft = nullptr;
+  VerifyParams p{};
+  p.target = target;
+  p.ts_b = target_seq_stride;
+  p.ts_d = target_pos_stride;
+  p.draft = draft;
+  p.ds_b = draft_seq_stride;
+  p.ds_d = draft_pos_stride;
+  p.tokens = tokens;
+  p.counts = counts;
+  p.rand = rand;
+  p.B = int(batch);
+  p.D = int(drafted);
+  p.V = int(vocab);
+  p.lut = v->d_lut;
+  p.lut_len = int32_t(v->len);
+  p.mult = v->mult;
+  p.shift = v->shift;
+  p.accepted = accepted;
+  p.out = out_tokens;
+  p.err = ctx->d_err;
+  TRY(ws_acquire(ctx, st));
+  const int64_t rows = batch * (2 * drafted + 1);
+  TRY(ensure(ctx->vfy, size_t(rows) * 12));
+  p.rsum = static_cast<uint64_t*>(ctx->vfy.p);
+  p.rmax = reinterpret_cast<int32_t*>(p.rsum + rows);
+  {
+    PdlScope pdl(ctx);
+    LaunchCfg l1(ctx, dim3(unsigned(batch * (drafted + 1 + (draft ? drafted : 0)))), dim3(VERIFY_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, verify_stats_kernel, p));
+    LaunchCfg l2(ctx, dim3(unsigned(batch)), dim3(VERIFY_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, verify_sample_kernel, p));
+    ctx->launches += 2;
+  }
+  return ws_release(ctx, st);
+}
+
+}  // extern "C"

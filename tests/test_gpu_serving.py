@@ -1,0 +1,532 @@
+"""The serving operators on the GPU against their plain 64-bit forms
+(serving_ref.py). Every result is one exact integer, so every comparison is
+for equality."""
+import numpy as np
+import pytest
+
+import serving_ref as R
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import myelith_b200 as myl  # noqa: E402
+
+DEVICE_ERR = myl.MYL_ERR_DEVICE
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    c = myl.Context(0)
+    yield c
+    c.close()
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def int16s(rng, shape, sigma):
+    return np.clip(np.rint(rng.normal(0, sigma, size=shape)), -32768, 32767).astype(np.int16)
+
+
+# ---- attention over a shared prefix ------------------------------------------------
+
+PLAN = dict(score_mult=2896, score_shift=23, exp_lut=R.EXP_LUT, lut_shift=6, prob_frac=14, out_shift=-1)
+
+
+def make_plan(ctx, c):
+    return myl.AttentionPlan(ctx, c["score_mult"], c["score_shift"], c["exp_lut"], c["lut_shift"], c["prob_frac"],
+                             c["out_shift"])
+
+
+def attention_problem(rng, B, T, nq, nkv, hd, P, S, sigma=3000.0):
+    return dict(q=int16s(rng, (B, T, nq, hd), sigma), k=int16s(rng, (nkv, P, hd), sigma),
+                v=int16s(rng, (nkv, P, hd), 9000.0), ks=int16s(rng, (B, nkv, S, hd), sigma),
+                vs=int16s(rng, (B, nkv, S, hd), 9000.0))
+
+
+def run_attention(ctx, x, lens, c):
+    plan, prefix = make_plan(ctx, c), myl.Prefix(ctx, dev(x["k"]), dev(x["v"]))
+    B, T, nq, hd = x["q"].shape
+    out = torch.full((B, T, nq * hd), 77, dtype=torch.int16, device="cuda")
+    prefix.attention_dev(plan, dev(x["q"]), dev(x["ks"]), dev(x["vs"]), dev(np.asarray(lens, np.int32)), out)
+    torch.cuda.synchronize()
+    return out.cpu().numpy()
+
+
+def check_attention(ctx, x, lens, c=PLAN):
+    got = run_attention(ctx, x, lens, c)
+    ctx.synchronize()
+    ref = R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **c)
+    assert np.array_equal(got, ref), f"{(got != ref).sum()} of {ref.size} differ"
+
+
+@pytest.mark.parametrize("B,T,nq,nkv,hd,P,S", [
+    (1, 1, 1, 1, 8, 1, 1),            # smallest
+    (1, 1, 14, 2, 64, 509, 65),       # 0.5B heads
+    (2, 1, 28, 4, 128, 700, 33),      # 7B heads
+    (3, 5, 4, 2, 128, 127, 40),       # drafted tokens, prefix one short of a block
+    (2, 3, 8, 1, 64, 128, 17),        # one block exactly
+    (2, 2, 6, 3, 64, 129, 9),         # one past a block
+    (5, 4, 14, 2, 64, 1030, 31),      # rows past one row tile per KV head
+    (21, 1, 28, 4, 128, 333, 20),
+    (40, 4, 7, 1, 128, 260, 12),      # several row tiles, the last ragged
+    (2, 1, 4, 4, 24, 50, 10),         # head sizes outside the tile sizes
+    (1, 2, 6, 2, 248, 300, 35),
+    (1, 1, 28, 4, 128, 4099, 3),      # longer prefixes
+    (2, 9, 14, 2, 64, 2500, 77),
+])
+def test_prefix_attention(ctx, B, T, nq, nkv, hd, P, S):
+    rng = np.random.default_rng(B * 1000 + P + hd)
+    x = attention_problem(rng, B, T, nq, nkv, hd, P, S)
+    lens = rng.integers(min(T, S), S + 1, size=B)
+    lens[0] = S
+    check_attention(ctx, x, lens)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [1, 150])
+def test_prefix_attention_extreme_values(ctx, hd, rows):
+    """Rows of the type's lowest and highest values, scores that wrap i32, ties and equal rows."""
+    rng = np.random.default_rng(hd + rows)
+    x = attention_problem(rng, rows, 1, 2, 1, hd, 200, 8)
+    x["q"][0] = -32768
+    x["k"][0, :50] = -32768
+    x["k"][0, 50:60] = 32767
+    x["v"][0, ::3] = -32768
+    x["v"][0, 1::3] = 32767
+    x["ks"][:, :, 2] = x["k"][:, 7][None]
+    lens = rng.integers(1, 9, size=rows)
+    check_attention(ctx, x, lens)
+    check_attention(ctx, x, lens, {**PLAN, "score_shift": 0})           # i32 wrap-around
+    check_attention(ctx, x, lens, {**PLAN, "score_mult": -2896})
+    check_attention(ctx, x, lens, {**PLAN, "score_shift": 40})          # nearly equal scores: ties
+    check_attention(ctx, x, lens, {**PLAN, "score_shift": 62, "score_mult": 2**40 + 12345})
+    x["q"][:] = 0
+    check_attention(ctx, x, lens)  # all scores equal
+
+
+@pytest.mark.parametrize("change", [
+    dict(prob_frac=0), dict(prob_frac=15), dict(prob_frac=1, lut_shift=0), dict(out_shift=0), dict(out_shift=3),
+    dict(out_shift=-5), dict(out_shift=30), dict(lut_shift=31), dict(score_mult=0),
+    dict(exp_lut=np.array([256, 128, 64], np.int16)), dict(exp_lut=np.array([1], np.int16)),
+    dict(exp_lut=np.array([3, 32767, 0, 9, 500], np.int16), prob_frac=15, lut_shift=10),  # not decreasing
+])
+@pytest.mark.parametrize("B", [1, 70])
+def test_prefix_attention_plans(ctx, change, B):
+    rng = np.random.default_rng(7)
+    x = attention_problem(rng, B, 2, 4, 2, 64, 190, 12)
+    check_attention(ctx, x, rng.integers(2, 13, size=B), {**PLAN, **change})
+
+
+def test_prefix_attention_empty_rows_and_lengths(ctx):
+    """No prefix, no suffix entries, fewer entries than new tokens, neither."""
+    rng = np.random.default_rng(3)
+    x = attention_problem(rng, 4, 3, 4, 2, 64, 0, 6)
+    check_attention(ctx, x, [0, 1, 2, 6])  # rows without any key give zeros
+    x = attention_problem(rng, 4, 3, 4, 2, 64, 65, 6)
+    check_attention(ctx, x, [0, 1, 3, 6])
+    x = attention_problem(rng, 2, 1, 4, 2, 64, 65, 0)
+    check_attention(ctx, x, [0, 0])
+    x = attention_problem(rng, 2, 1, 4, 2, 64, 0, 0)
+    check_attention(ctx, x, [0, 0])
+    plan, prefix = make_plan(ctx, PLAN), myl.Prefix(ctx, dev(x["k"]), dev(x["v"]))
+    none = torch.zeros((0, 1, 4, 64), dtype=torch.int16, device="cuda")
+    cache = torch.zeros((0, 2, 5, 64), dtype=torch.int16, device="cuda")
+    prefix.attention_dev(plan, none, cache, cache, torch.zeros(0, dtype=torch.int32, device="cuda"),
+                         torch.zeros((0, 1, 256), dtype=torch.int16, device="cuda"))
+    ctx.synchronize()
+
+
+@pytest.mark.parametrize("B", [2, 40])
+def test_prefix_attention_strides_and_streams(ctx, B):
+    """Queries inside fused q/k/v rows, caches inside larger ones, position-major
+    prefixes, a padded output, a stream of its own."""
+    rng = np.random.default_rng(11)
+    T, nq, nkv, hd, P, S = 2, 4, 2, 64, 150, 10
+    x = attention_problem(rng, B, T, nq, nkv, hd, P, S)
+    lens = rng.integers(T, S + 1, size=B)
+    ref = R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **PLAN)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        qkv = torch.full((B, T, nq + 2 * nkv, hd), -9, dtype=torch.int16, device="cuda")
+        qkv[:, :, :nq] = dev(x["q"])
+        kp, vp = (dev(x[n].transpose(1, 0, 2)).permute(1, 0, 2) for n in ("k", "v"))  # [P][nkv][hd] in memory
+        big = torch.full((2, B, 3, nkv, S + 4, hd), 5, dtype=torch.int16, device="cuda")
+        big[0, :, 1, :, :S], big[1, :, 1, :, :S] = dev(x["ks"]), dev(x["vs"])
+        out = torch.full((B, T, nq * hd + 24), 77, dtype=torch.int16, device="cuda")
+        prefix = myl.Prefix(ctx, kp, vp)
+        kp.fill_(1)  # the prefix holds its own copy
+        for _ in range(2):
+            prefix.attention_dev(make_plan(ctx, PLAN), qkv[:, :, :nq], big[0, :, 1, :, :S], big[1, :, 1, :, :S],
+                                 dev(lens.astype(np.int32)), out[:, :, : nq * hd])
+    s.synchronize()
+    assert np.array_equal(out[:, :, : nq * hd].cpu().numpy(), ref)
+    assert (out[:, :, nq * hd:] == 77).all()
+
+
+def test_prefix_attention_batch_equals_single_requests(ctx):
+    """A batch gives what each request gives alone, whatever kernels its size selects."""
+    rng = np.random.default_rng(5)
+    x = attention_problem(rng, 48, 1, 28, 4, 128, 1500, 20)
+    lens = rng.integers(1, 21, size=48)
+    got = run_attention(ctx, x, lens, PLAN)
+    for b in (0, 17, 47):
+        one = run_attention(ctx, {**x, "q": x["q"][b:b + 1], "ks": x["ks"][b:b + 1], "vs": x["vs"][b:b + 1]},
+                            lens[b:b + 1], PLAN)
+        assert np.array_equal(one[0], got[b])
+    ref = R.prefix_attention(x["q"][:1], x["k"], x["v"], x["ks"][:1], x["vs"][:1], lens[:1], **PLAN)
+    assert np.array_equal(got[:1], ref)
+
+
+def test_prefix_attention_rejects(ctx):
+    rng = np.random.default_rng(1)
+    x = attention_problem(rng, 2, 1, 4, 2, 64, 20, 8)
+    with pytest.raises(myl.MylError):
+        make_plan(ctx, {**PLAN, "prob_frac": 16})
+    with pytest.raises(myl.MylError):
+        make_plan(ctx, {**PLAN, "score_shift": 63})
+    with pytest.raises(myl.MylError):
+        make_plan(ctx, {**PLAN, "out_shift": 31})
+    for lut in ([], [0, 5], [5, -1]):
+        with pytest.raises(myl.MylError):
+            make_plan(ctx, {**PLAN, "exp_lut": np.array(lut, np.int16)})
+    with pytest.raises(myl.MylError):  # 32767 << 15 stays inside i32, but not the sum of 70000 keys
+        big = torch.zeros((1, 70000, 8), dtype=torch.int16, device="cuda")
+        c = torch.zeros((1, 1, 1, 8), dtype=torch.int16, device="cuda")
+        myl.Prefix(ctx, big, big).attention_dev(
+            make_plan(ctx, {**PLAN, "exp_lut": np.array([32767], np.int16)}), c, c, c,
+            torch.ones(1, dtype=torch.int32, device="cuda"), torch.zeros((1, 1, 8), dtype=torch.int16, device="cuda"))
+    with pytest.raises(myl.MylError):  # head_dim 20
+        z = torch.zeros((1, 4, 20), dtype=torch.int16, device="cuda")
+        myl.Prefix(ctx, z, z)
+    with pytest.raises(myl.MylError):
+        myl.Prefix(ctx, dev(x["k"]).int(), dev(x["v"]))
+    plan, prefix = make_plan(ctx, PLAN), myl.Prefix(ctx, dev(x["k"]), dev(x["v"]))
+    q, ks, vs, lens = dev(x["q"]), dev(x["ks"]), dev(x["vs"]), dev(np.array([3, 8], np.int32))
+    out = torch.zeros((2, 1, 256), dtype=torch.int16, device="cuda")
+    for bad in (dict(q=q[:, :, :3]), dict(q=q.cpu()), dict(q=q[..., :32]), dict(lens=lens[:1]), dict(lens=lens.long()),
+                dict(out=out[:, :, :255]), dict(vs=vs[:, :, :7])):
+        a = {**dict(q=q, ks=ks, vs=vs, lens=lens, out=out), **bad}
+        with pytest.raises(myl.MylError):
+            prefix.attention_dev(plan, a["q"], a["ks"], a["vs"], a["lens"], a["out"])
+    wide = torch.zeros((2, 1, 4, 72), dtype=torch.int16, device="cuda")
+    with pytest.raises(myl.MylError):  # queries off 16-byte boundaries
+        prefix.attention_dev(plan, wide.view(-1)[4:4 + 512].view(2, 1, 4, 64), ks, vs, lens, out)
+    # lengths outside the capacity: clamped, and reported at the next check
+    prefix.attention_dev(plan, q, ks, vs, dev(np.array([9, -1], np.int32)), out)
+    with pytest.raises(myl.MylError) as e:
+        torch.cuda.synchronize()
+        ctx.synchronize()
+    assert e.value.code == DEVICE_ERR
+    ref = R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], [8, 0], **PLAN)
+    assert np.array_equal(out.cpu().numpy(), ref)
+    ctx.synchronize()  # the context stays usable
+
+
+# ---- low-rank adapters ----------------------------------------------------------------
+
+def adapter_problem(rng, M, K, N, r, num, full=False):
+    lo, hi = (-128, 128) if full else (-127, 128)
+    kb = int(round(np.log2(73.6 * np.sqrt(K))))
+    rb = int(round(np.log2(73.6 * np.sqrt(r))))
+    return dict(x=int16s(rng, (M, K), 1024.0), W=rng.integers(lo, hi, size=(N, K)).astype(np.int8),
+                ws=(kb + rng.integers(-1, 2, size=N)).astype(np.uint8),
+                A=rng.integers(lo, hi, size=(num, r, K)).astype(np.int8),
+                sa=(kb + rng.integers(-1, 2, size=(num, r))).astype(np.uint8),
+                B=rng.integers(lo, hi, size=(num, N, r)).astype(np.int8),
+                sb=(rb + rng.integers(-1, 3, size=(num, N))).astype(np.uint8))
+
+
+def run_adapters(ctx, p, ids, fr=(8, 8, 8), x=None, y=None, out_frac=8, bias=None, stream=None):
+    w = myl.Weight(ctx, p["W"], p["W"].shape[1], p["ws"])
+    rq = w.requant(myl.RQ_SHIFT_I16, 8, out_frac)
+    if bias is not None:
+        rq.set_bias(bias[0], bias[1], out_frac)
+    ad = myl.Adapters(ctx, p["A"], p["sa"], p["B"], p["sb"], *fr)
+    x = dev(p["x"]) if x is None else x
+    y = torch.full((x.shape[0], p["W"].shape[0]), 77, dtype=torch.int16, device="cuda") if y is None else y
+    w.linear_adapters_dev(rq, ad, x, dev(np.asarray(ids, np.int32)), y, stream)
+    torch.cuda.synchronize()
+    return y.cpu().numpy()
+
+
+def adapter_ref(p, ids, fr=(8, 8, 8), out_frac=8, bias=None):
+    return R.linear_adapters(p["x"], p["W"], p["ws"], 8, out_frac, p["A"], p["sa"], p["B"], p["sb"], ids, *fr,
+                             bias=None if bias is None else bias[0], bias_shifts=None if bias is None else bias[1])
+
+
+@pytest.mark.parametrize("M,K,N,r,num", [
+    (1, 16, 8, 1, 1), (1, 896, 896, 16, 3), (2, 100, 77, 3, 2), (3, 1000, 129, 8, 4), (4, 4864, 300, 24, 2),
+    (5, 896, 640, 64, 6), (13, 333, 65, 17, 5), (64, 512, 384, 32, 9), (65, 512, 257, 16, 70), (130, 896, 512, 128, 3),
+    (300, 640, 130, 256, 2), (257, 18944, 64, 8, 2), (1, 18944, 130, 64, 2), (2, 1, 3, 2, 2),
+])
+def test_linear_adapters(ctx, M, K, N, r, num):
+    rng = np.random.default_rng(M + K + r)
+    p = adapter_problem(rng, M, K, N, r, num)
+    ids = rng.integers(-1, num, size=M)
+    ids[0] = num - 1
+    got = run_adapters(ctx, p, ids)
+    ctx.synchronize()
+    assert np.array_equal(got, adapter_ref(p, ids))
+    # one request's rows side by side (a prompt), then none with an adapter
+    ids = np.sort(rng.integers(-1, num, size=M))[::-1].copy()
+    assert np.array_equal(run_adapters(ctx, p, ids), adapter_ref(p, ids))
+    ids[:] = -1
+    assert np.array_equal(run_adapters(ctx, p, ids), adapter_ref(p, ids))
+
+
+@pytest.mark.parametrize("M", [1, 4, 9, 200])
+def test_linear_adapters_extremes_bias_and_fracs(ctx, M):
+    """Saturated rows, -128 weights, a bias, a per-channel output, left shifts."""
+    rng = np.random.default_rng(M)
+    p = adapter_problem(rng, M, 600, 200, 16, 3, full=True)
+    p["x"][0] = 32767
+    p["A"][1] = 127
+    p["A"][2] = -128
+    p["B"][1, ::2] = -128
+    ids = rng.integers(0, 3, size=M)
+    ids[0] = 1
+    bias = (rng.integers(-30000, 30000, size=200).astype(np.int16), rng.integers(6, 10, size=200).astype(np.uint8))
+    assert np.array_equal(run_adapters(ctx, p, ids, bias=bias), adapter_ref(p, ids, bias=bias))
+    of = rng.integers(4, 12, size=200).astype(np.uint8)
+    assert np.array_equal(run_adapters(ctx, p, ids, out_frac=of), adapter_ref(p, ids, out_frac=of))
+    p["sa"][:], p["sb"][:] = 0, 0
+    for fr in ((8, 8, 8), (0, 6, 12), (20, 3, 3), (62, 0, 0), (0, 0, 40)):
+        assert np.array_equal(run_adapters(ctx, p, ids, fr), adapter_ref(p, ids, fr)), fr
+
+
+@pytest.mark.parametrize("M", [1, 3, 40])
+def test_linear_adapters_strides_and_stream(ctx, M):
+    rng = np.random.default_rng(M)
+    K, N = 203, 90
+    p = adapter_problem(rng, M, K, N, 8, 4)
+    ids = rng.integers(-1, 4, size=M)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        xs = torch.full((M, K + 5), 3, dtype=torch.int16, device="cuda")  # rows off 16-byte boundaries
+        xs[:, 1:K + 1] = dev(p["x"])
+        ys = torch.full((M, N + 3), 77, dtype=torch.int16, device="cuda")
+        got = run_adapters(ctx, p, ids, x=xs[:, 1:K + 1], y=ys[:, 1:N + 1])
+    assert np.array_equal(got, adapter_ref(p, ids))
+    assert (ys[:, 0] == 77).all() and (ys[:, N + 1:] == 77).all()
+
+
+def test_linear_adapters_rejects(ctx):
+    rng = np.random.default_rng(2)
+    p = adapter_problem(rng, 3, 64, 32, 4, 2)
+    with pytest.raises(myl.MylError):
+        run_adapters(ctx, {**p, "sa": np.full((2, 4), 250, np.uint8)}, [0, 0, 0])
+    with pytest.raises(myl.MylError):
+        run_adapters(ctx, {**p, "B": p["B"][:, :, :3]}, [0, 0, 0])
+    with pytest.raises(myl.MylError):
+        myl.Adapters(ctx, np.zeros((1, 257, 8), np.int8), np.zeros((1, 257)), np.zeros((1, 4, 257), np.int8),
+                     np.zeros((1, 4)), 0, 0, 0)
+    with pytest.raises(myl.MylError):
+        run_adapters(ctx, {**p, "W": p["W"][:16], "ws": p["ws"][:16]}, [0, 0, 0])
+    with pytest.raises(myl.MylError):
+        run_adapters(ctx, p, [0, 0])
+    w = myl.Weight(ctx, p["W"], 64, p["ws"])
+    ad = myl.Adapters(ctx, p["A"], p["sa"], p["B"], p["sb"], 8, 8, 8)
+    with pytest.raises(myl.MylError):  # an int32 requant
+        w.linear_adapters_dev(w.requant(myl.RQ_SHIFT_I32, 8, 8), ad, dev(p["x"]), dev(np.zeros(3, np.int32)),
+                              torch.zeros((3, 32), dtype=torch.int16, device="cuda"))
+    for M, ids in ((3, [0, 2, -1]), (3, [1, -2, 0])):
+        got = run_adapters(ctx, p, ids)  # an unknown id adds nothing and is reported
+        with pytest.raises(myl.MylError) as e:
+            ctx.synchronize()
+        assert e.value.code == DEVICE_ERR
+        assert np.array_equal(got, adapter_ref(p, [a if 0 <= a < 2 else -1 for a in ids]))
+    ctx.synchronize()
+
+
+# ---- verification of drafted tokens -------------------------------------------------------
+
+def verify_problem(rng, B, D, V, sigma=200.0, noise=60.0, dist=True):
+    t = np.rint(rng.normal(0, sigma, size=(B, D + 1, V))).astype(np.int32)
+    d = (t[:, :D] + np.rint(rng.normal(0, noise, size=(B, D, V)))).astype(np.int32)
+    # likely tokens mostly, any token at times
+    tok = np.argmax(d + rng.gumbel(size=d.shape) * 64, axis=-1).astype(np.int32) if D else np.zeros((B, 0), np.int32)
+    odd = rng.random((B, D)) < 0.1
+    tok[odd] = rng.integers(0, V, size=int(odd.sum()))
+    rand = rng.integers(0, 2**64, size=(B, D + 1), dtype=np.uint64).view(np.int64)
+    return dict(target=t, draft=d if dist else None, tokens=tok, rand=rand)
+
+
+def run_verify(ctx, p, counts=None, lut=R.EXP_LUT, mult=4, shift=0, target=None, draft=None):
+    B, D1, V = p["target"].shape
+    v = myl.DraftVerifier(ctx, lut, mult, shift)
+    acc = torch.full((B,), 77, dtype=torch.int32, device="cuda")
+    out = torch.full((B, D1), 77, dtype=torch.int32, device="cuda")
+    t = dev(p["target"]) if target is None else target
+    d = draft if draft is not None else None if p["draft"] is None else dev(p["draft"])
+    v.verify_dev(t, d, dev(p["tokens"]), None if counts is None else dev(np.asarray(counts, np.int32)),
+                 dev(p["rand"]), acc, out)
+    torch.cuda.synchronize()
+    return acc.cpu().numpy(), out.cpu().numpy()
+
+
+def check_verify(ctx, p, counts=None, lut=R.EXP_LUT, mult=4, shift=0):
+    got = run_verify(ctx, p, counts, lut, mult, shift)
+    ctx.synchronize()
+    ref = R.verify(p["target"], p["draft"], p["tokens"], counts, p["rand"], lut, mult, shift)
+    assert np.array_equal(got[0], ref[0]) and np.array_equal(got[1], ref[1])
+    return ref
+
+
+@pytest.mark.parametrize("dist", [True, False])
+@pytest.mark.parametrize("B,D,V", [
+    (1, 0, 5), (1, 1, 1), (1, 1, 2), (3, 2, 31), (40, 3, 64), (7, 5, 997), (2, 4, 4096), (5, 1, 32003), (9, 2, 19007),
+    (2, 3, 151936), (1, 1, 152063), (33, 1, 1025),
+])
+def test_verify(ctx, B, D, V, dist):
+    rng = np.random.default_rng(B * 100 + D + V)
+    p = verify_problem(rng, B, D, V, dist=dist)
+    check_verify(ctx, p)
+    check_verify(ctx, p, counts=rng.integers(0, D + 1, size=B), mult=int(4 / 0.7 * 65536), shift=16)
+
+
+def test_verify_covers_every_outcome(ctx):
+    rng = np.random.default_rng(8)
+    p = verify_problem(rng, 200, 3, 50, sigma=100.0, noise=40.0)
+    acc, _ = check_verify(ctx, p)
+    assert set(acc.tolist()) == {0, 1, 2, 3}
+
+
+def test_verify_random_words_and_ties(ctx):
+    """Words of all zeros and all ones, equal distributions, equal logits, certain targets."""
+    rng = np.random.default_rng(9)
+    p = verify_problem(rng, 6, 2, 300)
+    for word in (0, -1, 0xFFFFFFFF, -2**32):
+        p["rand"][:] = word
+        check_verify(ctx, p)
+        check_verify(ctx, {**p, "draft": None})
+    same = {**p, "draft": p["target"][:, :2].copy()}
+    check_verify(ctx, same)
+    flat = {**p, "target": np.zeros_like(p["target"]), "draft": np.zeros_like(p["draft"])}
+    check_verify(ctx, flat)
+    one = {**flat, "target": flat["target"].copy()}
+    one["target"][:, :, 7] = 2**30  # all weight on token 7
+    one["tokens"] = np.full((6, 2), 7, np.int32)
+    check_verify(ctx, one)
+    check_verify(ctx, {**one, "draft": None})
+    one["tokens"][:] = 8  # a token without target weight
+    check_verify(ctx, one)
+    check_verify(ctx, {**one, "draft": one["target"][:, :2].copy()})  # without draft weight either: nothing is left
+
+
+def test_verify_extreme_logits_and_tables(ctx):
+    rng = np.random.default_rng(10)
+    p = verify_problem(rng, 5, 2, 500)
+    p["target"][0, 0, 3], p["target"][0, 0, 9] = 2**31 - 1, -2**31
+    p["target"][1, 0, :] = -2**31
+    p["draft"][1, 0, :] = -2**31
+    p["draft"][2, 1, 5] = 2**31 - 1
+    check_verify(ctx, p)
+    check_verify(ctx, p, mult=2**32 - 1, shift=62)  # nearly flat
+    check_verify(ctx, p, mult=2**32 - 1, shift=0)   # the maximum alone
+    check_verify(ctx, p, lut=np.array([1], np.int16))
+    check_verify(ctx, p, lut=np.array([3, 32767, 0, 5], np.int16), mult=1, shift=5)
+
+
+def test_verify_strides_and_empty_batch(ctx):
+    rng = np.random.default_rng(12)
+    p = verify_problem(rng, 4, 3, 701)
+    ref = R.verify(p["target"], p["draft"], p["tokens"], None, p["rand"], R.EXP_LUT, 4, 0)
+    for lead in (0, 1, 3):  # rows on every 4-byte boundary
+        t = torch.full((4, 4, 720), 2**31 - 1, dtype=torch.int32, device="cuda")
+        d = torch.full((4, 3, 711), 2**31 - 1, dtype=torch.int32, device="cuda")
+        t[:, :, lead:lead + 701], d[:, :, lead:lead + 701] = dev(p["target"]), dev(p["draft"])
+        got = run_verify(ctx, p, target=t[:, :, lead:lead + 701], draft=d[:, :, lead:lead + 701])
+        assert np.array_equal(got[0], ref[0]) and np.array_equal(got[1], ref[1])
+    # one prompt's logits for every request (a broadcast batch)
+    t = dev(p["target"][:1]).expand(4, 4, 701)
+    got = run_verify(ctx, p, target=t)
+    ref = R.verify(np.broadcast_to(p["target"][:1], (4, 4, 701)), p["draft"], p["tokens"], None, p["rand"], R.EXP_LUT,
+                   4, 0)
+    assert np.array_equal(got[0], ref[0]) and np.array_equal(got[1], ref[1])
+    run_verify(ctx, verify_problem(rng, 0, 2, 10))
+
+
+def test_verify_rejects(ctx):
+    rng = np.random.default_rng(13)
+    p = verify_problem(rng, 3, 2, 40)
+    for lut in ([], [0, 1], [4, -1]):
+        with pytest.raises(myl.MylError):
+            myl.DraftVerifier(ctx, np.array(lut, np.int16), 4, 0)
+    for mult, shift in ((0, 0), (2**32, 0), (-1, 0), (1, 63)):
+        with pytest.raises(myl.MylError):
+            myl.DraftVerifier(ctx, R.EXP_LUT, mult, shift)
+    with pytest.raises(myl.MylError):  # 2^14 * 262144 = 2^32
+        run_verify(ctx, dict(target=np.zeros((1, 1, 262144), np.int32), draft=None, tokens=np.zeros((1, 0), np.int32),
+                             rand=np.zeros((1, 1), np.int64)))
+    for bad in (dict(tokens=p["tokens"][:, :1]), dict(rand=p["rand"][:2]), dict(draft=p["draft"][:, :, :39]),
+                dict(target=p["target"].astype(np.int64))):
+        with pytest.raises(myl.MylError):
+            run_verify(ctx, {**p, **bad})
+    # tokens outside the vocabulary and counts outside [0, D]: defined results, reported
+    odd = {**p, "tokens": np.array([[40, 1], [0, -1], [2, 3]], np.int32)}
+    for dist in (odd["draft"], None):
+        q = {**odd, "draft": dist}
+        got = run_verify(ctx, q, counts=[2, 2, 2])
+        ref = R.verify(q["target"], q["draft"], q["tokens"], [2, 2, 2], q["rand"], R.EXP_LUT, 4, 0)
+        assert np.array_equal(got[0], ref[0]) and np.array_equal(got[1], ref[1])
+        with pytest.raises(myl.MylError) as e:
+            ctx.synchronize()
+        assert e.value.code == DEVICE_ERR
+    got = run_verify(ctx, p, counts=[5, -3, 2])
+    ref = R.verify(p["target"], p["draft"], p["tokens"], [2, 0, 2], p["rand"], R.EXP_LUT, 4, 0)
+    assert np.array_equal(got[0], ref[0]) and np.array_equal(got[1], ref[1])
+    with pytest.raises(myl.MylError):
+        ctx.synchronize()
+    ctx.synchronize()
+
+
+# ---- captured in a CUDA graph ------------------------------------------------------------
+
+def test_serving_operators_in_a_graph(ctx):
+    """After a first call has sized the workspaces, the operators can be captured and replayed."""
+    rng = np.random.default_rng(20)
+    x = attention_problem(rng, 3, 2, 4, 2, 64, 150, 10)
+    lens = [2, 10, 7]
+    plan, prefix = make_plan(ctx, PLAN), myl.Prefix(ctx, dev(x["k"]), dev(x["v"]))
+    q, ks, vs, dl = dev(x["q"]), dev(x["ks"]), dev(x["vs"]), dev(np.array(lens, np.int32))
+    out = torch.zeros((3, 2, 256), dtype=torch.int16, device="cuda")
+    p = verify_problem(rng, 3, 2, 500)
+    t, d, tok, rand = dev(p["target"]), dev(p["draft"]), dev(p["tokens"]), dev(p["rand"])
+    ver = myl.DraftVerifier(ctx, R.EXP_LUT, 4, 0)
+    acc, toks = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in ((3,), (3, 3)))
+    a = adapter_problem(rng, 6, 256, 64, 8, 3)
+    ids = rng.integers(-1, 3, size=6)
+    w = myl.Weight(ctx, a["W"], 256, a["ws"])
+    rq, ad = w.requant(myl.RQ_SHIFT_I16, 8, 8), myl.Adapters(ctx, a["A"], a["sa"], a["B"], a["sb"], 8, 8, 8)
+    ax, ai, ay = dev(a["x"]), dev(ids.astype(np.int32)), torch.zeros((6, 64), dtype=torch.int16, device="cuda")
+
+    def step():
+        prefix.attention_dev(plan, q, ks, vs, dl, out)
+        w.linear_adapters_dev(rq, ad, ax, ai, ay)
+        ver.verify_dev(t, d, tok, None, rand, acc, toks)
+
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        step()
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        step()
+    for z in (out, ay, acc, toks):
+        z.zero_()
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    assert np.array_equal(out.cpu().numpy(),
+                          R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **PLAN))
+    assert np.array_equal(ay.cpu().numpy(), adapter_ref(a, ids))
+    ref = R.verify(p["target"], p["draft"], p["tokens"], None, p["rand"], R.EXP_LUT, 4, 0)
+    assert np.array_equal(acc.cpu().numpy(), ref[0]) and np.array_equal(toks.cpu().numpy(), ref[1])
+    ctx.synchronize()
