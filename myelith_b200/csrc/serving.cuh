@@ -34,6 +34,9 @@ struct myl_verifier {
   int32_t max = 0;
   uint32_t mult = 0;
   int shift = 0;
+  int32_t reach = 0;  // see VerifyParams
+  uint32_t scaled = 0;
+  int pre = 0, post = 0;
   std::vector<void*> allocs;
 };
 
@@ -177,6 +180,45 @@ int run_adapter_expand(myl_ctx* ctx, const AdapterParams& p, int16_t* y, int64_t
   LaunchCfg lc(ctx, dim3(unsigned((p.N + 255) / 256), unsigned(std::min<int64_t>(p.M, 65535))), dim3(256), 0, st);
   CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_expand_kernel, p, y, ldy));
   ctx->launches++;
+  return MYL_OK;
+}
+
+// A cluster per position where the rows' slices fit its CTAs' shared memory,
+// a block per row otherwise.
+int run_verify(myl_ctx* ctx, VerifyParams& p, cudaStream_t st) {
+  const int64_t units = int64_t(p.B) * (p.D + 1);
+  const int64_t logit_bytes = p.draft ? 8 : 4;
+  // slices of at most 78 KB, so that two CTAs share an SM and one loads while
+  // the other sweeps; smaller ones where that leaves SMs without a CTA
+  int cl = 1;
+  while (cl < VERIFY_MAX_CL && p.V * logit_bytes > int64_t(cl) * 78 * 1024) cl *= 2;
+  while (cl < VERIFY_MAX_CL && 2 * units * cl <= ctx->num_sms && p.V >= cl * 4096) cl *= 2;
+  p.per = int(((p.V + cl - 1) / cl + 3) & ~3);
+  const int64_t smem = p.per * logit_bytes;
+  if (smem <= VERIFY_SMEM && units * cl <= INT32_MAX) {
+    const size_t had = ctx->vfy_done.cap;
+    TRY(ensure(ctx->vfy_done, size_t(p.B) * 4));
+    if (ctx->vfy_done.cap != had) CUDA_TRY(cudaMemsetAsync(ctx->vfy_done.p, 0, ctx->vfy_done.cap, st));
+    TRY(ensure(ctx->vfy, size_t(units) * 4));
+    p.done = static_cast<unsigned*>(ctx->vfy_done.p);
+    p.pos = static_cast<int32_t*>(ctx->vfy.p);
+    const void* fn = reinterpret_cast<const void*>(&verify_cluster_kernel);
+    TRY(kernel_smem_occupancy(ctx->device, fn, VERIFY_THREADS, VERIFY_SMEM, nullptr));
+    if (cl > 8) CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    LaunchCfg lc(ctx, dim3(unsigned(units * cl)), dim3(VERIFY_THREADS), size_t(smem), st, unsigned(cl));
+    CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, verify_cluster_kernel, p, cl));
+    ctx->launches++;
+    return MYL_OK;
+  }
+  const int64_t rows = int64_t(p.B) * (2 * p.D + 1);
+  TRY(ensure(ctx->vfy, size_t(rows) * 12));
+  p.rsum = static_cast<uint64_t*>(ctx->vfy.p);
+  p.rmax = reinterpret_cast<int32_t*>(p.rsum + rows);
+  LaunchCfg l1(ctx, dim3(unsigned(p.B * (p.D + 1 + (p.draft ? p.D : 0)))), dim3(VERIFY_THREADS), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, verify_stats_kernel, p));
+  LaunchCfg l2(ctx, dim3(unsigned(p.B)), dim3(VERIFY_THREADS), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, verify_sample_kernel, p));
+  ctx->launches += 2;
   return MYL_OK;
 }
 
@@ -376,7 +418,24 @@ int myl_verifier_create(myl_ctx* ctx, const int16_t* exp_lut, int64_t exp_len, u
   v->mult = temp_mult;
   v->shift = temp_shift;
   int rc = check_exp_lut(exp_lut, exp_len, &v->max);
-  if (rc == MYL_OK) rc = dev_upload(v->allocs, &v->d_lut, exp_lut, size_t(exp_len));
+  if (rc == MYL_OK) {
+    // (d * mult) >> shift < entries  <=>  d <= ((entries << shift) - 1) / mult, with the
+    // entries up to the last one above zero
+    while (v->len > 1 && exp_lut[v->len - 1] == 0) --v->len;
+    const unsigned __int128 d = (((unsigned __int128)v->len << temp_shift) - 1) / temp_mult;
+    v->reach = d < (unsigned __int128)INT32_MAX ? int32_t(d) : INT32_MAX;
+    // the lookup's 32-bit form, see VerifyParams (reach 0: every index is 0)
+    if (v->reach > 0) {
+      const int up = std::max(0, 32 - int(temp_shift));
+      v->pre = std::min(up, __builtin_clz(unsigned(v->reach)));
+      v->scaled = uint32_t(uint64_t(temp_mult) << (up - v->pre));
+      v->post = std::max(0, int(temp_shift) - 32);
+    }
+  }
+  if (rc == MYL_OK) rc = dev_alloc(v->allocs, &v->d_lut, size_t(v->len) + 1);
+  if (rc == MYL_OK && (cudaMemcpy(v->d_lut, exp_lut, size_t(v->len) * 2, cudaMemcpyHostToDevice) != cudaSuccess ||
+                       cudaMemset(v->d_lut + v->len, 0, 2) != cudaSuccess))
+    rc = fail(MYL_ERR_CUDA, "exp table upload");
   if (rc != MYL_OK) {
     free_handle(ctx, v);
     return rc;
@@ -425,21 +484,17 @@ int myl_verify_dev(myl_ctx* ctx, const myl_verifier* v, const int32_t* target, i
   p.lut_len = int32_t(v->len);
   p.mult = v->mult;
   p.shift = v->shift;
+  p.reach = v->reach;
+  p.scaled = v->scaled;
+  p.pre = v->pre;
+  p.post = v->post;
   p.accepted = accepted;
   p.out = out_tokens;
   p.err = ctx->d_err;
   TRY(ws_acquire(ctx, st));
-  const int64_t rows = batch * (2 * drafted + 1);
-  TRY(ensure(ctx->vfy, size_t(rows) * 12));
-  p.rsum = static_cast<uint64_t*>(ctx->vfy.p);
-  p.rmax = reinterpret_cast<int32_t*>(p.rsum + rows);
   {
     PdlScope pdl(ctx);
-    LaunchCfg l1(ctx, dim3(unsigned(batch * (drafted + 1 + (draft ? drafted : 0)))), dim3(VERIFY_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, verify_stats_kernel, p));
-    LaunchCfg l2(ctx, dim3(unsigned(batch)), dim3(VERIFY_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, verify_sample_kernel, p));
-    ctx->launches += 2;
+    TRY(run_verify(ctx, p, st));
   }
   return ws_release(ctx, st);
 }

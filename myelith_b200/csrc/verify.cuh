@@ -20,6 +20,10 @@
 namespace myl {
 
 constexpr int VERIFY_THREADS = 512;
+constexpr int VERIFY_WARPS = VERIFY_THREADS / 32;
+constexpr int VERIFY_MAX_CL = 16;         // CTAs per cluster (16 is the opt-in size)
+constexpr int VERIFY_SMEM = 220 * 1024;   // bytes of logits a CTA may hold
+constexpr int VERIFY_U = 5;               // 16-byte loads in flight per thread and row
 
 struct VerifyParams {
   const int32_t* target;  // [B][D + 1][V] with strides
@@ -30,10 +34,19 @@ struct VerifyParams {
   const int32_t* counts;  // [B] drafted tokens, null: D
   const uint64_t* rand;   // [B][D + 1]
   int B, D, V;
-  const int16_t* lut;
+  const int16_t* lut;  // [lut_len + 1], entry lut_len = 0
   int32_t lut_len;
   uint32_t mult;
   int shift;
+  int32_t reach;  // largest difference to the maximum with a table entry above zero; INT32_MAX: no bound
+  // (d * mult) >> shift for d <= reach as umulhi(d << pre, scaled) >> post: d * mult < 2^(31 + shift)
+  // there, so mult << (32 - shift - pre) fits 32 bits with reach << pre filling them
+  uint32_t scaled;
+  int pre, post;
+  int per;        // logits per CTA of a cluster (a multiple of 4)
+  int32_t* pos;    // [B][D + 1] outcome of a position: the drawn token, or -1 (accepted)
+  unsigned* done;  // [B] finished positions, zero between calls
+  // vocabularies beyond a cluster: row statistics
   int32_t* rmax;   // [B][2 D + 1]: target rows, then draft rows
   uint64_t* rsum;
   int32_t* accepted;  // [B]
@@ -41,10 +54,18 @@ struct VerifyParams {
   int* err;
 };
 
+// The weight of logit l below the maximum m; without a branch, so that the
+// lookups of several logits are in flight together.
 __device__ __forceinline__ uint32_t verify_weight(const VerifyParams& p, int32_t m, int32_t l) {
   const uint32_t d = min(uint32_t(m) - uint32_t(l), uint32_t(INT32_MAX));  // m >= l
-  const uint64_t idx = (uint64_t(d) * p.mult) >> p.shift;
-  return idx < uint64_t(p.lut_len) ? uint32_t(p.lut[idx]) : 0u;
+  const uint32_t idx = __umulhi(d << p.pre, p.scaled) >> p.post;
+  return uint32_t(uint16_t(__ldg(p.lut + (d <= uint32_t(p.reach) ? idx : uint32_t(p.lut_len)))));
+}
+
+// The smallest logit that can carry weight below the maximum m.
+__device__ __forceinline__ int32_t verify_floor(const VerifyParams& p, int32_t m) {
+  const int64_t t = int64_t(m) - p.reach;
+  return p.reach == INT32_MAX || t < INT32_MIN ? INT32_MIN : int32_t(t);
 }
 
 __device__ __forceinline__ int verify_count(const VerifyParams& p, int b) {
@@ -57,6 +78,299 @@ __device__ __forceinline__ int verify_count(const VerifyParams& p, int b) {
   return c;
 }
 
+// ---- one pass: a cluster per position --------------------------------------------------
+// Position i of request b is one cluster: its CTAs hold the target row and the
+// draft row in shared memory, a slice each, so that every logit is read from
+// HBM once. Maxima and weight sums cross the cluster through distributed
+// shared memory (two cluster barriers), the draw of a rejected position takes
+// a third; accepted positions stop after the second. All CTAs of a cluster
+// reach the same decisions from the same words. Weights past `reach` are zero,
+// so a slice is swept with one comparison per logit against max - reach, and a
+// warp looks the table up only where one of its logits passes. Positions past
+// the drafted ones are not read. The last position of a request to finish (a
+// counter per request) writes its output.
+struct VerifyShared {
+  int32_t mx[2][VERIFY_MAX_CL];              // slice maxima by CTA: target, draft
+  unsigned long long sum[2][VERIFY_MAX_CL];  // slice weight sums
+  unsigned long long rho[VERIFY_MAX_CL];     // slice sums of the residual weights
+  int32_t wmax[2][VERIFY_WARPS];
+  unsigned long long wsum[2][VERIFY_WARPS];
+};
+
+__device__ __forceinline__ void verify_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void verify_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Copies n logits of each row (ROWS = 1: the first alone) to shared memory,
+// all rows' loads of a batch in flight together; m: this thread's maxima.
+// Rows off 16-byte boundaries are read by single words.
+template <int ROWS>
+__device__ __forceinline__ void verify_load(const int32_t* const (&row)[2], int n, int32_t* const (&s)[2],
+                                            int32_t (&m)[2]) {
+  bool vec = true;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) vec = vec && (reinterpret_cast<uintptr_t>(row[r]) & 15) == 0;
+  int done = 0;
+  if (vec) {
+    const int nv = n / 4;
+    done = 4 * nv;
+    for (int v0 = threadIdx.x; v0 < nv; v0 += VERIFY_U * VERIFY_THREADS) {
+      int4 x[ROWS][VERIFY_U];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int u = 0; u < VERIFY_U; ++u) {
+          const int v = v0 + u * VERIFY_THREADS;
+          if (v < nv) x[r][u] = __ldcs(reinterpret_cast<const int4*>(row[r]) + v);
+        }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int u = 0; u < VERIFY_U; ++u) {
+          const int v = v0 + u * VERIFY_THREADS;
+          if (v < nv) {
+            const int4 y = x[r][u];
+            reinterpret_cast<int4*>(s[r])[v] = y;
+            m[r] = max(m[r], max(max(y.x, y.y), max(y.z, y.w)));
+          }
+        }
+    }
+  }
+  for (int j0 = done + int(threadIdx.x); j0 < n; j0 += 4 * VERIFY_U * VERIFY_THREADS) {
+    int32_t x[ROWS][4 * VERIFY_U];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int u = 0; u < 4 * VERIFY_U; ++u) {
+        const int j = j0 + u * VERIFY_THREADS;
+        if (j < n) x[r][u] = __ldcs(row[r] + j);
+      }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int u = 0; u < 4 * VERIFY_U; ++u) {
+        const int j = j0 + u * VERIFY_THREADS;
+        if (j < n) m[r] = max(m[r], s[r][j] = x[r][u]);
+      }
+  }
+}
+
+// Replaces n logits in shared memory by their weights and returns this
+// thread's sum (S < 2^32 over all slices). A warp whose vectors hold no logit
+// at the floor or above writes zeros without looking the table up.
+__device__ __forceinline__ uint32_t verify_sum(const VerifyParams& p, int32_t* s, int n, int32_t m) {
+  const int32_t t = verify_floor(p, m);
+  uint32_t w = 0;
+  for (int v0 = 0; 4 * v0 < n; v0 += VERIFY_THREADS) {
+    const int v = v0 + int(threadIdx.x);
+    const int left = n - 4 * v;  // logits of the vector inside the slice
+    int4 x = make_int4(0, 0, 0, 0);
+    if (left > 0) x = reinterpret_cast<const int4*>(s)[v];
+    if (__any_sync(0xffffffffu, left > 0 && max(max(x.x, x.y), max(x.z, x.w)) >= t)) {
+      x.x = int32_t(verify_weight(p, m, x.x));
+      x.y = left > 1 ? int32_t(verify_weight(p, m, x.y)) : 0;
+      x.z = left > 2 ? int32_t(verify_weight(p, m, x.z)) : 0;
+      x.w = left > 3 ? int32_t(verify_weight(p, m, x.w)) : 0;
+      w += left > 0 ? uint32_t(x.x) + uint32_t(x.y) + uint32_t(x.z) + uint32_t(x.w) : 0u;
+    } else {
+      x = make_int4(0, 0, 0, 0);
+    }
+    if (left > 0) reinterpret_cast<int4*>(s)[v] = x;
+  }
+  return w;
+}
+
+__global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_cluster_kernel(VerifyParams p, int cl) {
+  verify_arrive();
+  pdl_wait();
+  pdl_launch();
+  extern __shared__ __align__(16) int32_t s_logit[];  // target slice [per], draft slice [per]
+  __shared__ VerifyShared sm;
+  const int rank = int(cluster_ctarank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int unit = int(blockIdx.x) / cl, b = unit / (p.D + 1), i = unit % (p.D + 1);
+  const int cnt = verify_count(p, b);
+  const int j0 = min(p.V, rank * p.per), n = min(p.per, p.V - j0);
+  const bool need = i <= cnt;  // later positions are not reached
+  const bool drafted = i < cnt, pair = drafted && p.draft;
+  int32_t *s_t = s_logit, *s_d = s_logit + p.per;
+  const int32_t* trow = p.target + b * p.ts_b + i * p.ts_d;
+  const int32_t* drow = pair ? p.draft + b * p.ds_b + i * p.ds_d : trow;
+  int x = -1;
+  uint64_t word = 0;
+  if (need) {
+    if (drafted) x = p.tokens[int64_t(b) * p.D + i];
+    word = p.rand[int64_t(b) * (p.D + 1) + i];
+    int32_t m[2] = {INT32_MIN, INT32_MIN};
+    if (pair) verify_load<2>({trow + j0, drow + j0}, n, {s_t, s_d}, m);
+    else verify_load<1>({trow + j0, trow + j0}, n, {s_t, s_d}, m);
+    m[0] = __reduce_max_sync(0xffffffffu, m[0]);
+    m[1] = __reduce_max_sync(0xffffffffu, m[1]);
+    if (lane == 0) sm.wmax[0][warp] = m[0], sm.wmax[1][warp] = m[1];
+  }
+  __syncthreads();
+  verify_wait();  // every CTA of the cluster runs: its shared memory may be written
+  if (!need) return;
+  const bool inside = x >= 0 && x < p.V;
+  const int32_t lt = inside ? trow[x] : 0, ld = inside ? drow[x] : 0;
+  // warp 0 joins the warps' values; thread k < cl writes them into CTA k
+  if (warp == 0) {
+    const int32_t a = __reduce_max_sync(0xffffffffu, sm.wmax[0][lane % VERIFY_WARPS]);
+    const int32_t c = __reduce_max_sync(0xffffffffu, sm.wmax[1][lane % VERIFY_WARPS]);
+    if (lane < cl) {
+      st_shared_cluster_u32(mapa_shared(smem_addr(&sm.mx[0][rank]), lane), uint32_t(a));
+      st_shared_cluster_u32(mapa_shared(smem_addr(&sm.mx[1][rank]), lane), uint32_t(c));
+    }
+  }
+  cluster_sync_all();
+  const int32_t mt = __reduce_max_sync(0xffffffffu, sm.mx[0][lane % cl]);
+  const int32_t md = __reduce_max_sync(0xffffffffu, sm.mx[1][lane % cl]);
+  auto join = [&](const unsigned long long* w) {  // warp 0: the sum of the warps' values
+    unsigned long long v = lane < VERIFY_WARPS ? w[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  {
+    const uint32_t a = __reduce_add_sync(0xffffffffu, verify_sum(p, s_t, n, mt));
+    const uint32_t c = pair ? __reduce_add_sync(0xffffffffu, verify_sum(p, s_d, n, md)) : 0;
+    if (lane == 0) sm.wsum[0][warp] = a, sm.wsum[1][warp] = c;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const unsigned long long a = join(sm.wsum[0]), c = join(sm.wsum[1]);
+    if (lane < cl) {
+      st_shared_cluster_u64(mapa_shared(smem_addr(&sm.sum[0][rank]), lane), a);
+      st_shared_cluster_u64(mapa_shared(smem_addr(&sm.sum[1][rank]), lane), c);
+    }
+  }
+  cluster_sync_all();
+  uint64_t sw = 0, sz = pair ? 0 : 1;
+  for (int k = 0; k < cl; ++k) {
+    sw += sm.sum[0][k];
+    if (pair) sz += sm.sum[1][k];
+  }
+  bool accept = false;
+  if (drafted) {
+    uint64_t wx = 0, zx = 0;
+    if (inside) {
+      wx = verify_weight(p, mt, lt);
+      zx = pair ? verify_weight(p, md, ld) : 1;
+    } else if (rank == 0 && threadIdx.x == 0) {
+      atomicCAS(p.err, 0, DEV_BAD_TOKEN);
+    }
+    // u X < 2^32 Y iff floor(u X / 2^32) < Y
+    accept = __umul64hi((word >> 32) << 32, zx * sw) < wx * sz;
+  }
+  int drawn = -1;
+  bool writer = accept && rank == 0 && threadIdx.x == 0;
+  if (!accept) {
+    bool rest = drafted;
+    // the slice's vector v: target weights, or what the draft leaves of them
+    auto left4 = [&](int v, unsigned long long (&r)[4]) -> unsigned long long {
+      if (4 * v >= n) return r[0] = r[1] = r[2] = r[3] = 0;
+      const int4 w = reinterpret_cast<const int4*>(s_t)[v];
+      r[0] = uint32_t(w.x), r[1] = uint32_t(w.y), r[2] = uint32_t(w.z), r[3] = uint32_t(w.w);
+      const unsigned long long any = r[0] | r[1] | r[2] | r[3];
+      if (rest && any) {
+        int4 z = make_int4(0, 0, 0, 0);
+        if (pair) {
+          z = reinterpret_cast<const int4*>(s_d)[v];
+        } else if (unsigned(x - j0 - 4 * v) < 4u) {
+          const int e = x - j0 - 4 * v;
+          z = make_int4(e == 0, e == 1, e == 2, e == 3);
+        }
+        const uint32_t q[4] = {uint32_t(z.x), uint32_t(z.y), uint32_t(z.z), uint32_t(z.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint64_t a = r[e] * sz, c = q[e] * sw;
+          r[e] = a > c ? a - c : 0;
+        }
+      }
+      return r[0] + r[1] + r[2] + r[3];
+    };
+    unsigned long long w4[4];
+    if (rest) {
+      unsigned long long r = 0;
+      for (int v = threadIdx.x; 4 * v < n; v += VERIFY_THREADS) r += left4(v, w4);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+      if (lane == 0) sm.wsum[0][warp] = r;
+      __syncthreads();
+      if (warp == 0) {
+        const unsigned long long a = join(sm.wsum[0]);
+        if (lane < cl) st_shared_cluster_u64(mapa_shared(smem_addr(&sm.rho[rank]), lane), a);
+      }
+      cluster_sync_all();
+      unsigned long long total = 0;
+      for (int k = 0; k < cl; ++k) total += sm.rho[k];
+      rest = total != 0;  // nothing is left of the target: draw from its own weights
+    }
+    const unsigned long long* share = rest ? sm.rho : sm.sum[0];
+    unsigned long long total = 0, before = 0;
+    for (int k = 0; k < cl; ++k) {
+      if (k < rank) before += share[k];
+      total += share[k];
+    }
+    const unsigned long long tau = __umul64hi((word & 0xFFFFFFFFull) << 32, total);
+    if (tau >= before && tau - before < share[rank]) {  // the draw falls into this slice
+      // warp w: the consecutive 128-logit pieces [w * pw, (w + 1) * pw)
+      const int pw = ((n + 127) / 128 + VERIFY_WARPS - 1) / VERIFY_WARPS;
+      unsigned long long own = 0;
+      for (int q = warp * pw; q < (warp + 1) * pw; ++q) own += left4(32 * q + lane, w4);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+      if (lane == 0) sm.wsum[1][warp] = own;
+      __syncthreads();
+      unsigned long long run = before;
+      for (int k = 0; k < warp; ++k) run += sm.wsum[1][k];
+      if (tau >= run && tau - run < own) {  // this warp's pieces hold it
+        for (int q = warp * pw; q < (warp + 1) * pw; ++q) {
+          const unsigned long long mine = left4(32 * q + lane, w4);
+          unsigned long long at = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long up = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += up;
+          }
+          const unsigned long long all = __shfl_sync(0xffffffffu, at, 31);
+          if (tau - run < all) {
+            at += run - mine;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (tau >= at && tau - at < w4[e]) {
+                drawn = j0 + 4 * (32 * q + lane) + e;
+                writer = true;
+              }
+              at += w4[e];
+            }
+            break;
+          }
+          run += all;
+        }
+      }
+    }
+  }
+  if (writer) {
+    int32_t* pos = p.pos + int64_t(b) * (p.D + 1);
+    pos[i] = drawn;
+    __threadfence();
+    if (atomicAdd(p.done + b, 1u) == unsigned(cnt)) {  // the last of positions 0 .. cnt
+      __threadfence();
+      p.done[b] = 0;
+      int32_t* out = p.out + int64_t(b) * (p.D + 1);
+      int k = 0;
+      int32_t t;
+      while ((t = __ldcg(pos + k)) < 0) {  // position cnt always draws
+        out[k] = p.tokens[int64_t(b) * p.D + k];
+        ++k;
+      }
+      p.accepted[b] = k;
+      out[k] = t;
+      for (int r = k + 1; r <= p.D; ++r) out[r] = -1;
+    }
+  }
+}
+
+// ---- vocabularies beyond a cluster's shared memory ----------------------------------------
 // Row statistics: one block per logit row, its maximum and weight sum.
 __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(VerifyParams p) {
   pdl_wait();

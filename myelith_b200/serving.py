@@ -17,36 +17,40 @@ import ctypes as C
 
 import numpy as np
 
-_bound = False
+_L = None
+_DTYPES: dict = {}
+_current_stream = None
 
 
 def _lib():
-    global _bound
+    """The library with these entry points bound (once), and torch's part of a call."""
+    global _L
+    if _L is not None:
+        return _L
     from . import load_library
 
     L = load_library()
-    if not _bound:
-        vp, i64, u8, i32 = C.c_void_p, C.c_int64, C.c_uint8, C.c_int
-        pp = C.POINTER(vp)
-        for name, args in (
-                ("myl_attn_plan_create", [vp, i64, u8, vp, i64, u8, u8, i32, pp]),
-                ("myl_attn_plan_release", [vp, vp]),
-                ("myl_prefix_create", [vp, vp, vp, i64, i64, i64, i64, i64, vp, pp]),
-                ("myl_prefix_release", [vp, vp]),
-                ("myl_prefix_attention_dev", [vp, vp, vp, vp, i64, i64, i64, i64, vp, vp, i64, i64, i64, i64, vp,
-                                              vp, i64, vp]),
-                ("myl_adapters_register", [vp, i64, i64, i64, i64, vp, vp, vp, vp, u8, u8, u8, pp]),
-                ("myl_adapters_release", [vp, vp]),
-                ("myl_linear_adapters_dev", [vp, vp, vp, vp, vp, i64, i64, vp, vp, i64, vp]),
-                ("myl_verifier_create", [vp, vp, i64, C.c_uint32, u8, pp]),
-                ("myl_verifier_release", [vp, vp]),
-                ("myl_verify_dev", [vp, vp, vp, i64, i64, vp, i64, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp])):
-            f = getattr(L, name)
-            f.argtypes = args
-            f.restype = i32
-        L.myl_prefix_positions.argtypes = [vp]
-        L.myl_prefix_positions.restype = i64
-        _bound = True
+    vp, i64, u8, i32 = C.c_void_p, C.c_int64, C.c_uint8, C.c_int
+    pp = C.POINTER(vp)
+    for name, args in (
+            ("myl_attn_plan_create", [vp, i64, u8, vp, i64, u8, u8, i32, pp]),
+            ("myl_attn_plan_release", [vp, vp]),
+            ("myl_prefix_create", [vp, vp, vp, i64, i64, i64, i64, i64, vp, pp]),
+            ("myl_prefix_release", [vp, vp]),
+            ("myl_prefix_attention_dev", [vp, vp, vp, vp, i64, i64, i64, i64, vp, vp, i64, i64, i64, i64, vp, vp, i64,
+                                          vp]),
+            ("myl_adapters_register", [vp, i64, i64, i64, i64, vp, vp, vp, vp, u8, u8, u8, pp]),
+            ("myl_adapters_release", [vp, vp]),
+            ("myl_linear_adapters_dev", [vp, vp, vp, vp, vp, i64, i64, vp, vp, i64, vp]),
+            ("myl_verifier_create", [vp, vp, i64, C.c_uint32, u8, pp]),
+            ("myl_verifier_release", [vp, vp]),
+            ("myl_verify_dev", [vp, vp, vp, i64, i64, vp, i64, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp])):
+        f = getattr(L, name)
+        f.argtypes = args
+        f.restype = i32
+    L.myl_prefix_positions.argtypes = [vp]
+    L.myl_prefix_positions.restype = i64
+    _L = L
     return L
 
 
@@ -63,22 +67,32 @@ def _bad(fn: str, msg: str):
     return MylError(fn, MYL_ERR_SHAPE, msg)
 
 
-def _need(fn: str, ctx, what: str, t, dtype: str, dim: int):
+def _need(fn: str, ctx, what: str, t, dtype: str, dim: int) -> None:
     """A CUDA tensor of the context's device with `dim` dimensions, the last one dense."""
-    from . import MYL_ERR_ARG, MylError
+    if not _DTYPES:
+        import torch
 
-    if str(t.dtype) != "torch." + dtype or t.device.type != "cuda" or t.device.index != ctx.device:
+        _DTYPES.update(int16=torch.int16, int32=torch.int32, int64=torch.int64)
+    if t.dtype is not _DTYPES[dtype] or t.get_device() != ctx.device:
+        from . import MYL_ERR_ARG, MylError
+
         raise MylError(fn, MYL_ERR_ARG, f"{what}: a {dtype} tensor on cuda:{ctx.device} is needed, got {t.dtype} on "
                                         f"{t.device}")
-    if t.dim() != dim or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel()):
         raise _bad(fn, f"{what}: {dim} dimensions with a dense last one are needed, got {tuple(t.shape)} with "
                        f"strides {t.stride()}")
 
 
-def _stream(stream) -> int | None:
-    from . import _stream_ptr
+def _stream(ctx, stream) -> int | None:
+    """The stream's handle; by default torch's current stream on the context's device."""
+    global _current_stream
+    if stream is None:
+        if _current_stream is None:
+            import torch
 
-    return _stream_ptr(stream)
+            _current_stream = torch.cuda.current_stream
+        stream = _current_stream(ctx.device)
+    return int(getattr(stream, "cuda_stream", stream)) or None
 
 
 class _Handle:
@@ -134,7 +148,7 @@ class Prefix(_Handle):
         h = C.c_void_p()
         _check(fn, _lib().myl_prefix_create(
             ctx.handle, k.data_ptr() if P else None, v.data_ptr() if P else None, P, nkv, hd,
-            k.stride(1) if P > 1 else hd, k.stride(0) if nkv > 1 else 0, _stream(stream), C.byref(h)))
+            k.stride(1) if P > 1 else hd, k.stride(0) if nkv > 1 else 0, _stream(self.ctx, stream), C.byref(h)))
         self._h = h
         self.kv_heads, self.positions, self.head_dim = nkv, P, hd
 
@@ -169,7 +183,7 @@ class Prefix(_Handle):
         _check(fn, _lib().myl_prefix_attention_dev(
             self.ctx.handle, plan.handle, self._h, q.data_ptr(), B, T, nq, ldq, k_suffix.data_ptr() if S else None,
             v_suffix.data_ptr() if S else None, S, ks[0] if B > 1 else 0, ks[1] if self.kv_heads > 1 else 0,
-            ks[2] if S > 1 else hd, lens.data_ptr(), out.data_ptr(), ldo, _stream(stream)))
+            ks[2] if S > 1 else hd, lens.data_ptr(), out.data_ptr(), ldo, _stream(self.ctx, stream)))
 
 
 class Adapters(_Handle):
@@ -212,7 +226,7 @@ def linear_adapters_dev(weight, rq, adapters: Adapters, x, ids, y, stream=None) 
     _check(fn, _lib().myl_linear_adapters_dev(
         ctx.handle, weight.handle, rq.handle, adapters.handle, x.data_ptr(), M,
         x.stride(0) if M > 1 else weight.in_features, ids.data_ptr(), y.data_ptr(),
-        y.stride(0) if M > 1 else weight.out_features, _stream(stream)))
+        y.stride(0) if M > 1 else weight.out_features, _stream(ctx, stream)))
 
 
 class DraftVerifier(_Handle):
@@ -266,4 +280,4 @@ class DraftVerifier(_Handle):
             draft.data_ptr() if use else None, draft.stride(0) if use else 0,
             (draft.stride(1) if D1 > 2 else V) if use else V, B, D1 - 1, V, tokens.data_ptr() if D1 > 1 else None,
             None if counts is None else counts.data_ptr(), rand.data_ptr(), accepted.data_ptr(),
-            out_tokens.data_ptr(), _stream(stream)))
+            out_tokens.data_ptr(), _stream(self.ctx, stream)))

@@ -390,6 +390,24 @@ def test_verify(ctx, B, D, V, dist):
     check_verify(ctx, p, counts=rng.integers(0, D + 1, size=B), mult=int(4 / 0.7 * 65536), shift=16)
 
 
+@pytest.mark.parametrize("dist", [True, False])
+def test_verify_large_vocabulary(ctx, dist):
+    """Rows beyond a cluster's shared memory, with a table of smaller weights."""
+    rng = np.random.default_rng(21)
+    lut = (R.EXP_LUT >> 5).astype(np.int16)
+    for V in (470001, 930000):
+        p = verify_problem(rng, 2, 1, V, dist=dist)
+        check_verify(ctx, p, lut=lut)
+    check_verify(ctx, verify_problem(rng, 1, 2, 99, dist=dist), lut=lut)
+
+
+def test_verify_workspaces_of_changing_sizes(ctx):
+    """Few requests with many drafts, then many requests with few, and back."""
+    rng = np.random.default_rng(22)
+    for B, D in ((1, 200), (300, 0), (150, 1), (1, 200), (600, 2)):
+        check_verify(ctx, verify_problem(rng, B, D, 40), counts=rng.integers(0, D + 1, size=B))
+
+
 def test_verify_covers_every_outcome(ctx):
     rng = np.random.default_rng(8)
     p = verify_problem(rng, 200, 3, 50, sigma=100.0, noise=40.0)
