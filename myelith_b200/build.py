@@ -16,7 +16,7 @@ LIB = os.path.join(HERE, "libmyl_w8a16.so")
 SOURCES = ["myl_w8a16.cu"]
 HEADERS = ["common.cuh", "gemv.cuh", "gemm_tc.cuh", "moe.cuh", "backward.cuh", "select.cuh",
            "wire.cuh", "artifact.hpp", "forward.cuh", "model.cuh", "rownorm.cuh",
-           "prefix.cuh", "adapters.cuh", "verify.cuh", "serving.cuh"]
+           "prefix.cuh", "prefix_tc.cuh", "adapters.cuh", "verify.cuh", "serving.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -14,12 +14,14 @@
 // partial results would change values: scores with the row maxima, exponential
 // sums and weighted values are three passes over the scores.
 //
-// The prefix is laid out once, when it is registered, as byte planes
-// (x = 256 hi + lo, hi signed, lo unsigned): keys [kv head][position][hd] and
+// The prefix is laid out once, when it is registered, as unsigned byte planes
+// (x + 32768 = 256 hi + lo): keys [kv head][position][hd] and
 // values transposed [kv head][hd][position], positions padded with zeros to a
 // multiple of PFX_PAD. Rows of a KV head g are numbered
 // rho = (b * T + t) * G + (h - g * G), R = B * T * G of them; score rows are
-// g * R + rho, prefix scores in columns [0, P), suffix scores from column Pp.
+// g * R + rho, prefix scores in columns [0, P), suffix scores from column soff.
+// The kernels here run any head size and few rows; prefix_tc.cuh has the prefix
+// part for many rows, with these kernels on the suffixes.
 #pragma once
 
 #include "common.cuh"
@@ -51,7 +53,7 @@ struct PrefixParams {
   int32_t exp_len;
   int lut_shift, prob_frac, out_shift;
   int32_t* scores;  // [nkv * R][lds]
-  int64_t lds;
+  int64_t lds, soff;
   unsigned* rowmax;  // [nkv * R] as max (score ^ 0x80000000)
   int32_t* rowsum;
   unsigned long long* acc;  // [nkv * R][hd] int64 sums (two's complement)
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(256)
     }
     if (d < hd) {
       const int64_t o = (g * Pp + j) * hd + d;
-      kh[o] = uint8_t(uint16_t(kv) >> 8);
+      kh[o] = uint8_t((uint16_t(kv) >> 8) ^ 0x80);
       kl[o] = uint8_t(kv & 255);
     }
     tile[r][x] = vv;
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(256)
     if (d >= hd) continue;
     const int16_t vv = tile[x][r];
     const int64_t o = (g * hd + d) * Pp + j0 + x;
-    vth[o] = uint8_t(uint16_t(vv) >> 8);
+    vth[o] = uint8_t((uint16_t(vv) >> 8) ^ 0x80);
     vtl[o] = uint8_t(vv & 255);
   }
 }
@@ -131,7 +133,7 @@ __global__ void prefix_init_kernel(PrefixParams p, int64_t rows) {
   const int64_t n = rows * p.hd;
   for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
     p.acc[i] = 0;
-    if (i < rows) p.rowmax[i] = 0;
+    if (i < rows) p.rowmax[i] = 0, p.rowsum[i] = 0;
   }
 }
 
@@ -164,6 +166,7 @@ __device__ __forceinline__ void prefix_scores_block(const PrefixParams& p, int g
       } else {
         const int64_t o = (int64_t(g) * p.Pp + j) * hd + 8 * c;
         kh[i] = *reinterpret_cast<const uint2*>(p.kh + o);
+        kh[i].x ^= 0x80808080u, kh[i].y ^= 0x80808080u;  // signed high bytes
         kl[i] = *reinterpret_cast<const uint2*>(p.kl + o);
       }
     }
@@ -200,7 +203,7 @@ __device__ __forceinline__ void prefix_scores_block(const PrefixParams& p, int g
   if (SUFFIX && mine) mine = j < pfx_seen(p, n_b, (rho / p.G) % p.T);
   if (mine) {
     sc = pfx_score(p, int64_t(sh) * 256 + int64_t(sl));
-    p.scores[(int64_t(g) * p.R + rho) * p.lds + (SUFFIX ? p.Pp : 0) + j] = sc;
+    p.scores[(int64_t(g) * p.R + rho) * p.lds + (SUFFIX ? p.soff : 0) + j] = sc;
   }
   int32_t mx = sc;
 #pragma unroll
@@ -238,7 +241,8 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_scores_kernel(PrefixParams
 }
 
 // ---- pass 2: exponential sums, one block per row ----------------------------------------
-__global__ void __launch_bounds__(PFX_THREADS) prefix_sum_kernel(PrefixParams p) {
+// P0: prefix scores of the row to sum (0 where the tensor-core path sums them).
+__global__ void __launch_bounds__(PFX_THREADS) prefix_sum_kernel(PrefixParams p, int P0) {
   pdl_wait();
   pdl_launch();
   __shared__ int32_t s_red[PFX_THREADS / 32];
@@ -248,14 +252,14 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_sum_kernel(PrefixParams p)
   const int32_t m = int32_t(p.rowmax[row] ^ 0x80000000u);
   const int32_t* sc = p.scores + row * p.lds;
   int32_t s = 0;  // the host bounds the keys so that the i32 sum cannot overflow
-  for (int j = threadIdx.x; j < p.P; j += PFX_THREADS) s += pfx_exp(p, m, sc[j]);
-  for (int j = threadIdx.x; j < n; j += PFX_THREADS) s += pfx_exp(p, m, sc[p.Pp + j]);
+  for (int j = threadIdx.x; j < P0; j += PFX_THREADS) s += pfx_exp(p, m, sc[j]);
+  for (int j = threadIdx.x; j < n; j += PFX_THREADS) s += pfx_exp(p, m, sc[p.soff + j]);
   s = __reduce_add_sync(0xffffffffu, s);
   if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < PFX_THREADS / 32; ++w) s += s_red[w];
-    p.rowsum[row] = s;
+    if (s) atomicAdd(p.rowsum + row, s);
   }
 }
 
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_values_kernel(PrefixParams
       const int64_t row = int64_t(g) * p.R + rho;
       if (j < (suffix ? pfx_seen(p, n_b, (rho / p.G) % p.T) : p.P)) {
         const int32_t m = int32_t(p.rowmax[row] ^ 0x80000000u);
-        const int32_t ex = pfx_exp(p, m, p.scores[row * p.lds + (suffix ? p.Pp : 0) + j]);
+        const int32_t ex = pfx_exp(p, m, p.scores[row * p.lds + (suffix ? p.soff : 0) + j]);
         pr = uint32_t(softmax_prob(ex, p.rowsum[row], 0, 1, int32_t(one)));
       }
     }
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_values_kernel(PrefixParams
     } else {
       const int64_t o = (int64_t(g) * hd + d) * p.Pp + j0 + 16 * kg;
       const uint4 a = *reinterpret_cast<const uint4*>(p.vth + o), c = *reinterpret_cast<const uint4*>(p.vtl + o);
-      wh[0] = a.x, wh[1] = a.y, wh[2] = a.z, wh[3] = a.w;
+      wh[0] = a.x ^ 0x80808080u, wh[1] = a.y ^ 0x80808080u, wh[2] = a.z ^ 0x80808080u, wh[3] = a.w ^ 0x80808080u;
       wl[0] = c.x, wl[1] = c.y, wl[2] = c.z, wl[3] = c.w;
     }
 #pragma unroll

@@ -5,6 +5,7 @@
 
 #include "adapters.cuh"
 #include "prefix.cuh"
+#include "prefix_tc.cuh"
 #include "verify.cuh"
 
 struct myl_attn_plan {
@@ -13,12 +14,15 @@ struct myl_attn_plan {
   int32_t exp_max = 0;
   int64_t score_mult = 0;
   int score_shift = 0, lut_shift = 0, prob_frac = 0, out_shift = 0;
+  int cap = 0, lut_n = 0;  // see PrefixTc
+  bool tc = false;         // the constants fit the tensor-core kernels
   std::vector<void*> allocs;
 };
 
 struct myl_prefix {
   int64_t P = 0, Pp = 0, nkv = 0, hd = 0;
   uint8_t *kh = nullptr, *kl = nullptr, *vth = nullptr, *vtl = nullptr;
+  CUtensorMap tm_kh{}, tm_kl{}, tm_vh{}, tm_vl{};  // head_dim 64 and 128
   std::vector<void*> allocs;
 };
 
@@ -66,6 +70,9 @@ void free_handle(myl_ctx* ctx, T* h) {
   delete h;
 }
 
+// Query rows per KV head from which the prefix runs on the tensor cores.
+const int PTC_MIN_ROWS = std::getenv("MYL_PTC_MIN") ? std::atoi(std::getenv("MYL_PTC_MIN")) : 16;
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int attn_plan_build(myl_attn_plan* pl, int64_t score_mult, uint8_t score_shift, const int16_t* exp_lut,
@@ -84,7 +91,30 @@ int attn_plan_build(myl_attn_plan* pl, int64_t score_mult, uint8_t score_shift, 
   pl->lut_shift = lut_shift;
   pl->prob_frac = prob_frac;
   pl->out_shift = out_shift;
+  // Table entries up to the last one above zero, then a zero; a difference
+  // saturates at 2^31 - 1, so its index may end before that.
+  int64_t n = exp_len;
+  while (n > 1 && exp_lut[n - 1] == 0) --n;
+  const int64_t top = INT32_MAX >> lut_shift;
+  pl->cap = int(std::min(n, top));
+  pl->lut_n = pl->cap + 1;
+  // score = low word of a 64-bit value shifted by less than 32, 256 mult in 31 bits
+  pl->tc = score_shift >= 1 && score_shift <= 31 && score_mult >= 0 && score_mult < (1 << 23) && pl->lut_n <= PTC_LUT_MAX;
   return dev_upload(pl->allocs, &pl->d_lut, exp_lut, size_t(exp_len));
+}
+
+int encode_bytes(myl_ctx* ctx, CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int box_cols,
+                 int box_rows) {
+  cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(cols)};
+  cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                                 estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MYL_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return MYL_OK;
 }
 
 int prefix_build(myl_ctx* ctx, myl_prefix* pf, const int16_t* k, const int16_t* v, int64_t pos_stride,
@@ -100,15 +130,106 @@ int prefix_build(myl_ctx* ctx, myl_prefix* pf, const int16_t* k, const int16_t* 
                                                pf->kl, pf->vth, pf->vtl);
     CUDA_TRY(cudaGetLastError());
     ctx->launches++;
+    if (pf->hd == 64 || pf->hd == 128) {
+      const int hd = int(pf->hd);
+      TRY(encode_bytes(ctx, &pf->tm_kh, pf->kh, hd, pf->nkv * pf->Pp, hd, PTC_KEYS));
+      TRY(encode_bytes(ctx, &pf->tm_kl, pf->kl, hd, pf->nkv * pf->Pp, hd, PTC_KEYS));
+      TRY(encode_bytes(ctx, &pf->tm_vh, pf->vth, pf->Pp, pf->nkv * hd, PTC_VKEYS, hd));
+      TRY(encode_bytes(ctx, &pf->tm_vl, pf->vtl, pf->Pp, pf->nkv * hd, PTC_VKEYS, hd));
+    }
   }
   CUDA_TRY(cudaStreamSynchronize(st));
   return MYL_OK;
 }
 
+// Key steps per block so that `units` rows of blocks finish soonest on the
+// SMs, with a fixed cost per block of about `fixed` steps.
+int prefix_split(int units, int steps, int sms, int fixed) {
+  int best = steps;
+  int64_t cost = INT64_MAX;
+  for (int splits = 1; splits <= std::min(steps, 4 * sms / units + 1); ++splits) {
+    const int per = (steps + splits - 1) / splits, n = (steps + per - 1) / per;
+    const int64_t c = (int64_t(units) * n + sms - 1) / sms * (per + fixed);
+    if (c < cost) cost = c, best = per;
+  }
+  return best;
+}
+
+template <int HD>
+int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix* pf, PrefixParams& p, cudaStream_t st) {
+  const int64_t rows = int64_t(p.nkv) * p.R;
+  const int RT = (p.R + PTC_ROWS - 1) / PTC_ROWS, units = p.nkv * RT, n = sms(ctx);
+  PrefixTc qk{}, pv{};
+  qk.RT = pv.RT = RT;
+  qk.cap = pl->cap;
+  qk.lut_n = pl->lut_n;
+  qk.timeout_ns = pv.timeout_ns = ctx->timeout_ns;
+  qk.steps = p.Pp / PTC_KEYS;
+  pv.steps = p.Pp / PTC_VKEYS;
+  qk.per = prefix_split(units, qk.steps, n, 4);
+  pv.per = prefix_split(units, pv.steps, n, 3);
+  const int sq = (qk.steps + qk.per - 1) / qk.per, sv = (pv.steps + pv.per - 1) / pv.per;
+  p.soff = 0;
+  p.lds = (p.S + 31) & ~31;
+  MoeArena a;
+  const size_t o_acc = a.take<uint64_t>(rows * HD), o_max = a.take<uint32_t>(rows), o_sum = a.take<int32_t>(rows),
+               o_sc = a.take<int32_t>(rows * p.lds), o_e = a.take<uint16_t>(int64_t(units) * p.Pp * PTC_ROWS),
+               o_part = a.take<int64_t>(int64_t(sv) * units * HD * PTC_ROWS);
+  TRY(ensure(ctx->pfx, a.off));
+  uint8_t* ws = static_cast<uint8_t*>(ctx->pfx.p);
+  p.acc = reinterpret_cast<unsigned long long*>(ws + o_acc);
+  p.rowmax = reinterpret_cast<unsigned*>(ws + o_max);
+  p.rowsum = reinterpret_cast<int32_t*>(ws + o_sum);
+  p.scores = reinterpret_cast<int32_t*>(ws + o_sc);
+  qk.e = pv.e = reinterpret_cast<uint4*>(ws + o_e);
+  pv.part = reinterpret_cast<int64_t*>(ws + o_part);
+  using Cfg = PtcCfg<HD>;
+  const void *f0 = reinterpret_cast<const void*>(&prefix_qk_kernel<HD, 0>),
+             *f1 = reinterpret_cast<const void*>(&prefix_qk_kernel<HD, 1>),
+             *f2 = reinterpret_cast<const void*>(&prefix_pv_kernel<HD>);
+  TRY(kernel_smem_occupancy(ctx->device, f0, PTC_THREADS, Cfg::QK_SMEM, nullptr));
+  TRY(kernel_smem_occupancy(ctx->device, f1, PTC_THREADS, Cfg::QK_SMEM, nullptr));
+  TRY(kernel_smem_occupancy(ctx->device, f2, PTC_THREADS, Cfg::PV_SMEM, nullptr));
+  const unsigned gy = unsigned(p.nkv * ((p.T * p.G + PFX_ROWS - 1) / PFX_ROWS));
+  const int t1 = (p.S + PFX_SKEYS - 1) / PFX_SKEYS, t3 = (p.S + PFX_VKEYS - 1) / PFX_VKEYS;
+  const unsigned flat = unsigned(std::min<int64_t>((rows * p.hd + 255) / 256, int64_t(ctx->num_sms) * 8));
+  LaunchCfg l0(ctx, dim3(flat), dim3(256), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l0.cfg, prefix_init_kernel, p, rows));
+  if (p.S > 0) {
+    LaunchCfg l(ctx, dim3(unsigned(p.B * t1), gy), dim3(PFX_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_scores_kernel, p, 0, t1));
+  }
+  LaunchCfg l1(ctx, dim3(unsigned(sq), unsigned(units)), dim3(PTC_THREADS), Cfg::QK_SMEM, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 0>, pf->tm_kh, pf->tm_kl, p, qk));
+  if (p.S > 0) {
+    LaunchCfg l(ctx, dim3(unsigned(rows)), dim3(PFX_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_sum_kernel, p, 0));
+  }
+  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 1>, pf->tm_kh, pf->tm_kl, p, qk));
+  if (p.S > 0) {
+    LaunchCfg l(ctx, dim3(unsigned(p.B * t3), gy), dim3(PFX_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_values_kernel, p, 0, t3));
+  }
+  LaunchCfg l2(ctx, dim3(unsigned(sv), unsigned(units)), dim3(PTC_THREADS), Cfg::PV_SMEM, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_pv_kernel<HD>, pf->tm_vh, pf->tm_vl, p, pv));
+  LaunchCfg l3(ctx, dim3(unsigned(std::min<int64_t>(int64_t(units) * HD * PTC_ROWS / 256, int64_t(ctx->num_sms) * 16))),
+               dim3(256), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_join_kernel, p, pv, units, sv));
+  ctx->launches += p.S > 0 ? 8 : 5;
+  return MYL_OK;
+}
+
 // The attention of `p` (pointers, shapes and plan filled in) with the
 // context's workspace, which the caller holds.
-int run_prefix_attention(myl_ctx* ctx, PrefixParams& p, cudaStream_t st) {
+int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix* pf, PrefixParams& p,
+                         cudaStream_t st) {
   const int64_t rows = int64_t(p.nkv) * p.R;
+  p.err = ctx->d_err;
+  const unsigned gy = unsigned(p.nkv * ((p.R + PFX_ROWS - 1) / PFX_ROWS));
+  if (gy > 65535u) return fail(MYL_ERR_UNSUPPORTED, "%d query rows per KV head", p.R);
+  if (pl->tc && p.P > 0 && p.R >= PTC_MIN_ROWS && (p.hd == 64 || p.hd == 128))
+    return p.hd == 128 ? run_prefix_tc<128>(ctx, pl, pf, p, st) : run_prefix_tc<64>(ctx, pl, pf, p, st);
+  p.soff = p.Pp;
   p.lds = p.Pp + ((p.S + 31) & ~31);
   const size_t o_max = size_t(rows) * size_t(p.hd) * 8, o_sum = o_max + size_t(rows) * 4,
                o_sc = (o_sum + size_t(rows) * 4 + 255) & ~size_t(255);
@@ -118,7 +239,6 @@ int run_prefix_attention(myl_ctx* ctx, PrefixParams& p, cudaStream_t st) {
   p.rowmax = reinterpret_cast<unsigned*>(ws + o_max);
   p.rowsum = reinterpret_cast<int32_t*>(ws + o_sum);
   p.scores = reinterpret_cast<int32_t*>(ws + o_sc);
-  p.err = ctx->d_err;
   const unsigned flat = unsigned(std::min<int64_t>((rows * p.hd + 255) / 256, int64_t(ctx->num_sms) * 8));
   {
     LaunchCfg lc(ctx, dim3(flat), dim3(256), 0, st);
@@ -126,13 +246,11 @@ int run_prefix_attention(myl_ctx* ctx, PrefixParams& p, cudaStream_t st) {
     ctx->launches++;
   }
   if (p.P > 0 || p.S > 0) {
-    const unsigned gy = unsigned(p.nkv * ((p.R + PFX_ROWS - 1) / PFX_ROWS));
-    if (gy > 65535u) return fail(MYL_ERR_UNSUPPORTED, "%d query rows per KV head", p.R);
     const int nb1 = (p.P + PFX_SKEYS - 1) / PFX_SKEYS, t1 = (p.S + PFX_SKEYS - 1) / PFX_SKEYS;
     LaunchCfg l1(ctx, dim3(unsigned(nb1 + p.B * t1), gy), dim3(PFX_THREADS), 0, st);
     CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_scores_kernel, p, nb1, t1));
     LaunchCfg l2(ctx, dim3(unsigned(rows)), dim3(PFX_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_sum_kernel, p));
+    CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_sum_kernel, p, p.P));
     const int nb3 = (p.P + PFX_VKEYS - 1) / PFX_VKEYS, t3 = (p.S + PFX_VKEYS - 1) / PFX_VKEYS;
     LaunchCfg l3(ctx, dim3(unsigned(nb3 + p.B * t3), gy), dim3(PFX_THREADS), 0, st);
     CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_values_kernel, p, nb3, t3));
@@ -326,7 +444,7 @@ int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_
   TRY(ws_acquire(ctx, st));
   {
     PdlScope pdl(ctx);
-    TRY(run_prefix_attention(ctx, p, st));
+    TRY(run_prefix_attention(ctx, plan, prefix, p, st));
   }
   return ws_release(ctx, st);
 }
