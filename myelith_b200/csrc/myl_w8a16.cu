@@ -17,6 +17,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -134,7 +135,7 @@ struct myl_ctx {
   int pdl = 0;         // launch with programmatic stream serialization (the forward's chains)
   int64_t launches = 0;
   PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-  DevBuf x, y, rq, planes, part, h, hplanes, moe, xsum, crc, pfx, ad_h, vfy, vfy_done;
+  DevBuf x, y, rq, planes, part, h, hplanes, moe, xsum, crc, pfx, pfx_stat, ad_h, vfy, vfy_done;
   // Host-pointer calls on page-locked memory: copy-in and copy-out streams
   // and one event pair per chunk.
   cudaStream_t s_in = nullptr, s_out = nullptr;
@@ -891,7 +892,7 @@ int myl_destroy(myl_ctx* ctx) {
   for (auto& kv : ctx->backend_cache) myl_weight_release(ctx, kv.second);
   ctx->backend_cache.clear();
   for (DevBuf* b : {&ctx->x, &ctx->y, &ctx->rq, &ctx->planes, &ctx->part, &ctx->h, &ctx->hplanes,
-                    &ctx->moe, &ctx->xsum, &ctx->crc, &ctx->pfx, &ctx->ad_h, &ctx->vfy, &ctx->vfy_done})
+                    &ctx->moe, &ctx->xsum, &ctx->crc, &ctx->pfx, &ctx->pfx_stat, &ctx->ad_h, &ctx->vfy, &ctx->vfy_done})
     if (b->p) cudaFree(b->p);
   if (ctx->d_err) cudaFree(ctx->d_err);
   if (ctx->h_err) cudaFreeHost(ctx->h_err);

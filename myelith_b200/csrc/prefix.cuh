@@ -19,9 +19,9 @@
 // values transposed [kv head][hd][position], positions padded with zeros to a
 // multiple of PFX_PAD. Rows of a KV head g are numbered
 // rho = (b * T + t) * G + (h - g * G), R = B * T * G of them; score rows are
-// g * R + rho, prefix scores in columns [0, P), suffix scores from column soff.
-// The kernels here run any head size and few rows; prefix_tc.cuh has the prefix
-// part for many rows, with these kernels on the suffixes.
+// g * R + rho, prefix scores in columns [0, P), suffix scores from column Pp.
+// The kernels here run any head size and few rows; prefix_tc.cuh has the ones
+// for many rows (there the score rows hold the suffix alone).
 #pragma once
 
 #include "common.cuh"
@@ -53,7 +53,7 @@ struct PrefixParams {
   int32_t exp_len;
   int lut_shift, prob_frac, out_shift;
   int32_t* scores;  // [nkv * R][lds]
-  int64_t lds, soff;
+  int64_t lds;
   unsigned* rowmax;  // [nkv * R] as max (score ^ 0x80000000)
   int32_t* rowsum;
   unsigned long long* acc;  // [nkv * R][hd] int64 sums (two's complement)
@@ -71,6 +71,7 @@ __device__ __forceinline__ int pfx_len(const PrefixParams& p, int b) {
   }
   return n;
 }
+__device__ __forceinline__ int pfx_clamped(const PrefixParams& p, int b) { return min(max(p.lens[b], 0), p.S); }
 // Suffix entries that token t of a request with n entries sees.
 __device__ __forceinline__ int pfx_seen(const PrefixParams& p, int n, int t) { return max(0, n - p.T + t + 1); }
 
@@ -133,7 +134,7 @@ __global__ void prefix_init_kernel(PrefixParams p, int64_t rows) {
   const int64_t n = rows * p.hd;
   for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
     p.acc[i] = 0;
-    if (i < rows) p.rowmax[i] = 0, p.rowsum[i] = 0;
+    if (i < rows) p.rowmax[i] = 0;
   }
 }
 
@@ -203,7 +204,7 @@ __device__ __forceinline__ void prefix_scores_block(const PrefixParams& p, int g
   if (SUFFIX && mine) mine = j < pfx_seen(p, n_b, (rho / p.G) % p.T);
   if (mine) {
     sc = pfx_score(p, int64_t(sh) * 256 + int64_t(sl));
-    p.scores[(int64_t(g) * p.R + rho) * p.lds + (SUFFIX ? p.soff : 0) + j] = sc;
+    p.scores[(int64_t(g) * p.R + rho) * p.lds + (SUFFIX ? p.Pp : 0) + j] = sc;
   }
   int32_t mx = sc;
 #pragma unroll
@@ -241,8 +242,7 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_scores_kernel(PrefixParams
 }
 
 // ---- pass 2: exponential sums, one block per row ----------------------------------------
-// P0: prefix scores of the row to sum (0 where the tensor-core path sums them).
-__global__ void __launch_bounds__(PFX_THREADS) prefix_sum_kernel(PrefixParams p, int P0) {
+__global__ void __launch_bounds__(PFX_THREADS) prefix_sum_kernel(PrefixParams p) {
   pdl_wait();
   pdl_launch();
   __shared__ int32_t s_red[PFX_THREADS / 32];
@@ -252,14 +252,14 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_sum_kernel(PrefixParams p,
   const int32_t m = int32_t(p.rowmax[row] ^ 0x80000000u);
   const int32_t* sc = p.scores + row * p.lds;
   int32_t s = 0;  // the host bounds the keys so that the i32 sum cannot overflow
-  for (int j = threadIdx.x; j < P0; j += PFX_THREADS) s += pfx_exp(p, m, sc[j]);
-  for (int j = threadIdx.x; j < n; j += PFX_THREADS) s += pfx_exp(p, m, sc[p.soff + j]);
+  for (int j = threadIdx.x; j < p.P; j += PFX_THREADS) s += pfx_exp(p, m, sc[j]);
+  for (int j = threadIdx.x; j < n; j += PFX_THREADS) s += pfx_exp(p, m, sc[p.Pp + j]);
   s = __reduce_add_sync(0xffffffffu, s);
   if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < PFX_THREADS / 32; ++w) s += s_red[w];
-    if (s) atomicAdd(p.rowsum + row, s);
+    p.rowsum[row] = s;
   }
 }
 
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_values_kernel(PrefixParams
       const int64_t row = int64_t(g) * p.R + rho;
       if (j < (suffix ? pfx_seen(p, n_b, (rho / p.G) % p.T) : p.P)) {
         const int32_t m = int32_t(p.rowmax[row] ^ 0x80000000u);
-        const int32_t ex = pfx_exp(p, m, p.scores[row * p.lds + (suffix ? p.soff : 0) + j]);
+        const int32_t ex = pfx_exp(p, m, p.scores[row * p.lds + (suffix ? p.Pp : 0) + j]);
         pr = uint32_t(softmax_prob(ex, p.rowsum[row], 0, 1, int32_t(one)));
       }
     }

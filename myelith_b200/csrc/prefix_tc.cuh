@@ -3,24 +3,31 @@
 //
 // A tile is 128 query rows of one KV head (TMEM lane = row). Operands are
 // bytes: q = 256 qh + ql (qh signed), k + 32768 = 256 kh + kl (both unsigned,
-// as the prefix stores them), so for 64 keys one kind::i8 MMA of qh and one of
-// ql against the 128 stacked byte rows [kh | kl] give hh, hl, lh, ll and
+// as the prefix stores them), so for 32 keys one kind::i8 MMA of qh and one of
+// ql against the 64 stacked byte rows [kh | kl] give hh, hl, lh, ll and
 //   dot = 256 (256 hh + hl + lh) + ll - 32768 sum(q)
 // with every int32 sum exact (|hh| <= 128 * 128 * 255 at hd = 128). In the same
 // way p = 256 ph + pl and v + 32768 = 256 vh + vl give the weighted values. A
 // row's probabilities sum to less than 2^17, so the value sums stay inside
 // int32 over a whole row and TMEM accumulates them without a flush.
 //
-// The score of a row is one multiply-add chain: with per-row constants,
-//   V = t * (256 mult) + ll * mult + (2^(shift-1) - 32768 mult sum(q)),
-// t = 256 hh + hl + lh, is the shifted-up score plus half a unit; the low word
-// of V >> shift is the rounded score, made even when the bits below vanish.
+// The score needs no integer rounding: the 64-bit pattern of the double
+// 1.5 * 2^52 is added to dot with two wide multiply-adds, which makes the bits
+// the double X = 1.5 * 2^52 + dot (|dot| < 2^38), and
+//   fma(X, mult * 2^-shift, 1.5 * 2^52 * (1 - mult * 2^-shift))
+// is dot * mult * 2^-shift + 1.5 * 2^52 rounded once, to an integer with ties to
+// even: its low word is the score as i32, wrap-around included. The constant is
+// an exact integer for 0 <= mult <= 2^shift, shift <= 51.
 //
 // The maximum of a row must be known before the first exponential, and the sum
 // before the first probability, so the keys pass three times:
+//   prefix_suffix_kernel     suffix scores and maxima
 //   prefix_qk_kernel<HD, 0>  scores -> row maxima
 //   prefix_qk_kernel<HD, 1>  scores again -> exponentials (16 bits) and row sums
+//                            (the suffix's included)
+//   prefix_suffix_values_kernel  the suffix's weighted values
 //   prefix_pv_kernel<HD>     exponentials -> probabilities -> weighted values
+//   prefix_join_kernel       sum of the splits and suffix tiles, output
 // Computing the scores twice costs less than writing them as int32 and reading
 // them back (4 + 4 bytes a score against 2 MMA byte products per dimension).
 #pragma once
@@ -30,26 +37,34 @@
 namespace myl {
 
 constexpr int PTC_ROWS = 128;
-constexpr int PTC_KEYS = 64;        // keys per scores step
+constexpr int PTC_KEYS = 32;        // keys per scores step
+constexpr int PTC_BUFS = 3;         // TMEM score buffers
 constexpr int PTC_VKEYS = 128;      // keys per values step
-constexpr int PTC_WARPS = 16;       // worker warps: TMEM lane quarter x column quarter
-constexpr int PTC_THREADS = 64 + 32 * PTC_WARPS;
+constexpr int PTC_QK_WARPS = 4 * PTC_BUFS;  // worker warps: buffer x TMEM lane quarter
+constexpr int PTC_PV_WARPS = 16;    // TMEM lane quarter x column quarter
+constexpr int PTC_QK_THREADS = 64 + 32 * PTC_QK_WARPS;
+constexpr int PTC_PV_THREADS = 64 + 32 * PTC_PV_WARPS;
+constexpr int PTC_SFX_KEYS = 128;   // suffix keys per block
+constexpr int PTC_JOIN_DIMS = PFX_THREADS / PFX_ROWS;  // dimensions per block of the last kernel
 constexpr int PTC_LUT_MAX = 16384;  // exponential table entries in shared memory
 
 struct PrefixTc {
   int RT;      // row tiles per KV head
   int steps;   // steps of the kernel's keys over all of Pp
   int per;     // steps per block
+  double scale, offset;  // of a score, see above
+  int k256, k1;          // 256 and 1, kept from being folded: one multiply-add beats shifts and carries
+  int early;   // the scores kernel does not have to wait before its set-up
   int cap;     // largest table index looked up
   int lut_n;   // entries copied to shared memory (the one at cap included)
-  uint4* e;    // exponentials [unit][64-key block][16-key group][128 rows][16] u16
+  uint4* e;    // exponentials [unit][16-key group][128 rows][16] u16
   int64_t* part;  // value sums [split][unit][hd][128 rows]
   uint64_t timeout_ns;
 };
 
 struct PrefixCtl {
-  uint64_t full[8], empty[8];
-  uint64_t tfull[2], tempty[2];
+  uint64_t full[12], empty[12];
+  uint64_t tfull[PTC_BUFS], tempty[PTC_BUFS];
   uint32_t tmem_base;
   int abort;
   int rowval[PTC_ROWS];  // sum(q), or a row's sum of probabilities
@@ -57,13 +72,12 @@ struct PrefixCtl {
 
 template <int HD>
 struct PtcCfg {
-  static constexpr int A_BYTES = PTC_ROWS * HD;                   // one query plane
   static constexpr int K_STAGE = 2 * PTC_KEYS * HD;               // kh and kl of a step
-  static constexpr int K_STAGES = 6;
+  static constexpr int K_STAGES = 12;
   static constexpr int P_BYTES = PTC_ROWS * PTC_VKEYS;            // one probability plane
   static constexpr int V_STAGE = 2 * HD * PTC_VKEYS;              // vh and vl of a step
   static constexpr int V_STAGES = 3;
-  static constexpr int QK_SMEM = 2 * A_BYTES + K_STAGES * K_STAGE + 2 * (PTC_LUT_MAX + 8) + 1024;
+  static constexpr int QK_SMEM = K_STAGES * K_STAGE + 2 * (PTC_LUT_MAX + 8) + 1024;
   static constexpr int PV_SMEM = 4 * P_BYTES + V_STAGES * V_STAGE + 1024;
   static_assert(QK_SMEM <= 227 * 1024 - 1536 && PV_SMEM <= 227 * 1024 - 1536, "shared memory");
 };
@@ -83,11 +97,15 @@ __device__ __forceinline__ uint64_t ptc_desc(uint32_t saddr) {
   return d;
 }
 
-// Byte offset of (row, byte) in such a tile.
-template <int HD>
+// Byte offset of (row, byte) in a tile of 128-byte rows.
 __device__ __forceinline__ uint32_t ptc_at(int row, int byte) {
-  if constexpr (HD == 128) return uint32_t(row * 128 + ((((byte >> 4) ^ row) & 7) << 4) + (byte & 15));
-  return uint32_t(row * 64 + ((((byte >> 4) ^ (row >> 1)) & 3) << 4) + (byte & 15));
+  return uint32_t(row * 128 + ((((byte >> 4) ^ row) & 7) << 4) + (byte & 15));
+}
+
+__device__ __forceinline__ int64_t mad_wide(int32_t a, int32_t b, int64_t c) {
+  int64_t d;
+  asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(d) : "r"(a), "r"(b), "l"(c));
+  return d;
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -99,7 +117,7 @@ __device__ __forceinline__ void ptc_setup(PrefixCtl& ctl, int stages, int full_c
       mbar_init(smem_addr(&ctl.full[s]), 1);
       mbar_init(smem_addr(&ctl.empty[s]), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < PTC_BUFS; ++b) {
       mbar_init(smem_addr(&ctl.tfull[b]), uint32_t(full_count));
       mbar_init(smem_addr(&ctl.tempty[b]), uint32_t(tempty_count));
     }
@@ -123,15 +141,22 @@ __device__ __forceinline__ void ptc_drain(PrefixCtl& ctl, int issued, int stages
 }
 
 // MODE 0: row maxima; MODE 1: exponentials and row sums. grid.x: key range,
-// grid.y: unit (kv head * RT + row tile). Warp 0 loads key planes with TMA,
-// warp 1 issues the MMAs into two TMEM buffers [hh | hl | lh | ll] of 64 columns
-// each, 16 warps turn scores into their output: warp (q, c) has rows 32 q.. and
-// keys 16 c.. of a step, a thread one row.
+// grid.y: unit (kv head * RT + row tile). The query planes lie in TMEM, so an MMA
+// reads only its 64 key byte rows from shared memory (operand bytes from shared
+// memory, about 70 a clock here, set the pace of small MMAs: with the queries
+// there too, steps of 64 keys took 930 clocks instead of the 512 of the pipe).
+// Warp 0 loads key planes with TMA, warp 1 issues the MMAs into three score
+// buffers [hh | hl | lh | ll] of 32 columns each, and each buffer has four warps
+// that turn its scores into their output, so that three steps are worked on at
+// a time: warp (buffer, q) has rows 32 q.. of every third step, a thread one
+// row. In MODE 1 the blocks of a unit also share out its rows' suffix sums.
 template <int HD, int MODE>
-__global__ void __launch_bounds__(PTC_THREADS, 1)
+__global__ void __launch_bounds__(PTC_QK_THREADS, 1)
     prefix_qk_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant__ CUtensorMap tm_kl,
                      PrefixParams p, PrefixTc tc) {
-  pdl_wait();
+  // early: the kernel before this one belongs to the same call, so everything
+  // but the row statistics and the exponentials is in place already
+  if (!tc.early) pdl_wait();
   pdl_launch();
   using Cfg = PtcCfg<HD>;
   constexpr int ST = Cfg::K_STAGES;
@@ -139,36 +164,45 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
   __shared__ PrefixCtl ctl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* const base = dyn_smem + ((1024u - (smem_addr(dyn_smem) & 1023u)) & 1023u);
-  uint8_t *const a_hi = base, *const a_lo = base + Cfg::A_BYTES;
-  const uint32_t ring = smem_addr(base) + 2 * Cfg::A_BYTES;
-  uint16_t* const s_lut = reinterpret_cast<uint16_t*>(base + 2 * Cfg::A_BYTES + ST * Cfg::K_STAGE);
+  const uint32_t ring = smem_addr(base);
+  uint16_t* const s_lut = reinterpret_cast<uint16_t*>(base + ST * Cfg::K_STAGE);
   volatile int* abort = &ctl.abort;
   const int unit = int(blockIdx.y), g = unit / tc.RT, row0 = (unit % tc.RT) * PTC_ROWS;
   const int i0 = int(blockIdx.x) * tc.per, n = min(tc.per, tc.steps - i0);
 
-  ptc_setup(ctl, ST, 1, PTC_WARPS);
-  __syncthreads();
-  // query planes and sums; rows past R are zero
-  for (int e = threadIdx.x; e < PTC_ROWS * (HD / 8); e += PTC_THREADS) {
-    const int r = e / (HD / 8), c = e % (HD / 8), rho = row0 + r;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (rho < p.R)
-      v = *reinterpret_cast<const uint4*>(p.q + int64_t(rho / p.G) * p.ldq + int64_t(g * p.G + rho % p.G) * HD + 8 * c);
-    const uint32_t at = ptc_at<HD>(r, 8 * c);
-    *reinterpret_cast<uint2*>(a_hi + at) = make_uint2(__byte_perm(v.x, v.y, 0x7531), __byte_perm(v.z, v.w, 0x7531));
-    *reinterpret_cast<uint2*>(a_lo + at) = make_uint2(__byte_perm(v.x, v.y, 0x6420), __byte_perm(v.z, v.w, 0x6420));
-    int sum = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sum += lane16(v, k);
-    if (sum) atomicAdd(&ctl.rowval[r], sum);
-  }
-  if (MODE == 1)
-    for (int i = threadIdx.x; i < tc.lut_n; i += PTC_THREADS) s_lut[i] = i < p.exp_len ? uint16_t(p.exp_lut[i]) : uint16_t(0);
-  fence_async_smem();
+  ptc_setup(ctl, ST, 1, 4);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl.tmem_base;
+  const uint32_t tmem = ctl.tmem_base, a_hi = tmem + PTC_BUFS * 128, a_lo = a_hi + HD / 4;
+  // query planes and sums, a thread of the first worker group a row; rows past R are zero
+  if (warp >= 2 && warp < 6) {
+    const int r = 32 * (warp & 3) + lane, rho = row0 + r;
+    const uint4* src = rho < p.R ? reinterpret_cast<const uint4*>(p.q + int64_t(rho / p.G) * p.ldq + int64_t(g * p.G + rho % p.G) * HD) : nullptr;
+    int sum = 0;
+#pragma unroll
+    for (int h = 0; h < HD / 64; ++h) {
+      uint32_t hi[16], lo[16];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint4 v = src ? src[8 * h + c] : make_uint4(0u, 0u, 0u, 0u);
+        hi[2 * c] = __byte_perm(v.x, v.y, 0x7531), hi[2 * c + 1] = __byte_perm(v.z, v.w, 0x7531);
+        lo[2 * c] = __byte_perm(v.x, v.y, 0x6420), lo[2 * c + 1] = __byte_perm(v.z, v.w, 0x6420);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += lane16(v, k);
+      }
+      const uint32_t at = (uint32_t(32 * (warp & 3)) << 16) + 16 * h;
+      tmem_st_32x32b_x16(a_hi + at, hi);
+      tmem_st_32x32b_x16(a_lo + at, lo);
+    }
+    tmem_st_wait();
+    ctl.rowval[r] = sum;
+  }
+  if (MODE == 1)
+    for (int i = threadIdx.x; i < tc.lut_n; i += PTC_QK_THREADS) s_lut[i] = i < p.exp_len ? uint16_t(p.exp_lut[i]) : uint16_t(0);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -190,104 +224,121 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t id_h = idesc_i8(128, 2 * PTC_KEYS, true, false), id_l = idesc_i8(128, 2 * PTC_KEYS, false, false);
-      const uint32_t ah = smem_addr(a_hi), al = smem_addr(a_lo);
-      int i = 0;
+      int i = 0, b = 0;
+      uint32_t use = 0;  // parity of the buffers' use
       for (; i < n; ++i) {
-        const int s = i % ST, b = i & 1;
-        if (!mbar_wait_bounded(smem_addr(&ctl.tempty[b]), (uint32_t(i >> 1) & 1u) ^ 1u, tc.timeout_ns, abort) ||
+        const int s = i % ST;
+        if (!mbar_wait_bounded(smem_addr(&ctl.tempty[b]), use ^ 1u, tc.timeout_ns, abort) ||
             !mbar_wait_bounded(smem_addr(&ctl.full[s]), uint32_t(i / ST) & 1u, tc.timeout_ns, abort)) {
           tc_fail(p.err, abort, DEV_WAIT_MMA);
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem + uint32_t(b * 256), kb = ring + uint32_t(s * Cfg::K_STAGE);
+        const uint32_t d = tmem + uint32_t(b * 128), kb = ring + uint32_t(s * Cfg::K_STAGE);
 #pragma unroll
         for (int kk = 0; kk < HD / 32; ++kk) {
           const uint64_t db = ptc_desc<HD>(kb + 32 * kk);
-          mma_i8(d, ptc_desc<HD>(ah + 32 * kk), db, id_h, kk > 0);
-          mma_i8(d + 128, ptc_desc<HD>(al + 32 * kk), db, id_l, kk > 0);
+          mma_i8_ts(d, a_hi + 8 * kk, db, id_h, kk > 0);
+          mma_i8_ts(d + 64, a_lo + 8 * kk, db, id_l, kk > 0);
         }
         mma_commit(smem_addr(&ctl.empty[s]));
         mma_commit(smem_addr(&ctl.tfull[b]));
+        if (++b == PTC_BUFS) b = 0, use ^= 1u;
       }
       // the issued MMAs finish before TMEM is released
-      if (i > 0 && !mbar_wait_bounded(smem_addr(&ctl.tfull[(i - 1) & 1]), uint32_t((i - 1) >> 1) & 1u, tc.timeout_ns, nullptr))
+      if (i > 0 && !mbar_wait_bounded(smem_addr(&ctl.tfull[(i - 1) % PTC_BUFS]), uint32_t((i - 1) / PTC_BUFS) & 1u, tc.timeout_ns, nullptr))
         atomicCAS(p.err, 0, DEV_WAIT_DRAIN);
     }
   } else {
-    const int q = warp & 3, c = (warp - 2) >> 2;
+    const int q = warp & 3, b = (warp - 2) >> 2;
     const int r = 32 * q + lane, rho = row0 + r;
     const bool live = rho < p.R, warp_live = row0 + 32 * q < p.R;
     const int64_t row = int64_t(g) * p.R + rho;
-    const int shift = p.score_shift;
-    const int mult = int(p.score_mult), mult256 = mult * 256;
-    const uint32_t mask = (1u << shift) - 1u;
-    const int64_t c_row = (int64_t(1) << (shift - 1)) - int64_t(ctl.rowval[r]) * 32768 * mult;
+    // the pattern of 1.5 * 2^52, less the unsigned key bytes' share of the dot
+    const int64_t pattern = 0x4338000000000000ll - int64_t(ctl.rowval[r]) * 32768;
+    pdl_wait();
     int32_t mx = INT32_MIN, sum = 0;
     if (MODE == 1 && live) mx = int32_t(p.rowmax[row] ^ 0x80000000u);
-    for (int i = 0; i < n; ++i) {
-      const int b = i & 1;
-      if (!mbar_wait_bounded(smem_addr(&ctl.tfull[b]), uint32_t(i >> 1) & 1u, tc.timeout_ns, abort)) {
+    uint32_t use = 0;
+    for (int i = b; i < n; i += PTC_BUFS, use ^= 1u) {
+      if (!mbar_wait_bounded(smem_addr(&ctl.tfull[b]), use, tc.timeout_ns, abort)) {
         tc_fail(p.err, abort, DEV_WAIT_EPILOGUE);
         break;
       }
       if (*abort) break;
       tc_fence_after();
-      uint32_t hh[16], hl[16], lh[16], ll[16];
-      if (warp_live) {
-        const uint32_t t = tmem + (uint32_t(32 * q) << 16) + uint32_t(b * 256 + 16 * c);
-        tmem_ld_32x32b_x16(t, hh);
-        tmem_ld_32x32b_x16(t + 64, hl);
-        tmem_ld_32x32b_x16(t + 128, lh);
-        tmem_ld_32x32b_x16(t + 192, ll);
-        tmem_ld_wait();
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&ctl.tempty[b]));
-      if (!warp_live) continue;
-      const int kb = i0 + i, left = p.P - kb * PTC_KEYS - 16 * c;  // keys of this group inside the prefix
-      int32_t sc[16];
+      const int kb = i0 + i;
+      const uint32_t t0 = tmem + (uint32_t(32 * q) << 16) + uint32_t(b * 128);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int32_t t = int32_t(hh[j]) * 256 + int32_t(hl[j]) + int32_t(lh[j]);
-        const int64_t v = int64_t(t) * mult256 + (int64_t(int32_t(ll[j])) * mult + c_row);
-        const uint32_t lo = uint32_t(uint64_t(v)), hi = uint32_t(uint64_t(v) >> 32);
-        int32_t s = int32_t(__funnelshift_r(lo, hi, shift));
-        if ((lo & mask) == 0) s &= ~1;  // a tie goes to the even score
-        sc[j] = s;
-      }
-      if (MODE == 0) {
-        if (left >= 16) {
+      for (int h = 0; h < 2; ++h) {
+        uint32_t hh[16], hl[16], lh[16], ll[16];
+        if (warp_live) {
+          tmem_ld_32x32b_x16(t0 + 16 * h, hh);
+          tmem_ld_32x32b_x16(t0 + 16 * h + 32, hl);
+          tmem_ld_32x32b_x16(t0 + 16 * h + 64, lh);
+          tmem_ld_32x32b_x16(t0 + 16 * h + 96, ll);
+          tmem_ld_wait();
+        }
+        if (h == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&ctl.tempty[b]));
+        }
+        if (!warp_live) continue;
+        const int left = p.P - kb * PTC_KEYS - 16 * h;  // keys of this group inside the prefix
+        int32_t sc[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) mx = max(mx, sc[j]);
+        for (int j = 0; j < 16; ++j) {
+          const int32_t t = int32_t(hh[j]) * tc.k256 + (int32_t(hl[j]) + int32_t(lh[j]));
+          const double x = __longlong_as_double(mad_wide(t, tc.k256, mad_wide(int32_t(ll[j]), tc.k1, pattern)));
+          sc[j] = __double2loint(fma(x, tc.scale, tc.offset));
+        }
+        if (MODE == 0) {
+          if (left < 16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sc[j] = j < left ? sc[j] : INT32_MIN;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) mx = max(max(sc[j], sc[j + 1]), mx);
         } else {
+          uint32_t ex[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) mx = j < left ? max(mx, sc[j]) : mx;
+          for (int j = 0; j < 16; ++j)
+            ex[j] = s_lut[min((uint32_t(mx) - uint32_t(sc[j])) >> p.lut_shift, uint32_t(tc.cap))];
+          if (left < 16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) ex[j] = j < left ? ex[j] : 0u;
+          }
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sum += int32_t(ex[2 * j] + ex[2 * j + 1]);
+            w[j] = ex[2 * j] | (ex[2 * j + 1] << 16);
+          }
+          uint4* dst = tc.e + (((int64_t(unit) * tc.steps + kb) * 2 + h) * PTC_ROWS + r) * 2;
+          dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
-      } else {
-        uint32_t ex[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          ex[j] = s_lut[min((uint32_t(mx) - uint32_t(sc[j])) >> p.lut_shift, uint32_t(tc.cap))];
-        if (left < 16) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) ex[j] = j < left ? ex[j] : 0u;
-        }
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          sum += int32_t(ex[2 * j] + ex[2 * j + 1]);
-          w[j] = ex[2 * j] | (ex[2 * j + 1] << 16);
-        }
-        uint4* dst = tc.e + (((int64_t(unit) * tc.steps + kb) * 4 + c) * PTC_ROWS + r) * 2;
-        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
       }
     }
     if (live) {
       if (MODE == 0) atomicMax(p.rowmax + row, uint32_t(mx) ^ 0x80000000u);
       else atomicAdd(p.rowsum + row, sum);
+    }
+    if (MODE == 1 && p.S > 0) {
+      // the suffix's exponentials of this block's share of the rows, a warp per row
+      for (int k = int(blockIdx.x) + (warp - 2) * int(gridDim.x); k < PTC_ROWS; k += PTC_QK_WARPS * int(gridDim.x)) {
+        const int o = row0 + k;
+        if (o >= p.R) break;
+        const int64_t srow = int64_t(g) * p.R + o;
+        const int m = pfx_seen(p, pfx_clamped(p, o / (p.T * p.G)), (o / p.G) % p.T);
+        const int32_t top = int32_t(p.rowmax[srow] ^ 0x80000000u);
+        int32_t s = 0;
+        for (int j = lane; j < m; j += 32)
+          s += s_lut[min((uint32_t(top) - uint32_t(p.scores[srow * p.lds + j])) >> p.lut_shift, uint32_t(tc.cap))];
+        s = __reduce_add_sync(0xffffffffu, s);
+        if (lane == 0 && s) atomicAdd(p.rowsum + srow, s);
+      }
     }
   }
   tc_fence_before();
@@ -303,11 +354,10 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
 // the nearest integer and no tie, and anything else is redone in integers. The
 // byte planes of p go to shared memory as the MMA's A operand.
 template <int HD>
-__global__ void __launch_bounds__(PTC_THREADS, 1)
+__global__ void __launch_bounds__(PTC_PV_THREADS, 1)
     prefix_pv_kernel(const __grid_constant__ CUtensorMap tm_vh, const __grid_constant__ CUtensorMap tm_vl,
                      PrefixParams p, PrefixTc tc) {
-  pdl_wait();
-  pdl_launch();
+  pdl_launch();  // never a call's first kernel: only the workers have to wait
   using Cfg = PtcCfg<HD>;
   constexpr int ST = Cfg::V_STAGES;
   extern __shared__ uint8_t dyn_smem[];
@@ -320,7 +370,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
   const int i0 = int(blockIdx.x) * tc.per, n = min(tc.per, tc.steps - i0);
 
   // tfull / tempty: probability buffers written (16 warps) / consumed (a commit)
-  ptc_setup(ctl, ST, PTC_WARPS, 1);
+  ptc_setup(ctl, ST, PTC_PV_WARPS, 1);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -374,6 +424,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
     const int r = 32 * q + lane, rho = row0 + r;
     const bool live = rho < p.R;
     const int64_t row = int64_t(g) * p.R + rho;
+    pdl_wait();
     const int32_t S = live ? p.rowsum[row] : 1;
     const uint32_t one = 1u << p.prob_frac;
     const float ratio = float(one) / float(S);
@@ -384,8 +435,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
     int psum = 0;
     bool ok = true;
     auto load = [&](int i, uint4 (&x)[4]) {
-      const int kb = 2 * (i0 + i) + (c >> 1);
-      const uint4* src = tc.e + (((int64_t(unit) * (2 * tc.steps) + kb) * 4 + 2 * (c & 1)) * PTC_ROWS + r) * 2;
+      const uint4* src = tc.e + ((int64_t(unit) * tc.steps + i0 + i) * 8 + 2 * c) * PTC_ROWS * 2 + 2 * r;
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         x[u] = live ? __ldcs(src + (u >> 1) * PTC_ROWS * 2 + (u & 1)) : make_uint4(0u, 0u, 0u, 0u);
@@ -436,7 +486,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
       uint8_t* dst = base + 2 * b * Cfg::P_BYTES;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t at = ptc_at<128>(r, 32 * c + 16 * h);
+        const uint32_t at = ptc_at(r, 32 * c + 16 * h);
         *reinterpret_cast<uint4*>(dst + at) = make_uint4(ph[4 * h], ph[4 * h + 1], ph[4 * h + 2], ph[4 * h + 3]);
         *reinterpret_cast<uint4*>(dst + Cfg::P_BYTES + at) = make_uint4(pl[4 * h], pl[4 * h + 1], pl[4 * h + 2], pl[4 * h + 3]);
       }
@@ -448,7 +498,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
     }
     atomicAdd(&ctl.rowval[r], psum);
     // all of the block's probabilities are counted (worker warps only), the last MMAs done
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * PTC_WARPS) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * PTC_PV_WARPS) : "memory");
     if (ok && n > 0)
       ok = mbar_wait_bounded(smem_addr(&ctl.tempty[(n - 1) & 1]), uint32_t((n - 1) >> 1) & 1u, tc.timeout_ns, abort);
     if (ok && !*abort && row0 + 32 * q < p.R) {
@@ -478,21 +528,195 @@ __global__ void __launch_bounds__(PTC_THREADS, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// Sums the splits (and the suffix's share), rounds, rescales. One thread per
-// (unit, dimension, row), rows fastest as the value sums lie.
-__global__ void __launch_bounds__(256) prefix_join_kernel(PrefixParams p, PrefixTc tc, int units, int splits) {
+// The suffixes' scores and row maxima: a block per (PTC_SFX_KEYS keys, KV head
+// and PFX_ROWS query rows, request). 8 threads a key (part s: the 8-element
+// chunks s, s + 8, ...); a thread ends up with one row's scores of its keys.
+__global__ void __launch_bounds__(PFX_THREADS) prefix_suffix_kernel(PrefixParams p) {
   pdl_wait();
   pdl_launch();
-  const int64_t per = int64_t(p.hd) * PTC_ROWS, n = units * per;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
-    const int unit = int(i / per), d = int(i % per) / PTC_ROWS, r = int(i % PTC_ROWS);
-    const int g = unit / tc.RT, rho = (unit % tc.RT) * PTC_ROWS + r;
-    if (rho >= p.R) continue;
-    int64_t tot = p.S > 0 ? int64_t(p.acc[(int64_t(g) * p.R + rho) * p.hd + d]) : 0;
-    for (int s = 0; s < splits; ++s) tot += __ldcs(tc.part + s * n + i);
-    int32_t o = clamp16(p.prob_frac > 0 ? rshift_rne_i64(tot, p.prob_frac) : tot);
-    if (p.out_shift != 0) o = clamp16(rescale_i32_s(o, p.out_shift));
-    p.out[int64_t(rho / p.G) * p.ldo + int64_t(g * p.G + rho % p.G) * p.hd + d] = int16_t(o);
+  constexpr int KEYS = PFX_THREADS / 8, ITER = PTC_SFX_KEYS / KEYS;
+  __shared__ __align__(16) int16_t s_q[PFX_ROWS * 128];
+  __shared__ int32_t s_mx[PFX_THREADS / 32][PFX_ROWS];
+  const int b = int(blockIdx.z), g = int(blockIdx.y) % p.nkv, r0 = int(blockIdx.y) / p.nkv * PFX_ROWS;
+  const int n = pfx_len(p, b), nc8 = p.hd / 8, j0 = int(blockIdx.x) * PTC_SFX_KEYS;
+  if (j0 >= n) return;
+  const int jj = int(threadIdx.x) / 8, part = int(threadIdx.x) % 8;
+  const int16_t* kbase = p.ks + b * p.seq_stride + g * p.head_stride + 8 * part;
+  uint4 kv[ITER][2];
+#pragma unroll
+  for (int t = 0; t < ITER; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = j0 + t * KEYS + jj;
+      kv[t][i] = j < n && part + 8 * i < nc8 ? *reinterpret_cast<const uint4*>(kbase + j * p.pos_stride + 64 * i)
+                                             : make_uint4(0u, 0u, 0u, 0u);
+    }
+  const int per = p.T * p.G, nrow = min(PFX_ROWS, per - r0), rho0 = b * per + r0;
+  for (int e = threadIdx.x; e < PFX_ROWS * nc8; e += PFX_THREADS) {
+    const int rho = rho0 + e / nc8;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (e / nc8 < nrow)
+      v = *reinterpret_cast<const uint4*>(p.q + int64_t(rho / p.G) * p.ldq + int64_t(g * p.G + rho % p.G) * p.hd + 8 * (e % nc8));
+    reinterpret_cast<uint4*>(s_q)[e] = v;
+  }
+  __syncthreads();
+  const int rho = rho0 + part;  // this thread's row after the reduce-scatter
+  const int seen = part < nrow ? pfx_seen(p, n, (rho / p.G) % p.T) : 0;
+  int32_t* dst = p.scores + (int64_t(g) * p.R + rho) * p.lds;
+  int32_t mx = INT32_MIN;
+#pragma unroll
+  for (int t = 0; t < ITER; ++t) {
+    if (j0 + t * KEYS >= n) break;
+    int ah[PFX_ROWS], al[PFX_ROWS];
+#pragma unroll
+    for (int r = 0; r < PFX_ROWS; ++r) ah[r] = al[r] = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 w = kv[t][i];
+      const uint32_t hx = __byte_perm(w.x, w.y, 0x7531), hy = __byte_perm(w.z, w.w, 0x7531);
+      const uint32_t lx = __byte_perm(w.x, w.y, 0x6420), ly = __byte_perm(w.z, w.w, 0x6420);
+      const int c = part + 8 * i;
+      if (c < nc8) {
+#pragma unroll
+        for (int r = 0; r < PFX_ROWS; ++r) {
+          const uint4 q = reinterpret_cast<const uint4*>(s_q)[r * nc8 + c];
+          ah[r] = dp2a_hi_ss(q.y, hx, dp2a_lo_ss(q.x, hx, ah[r]));
+          ah[r] = dp2a_hi_ss(q.w, hy, dp2a_lo_ss(q.z, hy, ah[r]));
+          al[r] = dp2a_hi_su(q.y, lx, dp2a_lo_su(q.x, lx, al[r]));
+          al[r] = dp2a_hi_su(q.w, ly, dp2a_lo_su(q.z, ly, al[r]));
+        }
+      }
+    }
+    const int sh = att_reduce_scatter8(ah, part), sl = att_reduce_scatter8(al, part);
+    const int j = j0 + t * KEYS + jj;
+    if (j < seen) {
+      const int32_t sc = pfx_score(p, int64_t(sh) * 256 + int64_t(sl));
+      dst[j] = sc;
+      mx = max(mx, sc);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if ((threadIdx.x & 31) < 8) s_mx[threadIdx.x >> 5][part] = mx;
+  __syncthreads();
+  if (int(threadIdx.x) < nrow) {
+    int32_t m = s_mx[0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < PFX_THREADS / 32; ++w) m = max(m, s_mx[w][threadIdx.x]);
+    if (m != INT32_MIN) atomicMax(p.rowmax + int64_t(g) * p.R + rho0 + threadIdx.x, uint32_t(m) ^ 0x80000000u);
+  }
+}
+
+// The suffixes' probability-weighted values: a block per (PTC_SFX_KEYS keys, KV
+// head and PFX_ROWS query rows, request), its value rows in registers (a thread
+// 8 dimensions of PTC_SFX_KEYS * hd / 2048 keys). The
+// int32 sums hold: the keys carry at most 2^15 + 64 of probability. They go to
+// sums [tile][row][hd].
+template <int HD>
+__global__ void __launch_bounds__(PFX_THREADS) prefix_suffix_values_kernel(PrefixParams p, int32_t* sums, int64_t rows) {
+  pdl_launch();
+  constexpr int TPK = HD / 8, GROUPS = PFX_THREADS / TPK, PER = PTC_SFX_KEYS / GROUPS, WARPS = PFX_THREADS / 32;
+  __shared__ __align__(16) uint16_t s_p[PTC_SFX_KEYS][PFX_ROWS];
+  __shared__ __align__(16) int32_t s_part[WARPS][PFX_ROWS][HD];
+  const int b = int(blockIdx.z), g = int(blockIdx.y) % p.nkv, r0 = int(blockIdx.y) / p.nkv * PFX_ROWS, j0 = int(blockIdx.x) * PTC_SFX_KEYS;
+  const int n = pfx_len(p, b);
+  if (j0 >= n) return;
+  const int kg = int(threadIdx.x) / TPK, d8 = int(threadIdx.x) % TPK, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int16_t* vbase = p.vs + b * p.seq_stride + g * p.head_stride + 8 * d8;
+  uint4 v[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int j = j0 + kg + u * GROUPS;
+    v[u] = j < n ? *reinterpret_cast<const uint4*>(vbase + j * p.pos_stride) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  pdl_wait();  // the row sums (never a call's first kernel: the inputs are in place)
+  const int32_t one = int32_t(1) << p.prob_frac;
+  const int per = p.T * p.G;
+  const int nrow = min(PFX_ROWS, per - r0), rho0 = b * per + r0;
+  const int64_t row0 = int64_t(g) * p.R + rho0;
+  {  // probabilities: a warp's 32 lanes take 4 keys of each of the 8 rows
+    const int r = lane % PFX_ROWS;
+    const bool live = r < nrow;
+    const int seen = live ? pfx_seen(p, n, ((rho0 + r) / p.G) % p.T) - j0 : 0;
+    const int32_t S = live ? p.rowsum[row0 + r] : 1;
+    const int32_t top = live ? int32_t(p.rowmax[row0 + r] ^ 0x80000000u) : 0;
+    const uint64_t recip = softmax_recip(S);
+    const int32_t* sc = p.scores + (row0 + r) * p.lds + j0;
+#pragma unroll
+    for (int u = 0; u < PTC_SFX_KEYS * PFX_ROWS / PFX_THREADS; ++u) {
+      const int jj = (u * WARPS + warp) * (32 / PFX_ROWS) + lane / PFX_ROWS;
+      const int32_t ex = jj < seen ? pfx_exp(p, top, sc[jj]) : 0;
+      s_p[jj][r] = uint16_t(softmax_prob_r(ex, S, recip, 0, 1, one));
+    }
+  }
+  __syncthreads();
+  int32_t acc[PFX_ROWS][8];
+#pragma unroll
+  for (int r = 0; r < PFX_ROWS; ++r)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[r][e] = 0;
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const uint4 pw = *reinterpret_cast<const uint4*>(&s_p[kg + u * GROUPS][0]);
+    const uint32_t pr[4] = {pw.x, pw.y, pw.z, pw.w};
+    int32_t ve[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ve[e] = lane16(v[u], e);
+#pragma unroll
+    for (int r = 0; r < PFX_ROWS; ++r) {
+      const int32_t pj = int32_t((r & 1) ? pr[r / 2] >> 16 : pr[r / 2] & 0xFFFFu);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[r][e] += pj * ve[e];
+    }
+  }
+  // the warp's key groups (32 / TPK of them), then the warps'
+#pragma unroll
+  for (int r = 0; r < PFX_ROWS; ++r) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int o = TPK; o < 32; o <<= 1) acc[r][e] += __shfl_xor_sync(0xffffffffu, acc[r][e], o);
+    if (lane < TPK) {
+      *reinterpret_cast<int4*>(&s_part[warp][r][8 * d8]) = make_int4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+      *reinterpret_cast<int4*>(&s_part[warp][r][8 * d8 + 4]) = make_int4(acc[r][4], acc[r][5], acc[r][6], acc[r][7]);
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < nrow * HD; e += PFX_THREADS) {
+    int32_t t = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) t += s_part[w][e / HD][e % HD];
+    sums[(int64_t(blockIdx.x) * rows + row0 + e / HD) * HD + e % HD] = t;
+  }
+}
+
+// Output: the splits' and the suffix tiles' sums, rounding and rescale; the
+// rows' maxima and sums are set back to zero. A block per PFX_ROWS rows of a unit
+// and PTC_JOIN_DIMS dimensions, a thread one output (8 rows x 8 bytes of a
+// dimension lie together), so that all its loads are in flight at once.
+__global__ void __launch_bounds__(PFX_THREADS)
+    prefix_join_kernel(PrefixParams p, PrefixTc tc, int units, int splits, const int32_t* __restrict__ sums) {
+  pdl_wait();
+  pdl_launch();
+  const int unit = int(blockIdx.y), g = unit / tc.RT, hd = p.hd;
+  const int rt = int(blockIdx.x) * PFX_ROWS + int(threadIdx.x) % PFX_ROWS, rho = (unit % tc.RT) * PTC_ROWS + rt;
+  const int d = int(blockIdx.z) * PTC_JOIN_DIMS + int(threadIdx.x) / PFX_ROWS;
+  if (rho >= p.R) return;
+  const int64_t row = int64_t(g) * p.R + rho, rows = int64_t(p.nkv) * p.R, step = int64_t(units) * hd * PTC_ROWS;
+  const int tiles = p.S > 0 ? (pfx_clamped(p, rho / (p.T * p.G)) + PTC_SFX_KEYS - 1) / PTC_SFX_KEYS : 0;
+  const int64_t* src = tc.part + (int64_t(unit) * hd + d) * PTC_ROWS + rt;
+  int64_t tot = 0;
+#pragma unroll 16
+  for (int s = 0; s < splits; ++s) tot += __ldcs(src + s * step);
+  const int32_t* sfx = sums + row * hd + d;
+#pragma unroll 4
+  for (int t = 0; t < tiles; ++t) tot += sfx[t * rows * hd];
+  int32_t o = clamp16(p.prob_frac > 0 ? rshift_rne_i64(tot, p.prob_frac) : tot);
+  if (p.out_shift != 0) o = clamp16(rescale_i32_s(o, p.out_shift));
+  p.out[int64_t(rho / p.G) * p.ldo + int64_t(g * p.G + rho % p.G) * hd + d] = int16_t(o);
+  if (blockIdx.z == 0 && int(threadIdx.x) < PFX_ROWS) {  // read by earlier kernels alone
+    p.rowmax[row] = 0;
+    p.rowsum[row] = 0;
   }
 }
 

@@ -15,7 +15,8 @@ struct myl_attn_plan {
   int64_t score_mult = 0;
   int score_shift = 0, lut_shift = 0, prob_frac = 0, out_shift = 0;
   int cap = 0, lut_n = 0;  // see PrefixTc
-  bool tc = false;         // the constants fit the tensor-core kernels
+  double scale = 0, offset = 0;
+  bool tc = false;  // the constants fit the tensor-core kernels
   std::vector<void*> allocs;
 };
 
@@ -98,8 +99,11 @@ int attn_plan_build(myl_attn_plan* pl, int64_t score_mult, uint8_t score_shift, 
   const int64_t top = INT32_MAX >> lut_shift;
   pl->cap = int(std::min(n, top));
   pl->lut_n = pl->cap + 1;
-  // score = low word of a 64-bit value shifted by less than 32, 256 mult in 31 bits
-  pl->tc = score_shift >= 1 && score_shift <= 31 && score_mult >= 0 && score_mult < (1 << 23) && pl->lut_n <= PTC_LUT_MAX;
+  // the tensor-core path's score is one double multiply-add, see prefix_tc.cuh
+  pl->tc = score_shift <= 51 && score_mult >= 0 && score_mult < (1 << 25) && score_mult <= int64_t(1) << score_shift &&
+           pl->lut_n <= PTC_LUT_MAX;
+  pl->scale = std::ldexp(double(score_mult), -int(score_shift));
+  pl->offset = std::ldexp(1.5, 52) - std::ldexp(1.5 * double(score_mult), 52 - int(score_shift));
   return dev_upload(pl->allocs, &pl->d_lut, exp_lut, size_t(exp_len));
 }
 
@@ -142,6 +146,14 @@ int prefix_build(myl_ctx* ctx, myl_prefix* pf, const int16_t* k, const int16_t* 
   return MYL_OK;
 }
 
+// A workspace of words that every call leaves at zero.
+int zero_kept(DevBuf& b, size_t bytes, cudaStream_t st) {
+  const size_t had = b.cap;
+  TRY(ensure(b, bytes));
+  if (b.cap != had) CUDA_TRY(cudaMemsetAsync(b.p, 0, b.cap, st));
+  return MYL_OK;
+}
+
 // Key steps per block so that `units` rows of blocks finish soonest on the
 // SMs, with a fixed cost per block of about `fixed` steps.
 int prefix_split(int units, int steps, int sms, int fixed) {
@@ -163,23 +175,27 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix* pf, P
   qk.RT = pv.RT = RT;
   qk.cap = pl->cap;
   qk.lut_n = pl->lut_n;
+  qk.scale = pl->scale;
+  qk.offset = pl->offset;
+  qk.k256 = 256;
+  qk.k1 = 1;
   qk.timeout_ns = pv.timeout_ns = ctx->timeout_ns;
   qk.steps = p.Pp / PTC_KEYS;
   pv.steps = p.Pp / PTC_VKEYS;
-  qk.per = prefix_split(units, qk.steps, n, 4);
+  qk.per = prefix_split(units, qk.steps, n, 8);
   pv.per = prefix_split(units, pv.steps, n, 3);
   const int sq = (qk.steps + qk.per - 1) / qk.per, sv = (pv.steps + pv.per - 1) / pv.per;
-  p.soff = 0;
   p.lds = (p.S + 31) & ~31;
+  const int tiles = (p.S + PTC_SFX_KEYS - 1) / PTC_SFX_KEYS;
   MoeArena a;
-  const size_t o_acc = a.take<uint64_t>(rows * HD), o_max = a.take<uint32_t>(rows), o_sum = a.take<int32_t>(rows),
-               o_sc = a.take<int32_t>(rows * p.lds), o_e = a.take<uint16_t>(int64_t(units) * p.Pp * PTC_ROWS),
-               o_part = a.take<int64_t>(int64_t(sv) * units * HD * PTC_ROWS);
+  const size_t o_sc = a.take<int32_t>(rows * p.lds), o_e = a.take<uint16_t>(int64_t(units) * p.Pp * PTC_ROWS),
+               o_part = a.take<int64_t>(int64_t(sv) * units * HD * PTC_ROWS),
+               o_sfx = a.take<int32_t>(int64_t(tiles) * rows * HD);
   TRY(ensure(ctx->pfx, a.off));
   uint8_t* ws = static_cast<uint8_t*>(ctx->pfx.p);
-  p.acc = reinterpret_cast<unsigned long long*>(ws + o_acc);
-  p.rowmax = reinterpret_cast<unsigned*>(ws + o_max);
-  p.rowsum = reinterpret_cast<int32_t*>(ws + o_sum);
+  TRY(zero_kept(ctx->pfx_stat, size_t(rows) * 8, st));
+  p.rowmax = static_cast<unsigned*>(ctx->pfx_stat.p);
+  p.rowsum = reinterpret_cast<int32_t*>(p.rowmax + rows);
   p.scores = reinterpret_cast<int32_t*>(ws + o_sc);
   qk.e = pv.e = reinterpret_cast<uint4*>(ws + o_e);
   pv.part = reinterpret_cast<int64_t*>(ws + o_part);
@@ -187,35 +203,29 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix* pf, P
   const void *f0 = reinterpret_cast<const void*>(&prefix_qk_kernel<HD, 0>),
              *f1 = reinterpret_cast<const void*>(&prefix_qk_kernel<HD, 1>),
              *f2 = reinterpret_cast<const void*>(&prefix_pv_kernel<HD>);
-  TRY(kernel_smem_occupancy(ctx->device, f0, PTC_THREADS, Cfg::QK_SMEM, nullptr));
-  TRY(kernel_smem_occupancy(ctx->device, f1, PTC_THREADS, Cfg::QK_SMEM, nullptr));
-  TRY(kernel_smem_occupancy(ctx->device, f2, PTC_THREADS, Cfg::PV_SMEM, nullptr));
-  const unsigned gy = unsigned(p.nkv * ((p.T * p.G + PFX_ROWS - 1) / PFX_ROWS));
-  const int t1 = (p.S + PFX_SKEYS - 1) / PFX_SKEYS, t3 = (p.S + PFX_VKEYS - 1) / PFX_VKEYS;
-  const unsigned flat = unsigned(std::min<int64_t>((rows * p.hd + 255) / 256, int64_t(ctx->num_sms) * 8));
-  LaunchCfg l0(ctx, dim3(flat), dim3(256), 0, st);
-  CUDA_TRY(cudaLaunchKernelEx(&l0.cfg, prefix_init_kernel, p, rows));
+  TRY(kernel_smem_occupancy(ctx->device, f0, PTC_QK_THREADS, Cfg::QK_SMEM, nullptr));
+  TRY(kernel_smem_occupancy(ctx->device, f1, PTC_QK_THREADS, Cfg::QK_SMEM, nullptr));
+  TRY(kernel_smem_occupancy(ctx->device, f2, PTC_PV_THREADS, Cfg::PV_SMEM, nullptr));
+  int32_t* sums = reinterpret_cast<int32_t*>(ws + o_sfx);
+  const dim3 suffix(unsigned(tiles), unsigned(p.nkv * ((p.T * p.G + PFX_ROWS - 1) / PFX_ROWS)), unsigned(p.B));
   if (p.S > 0) {
-    LaunchCfg l(ctx, dim3(unsigned(p.B * t1), gy), dim3(PFX_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_scores_kernel, p, 0, t1));
+    LaunchCfg l0(ctx, suffix, dim3(PFX_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l0.cfg, prefix_suffix_kernel, p));
+    qk.early = 1;
   }
-  LaunchCfg l1(ctx, dim3(unsigned(sq), unsigned(units)), dim3(PTC_THREADS), Cfg::QK_SMEM, st);
+  LaunchCfg l1(ctx, dim3(unsigned(sq), unsigned(units)), dim3(PTC_QK_THREADS), Cfg::QK_SMEM, st);
   CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 0>, pf->tm_kh, pf->tm_kl, p, qk));
-  if (p.S > 0) {
-    LaunchCfg l(ctx, dim3(unsigned(rows)), dim3(PFX_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_sum_kernel, p, 0));
-  }
+  qk.early = 1;
   CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 1>, pf->tm_kh, pf->tm_kl, p, qk));
   if (p.S > 0) {
-    LaunchCfg l(ctx, dim3(unsigned(p.B * t3), gy), dim3(PFX_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_values_kernel, p, 0, t3));
+    LaunchCfg l(ctx, suffix, dim3(PFX_THREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_suffix_values_kernel<HD>, p, sums, rows));
   }
-  LaunchCfg l2(ctx, dim3(unsigned(sv), unsigned(units)), dim3(PTC_THREADS), Cfg::PV_SMEM, st);
+  LaunchCfg l2(ctx, dim3(unsigned(sv), unsigned(units)), dim3(PTC_PV_THREADS), Cfg::PV_SMEM, st);
   CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_pv_kernel<HD>, pf->tm_vh, pf->tm_vl, p, pv));
-  LaunchCfg l3(ctx, dim3(unsigned(std::min<int64_t>(int64_t(units) * HD * PTC_ROWS / 256, int64_t(ctx->num_sms) * 16))),
-               dim3(256), 0, st);
-  CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_join_kernel, p, pv, units, sv));
-  ctx->launches += p.S > 0 ? 8 : 5;
+  LaunchCfg l3(ctx, dim3(PTC_ROWS / PFX_ROWS, unsigned(units), HD / PTC_JOIN_DIMS), dim3(PFX_THREADS), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_join_kernel, p, pv, units, sv, static_cast<const int32_t*>(sums)));
+  ctx->launches += p.S > 0 ? 6 : 4;
   return MYL_OK;
 }
 
@@ -229,7 +239,6 @@ int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix
   if (gy > 65535u) return fail(MYL_ERR_UNSUPPORTED, "%d query rows per KV head", p.R);
   if (pl->tc && p.P > 0 && p.R >= PTC_MIN_ROWS && (p.hd == 64 || p.hd == 128))
     return p.hd == 128 ? run_prefix_tc<128>(ctx, pl, pf, p, st) : run_prefix_tc<64>(ctx, pl, pf, p, st);
-  p.soff = p.Pp;
   p.lds = p.Pp + ((p.S + 31) & ~31);
   const size_t o_max = size_t(rows) * size_t(p.hd) * 8, o_sum = o_max + size_t(rows) * 4,
                o_sc = (o_sum + size_t(rows) * 4 + 255) & ~size_t(255);
@@ -250,7 +259,7 @@ int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix
     LaunchCfg l1(ctx, dim3(unsigned(nb1 + p.B * t1), gy), dim3(PFX_THREADS), 0, st);
     CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_scores_kernel, p, nb1, t1));
     LaunchCfg l2(ctx, dim3(unsigned(rows)), dim3(PFX_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_sum_kernel, p, p.P));
+    CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_sum_kernel, p));
     const int nb3 = (p.P + PFX_VKEYS - 1) / PFX_VKEYS, t3 = (p.S + PFX_VKEYS - 1) / PFX_VKEYS;
     LaunchCfg l3(ctx, dim3(unsigned(nb3 + p.B * t3), gy), dim3(PFX_THREADS), 0, st);
     CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_values_kernel, p, nb3, t3));
@@ -314,9 +323,7 @@ int run_verify(myl_ctx* ctx, VerifyParams& p, cudaStream_t st) {
   p.per = int(((p.V + cl - 1) / cl + 3) & ~3);
   const int64_t smem = p.per * logit_bytes;
   if (smem <= VERIFY_SMEM && units * cl <= INT32_MAX) {
-    const size_t had = ctx->vfy_done.cap;
-    TRY(ensure(ctx->vfy_done, size_t(p.B) * 4));
-    if (ctx->vfy_done.cap != had) CUDA_TRY(cudaMemsetAsync(ctx->vfy_done.p, 0, ctx->vfy_done.cap, st));
+    TRY(zero_kept(ctx->vfy_done, size_t(p.B) * 4, st));
     TRY(ensure(ctx->vfy, size_t(units) * 4));
     p.done = static_cast<unsigned*>(ctx->vfy_done.p);
     p.pos = static_cast<int32_t*>(ctx->vfy.p);
