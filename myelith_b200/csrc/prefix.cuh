@@ -15,9 +15,12 @@
 // sums and weighted values are three passes over the scores.
 //
 // The prefix is laid out once, when it is registered, as unsigned byte planes
-// (x + 32768 = 256 hi + lo): keys [kv head][position][hd] and
-// values transposed [kv head][hd][position], positions padded with zeros to a
-// multiple of PFX_PAD. Rows of a KV head g are numbered
+// (x + 32768 = 256 hi + lo) in the order in which the tensor cores read them from
+// shared memory, so that one bulk copy brings a block of positions: keys as
+// [kv head][32 positions][hi 32 rows, lo 32 rows][hd], values transposed as
+// [kv head][128 positions][hi hd rows, lo hd rows][128], the 16-byte pieces of a
+// row swapped by the 128-byte (64-byte for key rows of 64) swizzle; positions
+// padded with zeros to a multiple of PFX_PAD. Rows of a KV head g are numbered
 // rho = (b * T + t) * G + (h - g * G), R = B * T * G of them; score rows are
 // g * R + rho, prefix scores in columns [0, P), suffix scores from column Pp.
 // The kernels here run any head size and few rows; prefix_tc.cuh has the ones
@@ -40,8 +43,7 @@ struct PrefixParams {
   const int16_t* q;
   int64_t ldq;  // elements between token rows
   int B, T, nq, nkv, G, hd, R;
-  const uint8_t *kh, *kl;    // [nkv][Pp][hd]
-  const uint8_t *vth, *vtl;  // [nkv][hd][Pp]
+  const uint8_t *k, *v;  // the prefix's planes
   int P, Pp;
   const int16_t *ks, *vs;  // suffix caches
   int64_t seq_stride, head_stride, pos_stride;
@@ -87,13 +89,29 @@ __device__ __forceinline__ int32_t pfx_exp(const PrefixParams& p, int32_t m, int
 }
 
 // ---- the prefix's planes ------------------------------------------------------------
+// Byte offset of a 16-byte piece `c16` of byte row `row` (hd bytes long) of a key block.
+__host__ __device__ __forceinline__ int pfx_piece(int hd, int row, int c16) {
+  return row * hd + ((hd == 128 ? c16 ^ (row & 7) : hd == 64 ? c16 ^ ((row >> 1) & 3) : c16) << 4);
+}
+// Offset of bytes d.. (inside one piece) of plane `lo` of position j of head g.
+__device__ __forceinline__ int64_t pfx_key_at(int64_t Pp, int hd, int64_t g, int64_t j, int lo, int d) {
+  const int row = 32 * lo + int(j & 31);
+  const int at = hd % 16 ? row * hd + d : pfx_piece(hd, row, d >> 4) + (d & 15);
+  return (g * (Pp / 32) + (j >> 5)) * 64 * hd + at;
+}
+// Offset of positions j.. (inside one piece) of plane `lo` of dimension d of head g.
+__device__ __forceinline__ int64_t pfx_value_at(int64_t Pp, int hd, int64_t g, int64_t j, int lo, int d) {
+  const int row = lo * hd + d;
+  return ((g * (Pp / 128) + (j >> 7)) * 2 * hd + row) * 128 + ((((int(j) >> 4) ^ row) & 7) << 4) + (int(j) & 15);
+}
+
 // grid: (Pp / 32, ceil(hd / 32), nkv); a 32 x 32 tile goes through shared
 // memory so that both the key rows and the transposed value rows are written
 // in their own order.
 __global__ void __launch_bounds__(256)
     prefix_planes_kernel(const int16_t* __restrict__ k, const int16_t* __restrict__ v, int64_t P, int64_t Pp,
-                         int hd, int64_t pos_stride, int64_t head_stride, uint8_t* __restrict__ kh,
-                         uint8_t* __restrict__ kl, uint8_t* __restrict__ vth, uint8_t* __restrict__ vtl) {
+                         int hd, int64_t pos_stride, int64_t head_stride, uint8_t* __restrict__ kp,
+                         uint8_t* __restrict__ vp) {
   pdl_wait();
   pdl_launch();
   __shared__ int16_t tile[32][33];
@@ -110,9 +128,8 @@ __global__ void __launch_bounds__(256)
       vv = v[g * head_stride + j * pos_stride + d];
     }
     if (d < hd) {
-      const int64_t o = (g * Pp + j) * hd + d;
-      kh[o] = uint8_t((uint16_t(kv) >> 8) ^ 0x80);
-      kl[o] = uint8_t(kv & 255);
+      kp[pfx_key_at(Pp, hd, g, j, 0, d)] = uint8_t((uint16_t(kv) >> 8) ^ 0x80);
+      kp[pfx_key_at(Pp, hd, g, j, 1, d)] = uint8_t(kv & 255);
     }
     tile[r][x] = vv;
   }
@@ -121,9 +138,8 @@ __global__ void __launch_bounds__(256)
     const int d = d0 + r;
     if (d >= hd) continue;
     const int16_t vv = tile[x][r];
-    const int64_t o = (g * hd + d) * Pp + j0 + x;
-    vth[o] = uint8_t((uint16_t(vv) >> 8) ^ 0x80);
-    vtl[o] = uint8_t(vv & 255);
+    vp[pfx_value_at(Pp, hd, g, j0 + x, 0, d)] = uint8_t((uint16_t(vv) >> 8) ^ 0x80);
+    vp[pfx_value_at(Pp, hd, g, j0 + x, 1, d)] = uint8_t(vv & 255);
   }
 }
 
@@ -165,10 +181,9 @@ __device__ __forceinline__ void prefix_scores_block(const PrefixParams& p, int g
         kh[i] = make_uint2(__byte_perm(w.x, w.y, 0x7531), __byte_perm(w.z, w.w, 0x7531));
         kl[i] = make_uint2(__byte_perm(w.x, w.y, 0x6420), __byte_perm(w.z, w.w, 0x6420));
       } else {
-        const int64_t o = (int64_t(g) * p.Pp + j) * hd + 8 * c;
-        kh[i] = *reinterpret_cast<const uint2*>(p.kh + o);
+        kh[i] = *reinterpret_cast<const uint2*>(p.k + pfx_key_at(p.Pp, hd, g, j, 0, 8 * c));
         kh[i].x ^= 0x80808080u, kh[i].y ^= 0x80808080u;  // signed high bytes
-        kl[i] = *reinterpret_cast<const uint2*>(p.kl + o);
+        kl[i] = *reinterpret_cast<const uint2*>(p.k + pfx_key_at(p.Pp, hd, g, j, 1, 8 * c));
       }
     }
   }
@@ -341,8 +356,8 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_values_kernel(PrefixParams
         }
       }
     } else {
-      const int64_t o = (int64_t(g) * hd + d) * p.Pp + j0 + 16 * kg;
-      const uint4 a = *reinterpret_cast<const uint4*>(p.vth + o), c = *reinterpret_cast<const uint4*>(p.vtl + o);
+      const uint4 a = *reinterpret_cast<const uint4*>(p.v + pfx_value_at(p.Pp, hd, g, j0 + 16 * kg, 0, d));
+      const uint4 c = *reinterpret_cast<const uint4*>(p.v + pfx_value_at(p.Pp, hd, g, j0 + 16 * kg, 1, d));
       wh[0] = a.x ^ 0x80808080u, wh[1] = a.y ^ 0x80808080u, wh[2] = a.z ^ 0x80808080u, wh[3] = a.w ^ 0x80808080u;
       wl[0] = c.x, wl[1] = c.y, wl[2] = c.z, wl[3] = c.w;
     }

@@ -38,8 +38,8 @@ namespace myl {
 
 constexpr int PTC_ROWS = 128;
 constexpr int PTC_KEYS = 32;        // keys per scores step
+constexpr int PTC_BLOCK = 128;      // keys per bulk copy
 constexpr int PTC_BUFS = 3;         // TMEM score buffers
-constexpr int PTC_VKEYS = 128;      // keys per values step
 constexpr int PTC_QK_WARPS = 4 * PTC_BUFS;  // worker warps: buffer x TMEM lane quarter
 constexpr int PTC_PV_WARPS = 16;    // TMEM lane quarter x column quarter
 constexpr int PTC_QK_THREADS = 64 + 32 * PTC_QK_WARPS;
@@ -50,8 +50,8 @@ constexpr int PTC_LUT_MAX = 16384;  // exponential table entries in shared memor
 
 struct PrefixTc {
   int RT;      // row tiles per KV head
-  int steps;   // steps of the kernel's keys over all of Pp
-  int per;     // steps per block
+  int blocks;  // 128-key blocks of the prefix
+  int per;     // of these per thread block
   double scale, offset;  // of a score, see above
   int k256, k1;          // 256 and 1, kept from being folded: one multiply-add beats shifts and carries
   int early;   // the scores kernel does not have to wait before its set-up
@@ -63,7 +63,7 @@ struct PrefixTc {
 };
 
 struct PrefixCtl {
-  uint64_t full[12], empty[12];
+  uint64_t full[4], empty[4];
   uint64_t tfull[PTC_BUFS], tempty[PTC_BUFS];
   uint32_t tmem_base;
   int abort;
@@ -72,10 +72,10 @@ struct PrefixCtl {
 
 template <int HD>
 struct PtcCfg {
-  static constexpr int K_STAGE = 2 * PTC_KEYS * HD;               // kh and kl of a step
-  static constexpr int K_STAGES = 12;
-  static constexpr int P_BYTES = PTC_ROWS * PTC_VKEYS;            // one probability plane
-  static constexpr int V_STAGE = 2 * HD * PTC_VKEYS;              // vh and vl of a step
+  static constexpr int K_STAGE = 2 * PTC_BLOCK * HD;              // kh and kl of 128 keys
+  static constexpr int K_STAGES = 4;
+  static constexpr int P_BYTES = PTC_ROWS * PTC_BLOCK;            // one probability plane
+  static constexpr int V_STAGE = 2 * HD * PTC_BLOCK;              // vh and vl of 128 keys
   static constexpr int V_STAGES = 3;
   static constexpr int QK_SMEM = K_STAGES * K_STAGE + 2 * (PTC_LUT_MAX + 8) + 1024;
   static constexpr int PV_SMEM = 4 * P_BYTES + V_STAGES * V_STAGE + 1024;
@@ -106,6 +106,20 @@ __device__ __forceinline__ int64_t mad_wide(int32_t a, int32_t b, int64_t c) {
   int64_t d;
   asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(d) : "r"(a), "r"(b), "l"(c));
   return d;
+}
+
+// Untiled bulk copy global -> shared (16-byte aligned, a multiple of 16 bytes).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -145,15 +159,16 @@ __device__ __forceinline__ void ptc_drain(PrefixCtl& ctl, int issued, int stages
 // reads only its 64 key byte rows from shared memory (operand bytes from shared
 // memory, about 70 a clock here, set the pace of small MMAs: with the queries
 // there too, steps of 64 keys took 930 clocks instead of the 512 of the pipe).
-// Warp 0 loads key planes with TMA, warp 1 issues the MMAs into three score
+// Warp 0 copies key planes in blocks of 128 positions (tiled copies of 32 or 64
+// rows cost about 400 clocks each whatever their size, one bulk copy of a block
+// no more than that), warp 1 issues the MMAs into three score
 // buffers [hh | hl | lh | ll] of 32 columns each, and each buffer has four warps
 // that turn its scores into their output, so that three steps are worked on at
 // a time: warp (buffer, q) has rows 32 q.. of every third step, a thread one
 // row. In MODE 1 the blocks of a unit also share out its rows' suffix sums.
 template <int HD, int MODE>
 __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
-    prefix_qk_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant__ CUtensorMap tm_kl,
-                     PrefixParams p, PrefixTc tc) {
+    prefix_qk_kernel(PrefixParams p, PrefixTc tc) {
   // early: the kernel before this one belongs to the same call, so everything
   // but the row statistics and the exponentials is in place already
   if (!tc.early) pdl_wait();
@@ -168,7 +183,8 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
   uint16_t* const s_lut = reinterpret_cast<uint16_t*>(base + ST * Cfg::K_STAGE);
   volatile int* abort = &ctl.abort;
   const int unit = int(blockIdx.y), g = unit / tc.RT, row0 = (unit % tc.RT) * PTC_ROWS;
-  const int i0 = int(blockIdx.x) * tc.per, n = min(tc.per, tc.steps - i0);
+  const int i0 = int(blockIdx.x) * tc.per, n = min(tc.per, tc.blocks - i0);  // 128-key blocks
+  constexpr int SUB = PTC_BLOCK / PTC_KEYS;                                  // steps each
 
   ptc_setup(ctl, ST, 1, 4);
   tc_fence_before();
@@ -213,42 +229,44 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
           tc_fail(p.err, abort, DEV_WAIT_PRODUCER);
           break;
         }
-        const uint32_t fb = smem_addr(&ctl.full[s]), dst = ring + uint32_t(s * Cfg::K_STAGE);
-        const int32_t row = g * p.Pp + (i0 + i) * PTC_KEYS;
+        const uint32_t fb = smem_addr(&ctl.full[s]);
         mbar_arrive_expect_tx(fb, uint32_t(Cfg::K_STAGE));
-        tma_load_2d(dst, &tm_kh, fb, 0, row);
-        tma_load_2d(dst + Cfg::K_STAGE / 2, &tm_kl, fb, 0, row);
+        bulk_load(ring + uint32_t(s * Cfg::K_STAGE), p.k + (int64_t(g) * tc.blocks + i0 + i) * Cfg::K_STAGE, Cfg::K_STAGE, fb);
       }
       ptc_drain(ctl, i, ST, tc.timeout_ns, p.err);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t id_h = idesc_i8(128, 2 * PTC_KEYS, true, false), id_l = idesc_i8(128, 2 * PTC_KEYS, false, false);
-      int i = 0, b = 0;
-      uint32_t use = 0;  // parity of the buffers' use
-      for (; i < n; ++i) {
-        const int s = i % ST;
-        if (!mbar_wait_bounded(smem_addr(&ctl.tempty[b]), use ^ 1u, tc.timeout_ns, abort) ||
-            !mbar_wait_bounded(smem_addr(&ctl.full[s]), uint32_t(i / ST) & 1u, tc.timeout_ns, abort)) {
-          tc_fail(p.err, abort, DEV_WAIT_MMA);
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem + uint32_t(b * 128), kb = ring + uint32_t(s * Cfg::K_STAGE);
+    // The whole warp walks the steps and one elected lane issues: operands that
+    // the compiler can see are warp-uniform need no move into uniform registers
+    // before every MMA.
+    constexpr uint32_t id_h = idesc_i8(128, 2 * PTC_KEYS, true, false), id_l = idesc_i8(128, 2 * PTC_KEYS, false, false);
+    int i = 0, b = 0;  // step, its buffer
+    uint32_t use = 0;  // parity of the buffers' use
+    for (; i < n * SUB; ++i) {
+      const int blk = i / SUB, s = blk % ST;
+      if (!mbar_wait_bounded(smem_addr(&ctl.tempty[b]), use ^ 1u, tc.timeout_ns, abort) ||
+          (i % SUB == 0 && !mbar_wait_bounded(smem_addr(&ctl.full[s]), uint32_t(blk / ST) & 1u, tc.timeout_ns, abort))) {
+        tc_fail(p.err, abort, DEV_WAIT_MMA);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + uint32_t(b * 128);
+      const uint64_t db = ptc_desc<HD>(ring + uint32_t(s * Cfg::K_STAGE + i % SUB * (Cfg::K_STAGE / SUB)));
+      if (elect_lane()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 32; ++kk) {
-          const uint64_t db = ptc_desc<HD>(kb + 32 * kk);
-          mma_i8_ts(d, a_hi + 8 * kk, db, id_h, kk > 0);
-          mma_i8_ts(d + 64, a_lo + 8 * kk, db, id_l, kk > 0);
+          mma_i8_ts(d, a_hi + 8 * kk, db + 2 * kk, id_h, kk > 0);
+          mma_i8_ts(d + 64, a_lo + 8 * kk, db + 2 * kk, id_l, kk > 0);
         }
-        mma_commit(smem_addr(&ctl.empty[s]));
+        if (i % SUB == SUB - 1) mma_commit(smem_addr(&ctl.empty[s]));
         mma_commit(smem_addr(&ctl.tfull[b]));
-        if (++b == PTC_BUFS) b = 0, use ^= 1u;
       }
-      // the issued MMAs finish before TMEM is released
-      if (i > 0 && !mbar_wait_bounded(smem_addr(&ctl.tfull[(i - 1) % PTC_BUFS]), uint32_t((i - 1) / PTC_BUFS) & 1u, tc.timeout_ns, nullptr))
-        atomicCAS(p.err, 0, DEV_WAIT_DRAIN);
+      __syncwarp();
+      if (++b == PTC_BUFS) b = 0, use ^= 1u;
     }
+    // the issued MMAs finish before TMEM is released
+    if (i > 0 && !mbar_wait_bounded(smem_addr(&ctl.tfull[(i - 1) % PTC_BUFS]), uint32_t((i - 1) / PTC_BUFS) & 1u, tc.timeout_ns, nullptr))
+      atomicCAS(p.err, 0, DEV_WAIT_DRAIN);
   } else {
     const int q = warp & 3, b = (warp - 2) >> 2;
     const int r = 32 * q + lane, rho = row0 + r;
@@ -260,14 +278,14 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
     int32_t mx = INT32_MIN, sum = 0;
     if (MODE == 1 && live) mx = int32_t(p.rowmax[row] ^ 0x80000000u);
     uint32_t use = 0;
-    for (int i = b; i < n; i += PTC_BUFS, use ^= 1u) {
+    for (int i = b; i < n * SUB; i += PTC_BUFS, use ^= 1u) {
       if (!mbar_wait_bounded(smem_addr(&ctl.tfull[b]), use, tc.timeout_ns, abort)) {
         tc_fail(p.err, abort, DEV_WAIT_EPILOGUE);
         break;
       }
       if (*abort) break;
       tc_fence_after();
-      const int kb = i0 + i;
+      const int kb = i0 * SUB + i;
       const uint32_t t0 = tmem + (uint32_t(32 * q) << 16) + uint32_t(b * 128);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -315,7 +333,7 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
             sum += int32_t(ex[2 * j] + ex[2 * j + 1]);
             w[j] = ex[2 * j] | (ex[2 * j + 1] << 16);
           }
-          uint4* dst = tc.e + (((int64_t(unit) * tc.steps + kb) * 2 + h) * PTC_ROWS + r) * 2;
+          uint4* dst = tc.e + (((int64_t(unit) * tc.blocks * SUB + kb) * 2 + h) * PTC_ROWS + r) * 2;
           dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
           dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
@@ -355,8 +373,7 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
 // byte planes of p go to shared memory as the MMA's A operand.
 template <int HD>
 __global__ void __launch_bounds__(PTC_PV_THREADS, 1)
-    prefix_pv_kernel(const __grid_constant__ CUtensorMap tm_vh, const __grid_constant__ CUtensorMap tm_vl,
-                     PrefixParams p, PrefixTc tc) {
+    prefix_pv_kernel(PrefixParams p, PrefixTc tc) {
   pdl_launch();  // never a call's first kernel: only the workers have to wait
   using Cfg = PtcCfg<HD>;
   constexpr int ST = Cfg::V_STAGES;
@@ -367,7 +384,7 @@ __global__ void __launch_bounds__(PTC_PV_THREADS, 1)
   const uint32_t ring = smem_addr(base) + 4 * Cfg::P_BYTES;
   volatile int* abort = &ctl.abort;
   const int unit = int(blockIdx.y), g = unit / tc.RT, row0 = (unit % tc.RT) * PTC_ROWS;
-  const int i0 = int(blockIdx.x) * tc.per, n = min(tc.per, tc.steps - i0);
+  const int i0 = int(blockIdx.x) * tc.per, n = min(tc.per, tc.blocks - i0);
 
   // tfull / tempty: probability buffers written (16 warps) / consumed (a commit)
   ptc_setup(ctl, ST, PTC_PV_WARPS, 1);
@@ -385,40 +402,39 @@ __global__ void __launch_bounds__(PTC_PV_THREADS, 1)
           tc_fail(p.err, abort, DEV_WAIT_PRODUCER);
           break;
         }
-        const uint32_t fb = smem_addr(&ctl.full[s]), dst = ring + uint32_t(s * Cfg::V_STAGE);
-        const int32_t key = (i0 + i) * PTC_VKEYS;
+        const uint32_t fb = smem_addr(&ctl.full[s]);
         mbar_arrive_expect_tx(fb, uint32_t(Cfg::V_STAGE));
-        tma_load_2d(dst, &tm_vh, fb, key, g * HD);
-        tma_load_2d(dst + Cfg::V_STAGE / 2, &tm_vl, fb, key, g * HD);
+        bulk_load(ring + uint32_t(s * Cfg::V_STAGE), p.v + (int64_t(g) * tc.blocks + i0 + i) * Cfg::V_STAGE, Cfg::V_STAGE, fb);
       }
       ptc_drain(ctl, i, ST, tc.timeout_ns, p.err);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t id = idesc_i8(128, 2 * HD, false, false);
-      int i = 0;
-      for (; i < n; ++i) {
-        const int s = i % ST, b = i & 1;
-        if (!mbar_wait_bounded(smem_addr(&ctl.full[s]), uint32_t(i / ST) & 1u, tc.timeout_ns, abort) ||
-            !mbar_wait_bounded(smem_addr(&ctl.tfull[b]), uint32_t(i >> 1) & 1u, tc.timeout_ns, abort)) {
-          tc_fail(p.err, abort, DEV_WAIT_MMA);
-          break;
-        }
-        tc_fence_after();
-        const uint32_t ph = smem_addr(base) + uint32_t(2 * b * Cfg::P_BYTES), vb = ring + uint32_t(s * Cfg::V_STAGE);
+    constexpr uint32_t id = idesc_i8(128, 2 * HD, false, false);
+    int i = 0;
+    for (; i < n; ++i) {
+      const int s = i % ST, b = i & 1;
+      if (!mbar_wait_bounded(smem_addr(&ctl.full[s]), uint32_t(i / ST) & 1u, tc.timeout_ns, abort) ||
+          !mbar_wait_bounded(smem_addr(&ctl.tfull[b]), uint32_t(i >> 1) & 1u, tc.timeout_ns, abort)) {
+        tc_fail(p.err, abort, DEV_WAIT_MMA);
+        break;
+      }
+      tc_fence_after();
+      const uint64_t dp = smem_desc_k_sw128(smem_addr(base) + uint32_t(2 * b * Cfg::P_BYTES));
+      const uint64_t dv = smem_desc_k_sw128(ring + uint32_t(s * Cfg::V_STAGE));
+      if (elect_lane()) {
 #pragma unroll
-        for (int kk = 0; kk < PTC_VKEYS / 32; ++kk) {
-          const uint64_t db = smem_desc_k_sw128(vb + 32 * kk);
+        for (int kk = 0; kk < PTC_BLOCK / 32; ++kk) {
           const uint32_t acc = i > 0 || kk > 0;
-          mma_i8(tmem, smem_desc_k_sw128(ph + 32 * kk), db, id, acc);
-          mma_i8(tmem + 2 * HD, smem_desc_k_sw128(ph + Cfg::P_BYTES + 32 * kk), db, id, acc);
+          mma_i8(tmem, dp + 2 * kk, dv + 2 * kk, id, acc);
+          mma_i8(tmem + 2 * HD, dp + (Cfg::P_BYTES >> 4) + 2 * kk, dv + 2 * kk, id, acc);
         }
         mma_commit(smem_addr(&ctl.empty[s]));
         mma_commit(smem_addr(&ctl.tempty[b]));
       }
-      if (i > 0 && !mbar_wait_bounded(smem_addr(&ctl.tempty[(i - 1) & 1]), uint32_t((i - 1) >> 1) & 1u, tc.timeout_ns, nullptr))
-        atomicCAS(p.err, 0, DEV_WAIT_DRAIN);
+      __syncwarp();
     }
+    if (i > 0 && !mbar_wait_bounded(smem_addr(&ctl.tempty[(i - 1) & 1]), uint32_t((i - 1) >> 1) & 1u, tc.timeout_ns, nullptr))
+      atomicCAS(p.err, 0, DEV_WAIT_DRAIN);
   } else {
     const int q = warp & 3, c = (warp - 2) >> 2;
     const int r = 32 * q + lane, rho = row0 + r;
@@ -435,7 +451,7 @@ __global__ void __launch_bounds__(PTC_PV_THREADS, 1)
     int psum = 0;
     bool ok = true;
     auto load = [&](int i, uint4 (&x)[4]) {
-      const uint4* src = tc.e + ((int64_t(unit) * tc.steps + i0 + i) * 8 + 2 * c) * PTC_ROWS * 2 + 2 * r;
+      const uint4* src = tc.e + ((int64_t(unit) * tc.blocks + i0 + i) * 8 + 2 * c) * PTC_ROWS * 2 + 2 * r;
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         x[u] = live ? __ldcs(src + (u >> 1) * PTC_ROWS * 2 + (u & 1)) : make_uint4(0u, 0u, 0u, 0u);

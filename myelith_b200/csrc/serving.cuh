@@ -22,8 +22,7 @@ struct myl_attn_plan {
 
 struct myl_prefix {
   int64_t P = 0, Pp = 0, nkv = 0, hd = 0;
-  uint8_t *kh = nullptr, *kl = nullptr, *vth = nullptr, *vtl = nullptr;
-  CUtensorMap tm_kh{}, tm_kl{}, tm_vh{}, tm_vl{};  // head_dim 64 and 128
+  uint8_t *k = nullptr, *v = nullptr;
   std::vector<void*> allocs;
 };
 
@@ -107,40 +106,16 @@ int attn_plan_build(myl_attn_plan* pl, int64_t score_mult, uint8_t score_shift, 
   return dev_upload(pl->allocs, &pl->d_lut, exp_lut, size_t(exp_len));
 }
 
-int encode_bytes(myl_ctx* ctx, CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int box_cols,
-                 int box_rows) {
-  cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
-  cuuint64_t strides[1] = {cuuint64_t(cols)};
-  cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)};
-  cuuint32_t estr[2] = {1, 1};
-  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
-                                 estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                 box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(MYL_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
-  return MYL_OK;
-}
-
 int prefix_build(myl_ctx* ctx, myl_prefix* pf, const int16_t* k, const int16_t* v, int64_t pos_stride,
                  int64_t head_stride, cudaStream_t st) {
-  const size_t n = size_t(pf->nkv) * size_t(pf->Pp) * size_t(pf->hd);
-  TRY(dev_alloc(pf->allocs, &pf->kh, n));
-  TRY(dev_alloc(pf->allocs, &pf->kl, n));
-  TRY(dev_alloc(pf->allocs, &pf->vth, n));
-  TRY(dev_alloc(pf->allocs, &pf->vtl, n));
+  const size_t n = 2 * size_t(pf->nkv) * size_t(pf->Pp) * size_t(pf->hd);
+  TRY(dev_alloc(pf->allocs, &pf->k, n));
+  TRY(dev_alloc(pf->allocs, &pf->v, n));
   if (pf->P > 0) {
     const dim3 grid(unsigned(pf->Pp / 32), unsigned((pf->hd + 31) / 32), unsigned(pf->nkv));
-    prefix_planes_kernel<<<grid, 256, 0, st>>>(k, v, pf->P, pf->Pp, int(pf->hd), pos_stride, head_stride, pf->kh,
-                                               pf->kl, pf->vth, pf->vtl);
+    prefix_planes_kernel<<<grid, 256, 0, st>>>(k, v, pf->P, pf->Pp, int(pf->hd), pos_stride, head_stride, pf->k, pf->v);
     CUDA_TRY(cudaGetLastError());
     ctx->launches++;
-    if (pf->hd == 64 || pf->hd == 128) {
-      const int hd = int(pf->hd);
-      TRY(encode_bytes(ctx, &pf->tm_kh, pf->kh, hd, pf->nkv * pf->Pp, hd, PTC_KEYS));
-      TRY(encode_bytes(ctx, &pf->tm_kl, pf->kl, hd, pf->nkv * pf->Pp, hd, PTC_KEYS));
-      TRY(encode_bytes(ctx, &pf->tm_vh, pf->vth, pf->Pp, pf->nkv * hd, PTC_VKEYS, hd));
-      TRY(encode_bytes(ctx, &pf->tm_vl, pf->vtl, pf->Pp, pf->nkv * hd, PTC_VKEYS, hd));
-    }
   }
   CUDA_TRY(cudaStreamSynchronize(st));
   return MYL_OK;
@@ -154,8 +129,8 @@ int zero_kept(DevBuf& b, size_t bytes, cudaStream_t st) {
   return MYL_OK;
 }
 
-// Key steps per block so that `units` rows of blocks finish soonest on the
-// SMs, with a fixed cost per block of about `fixed` steps.
+// Key blocks per thread block so that `units` rows of thread blocks finish
+// soonest on the SMs, each with a fixed cost of about `fixed` key blocks.
 int prefix_split(int units, int steps, int sms, int fixed) {
   int best = steps;
   int64_t cost = INT64_MAX;
@@ -168,7 +143,7 @@ int prefix_split(int units, int steps, int sms, int fixed) {
 }
 
 template <int HD>
-int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix* pf, PrefixParams& p, cudaStream_t st) {
+int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaStream_t st) {
   const int64_t rows = int64_t(p.nkv) * p.R;
   const int RT = (p.R + PTC_ROWS - 1) / PTC_ROWS, units = p.nkv * RT, n = sms(ctx);
   PrefixTc qk{}, pv{};
@@ -180,16 +155,14 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix* pf, P
   qk.k256 = 256;
   qk.k1 = 1;
   qk.timeout_ns = pv.timeout_ns = ctx->timeout_ns;
-  qk.steps = p.Pp / PTC_KEYS;
-  pv.steps = p.Pp / PTC_VKEYS;
-  qk.per = prefix_split(units, qk.steps, n, 8);
-  pv.per = prefix_split(units, pv.steps, n, 3);
-  const int sq = (qk.steps + qk.per - 1) / qk.per, sv = (pv.steps + pv.per - 1) / pv.per;
+  qk.blocks = pv.blocks = p.Pp / PTC_BLOCK;
+  qk.per = pv.per = prefix_split(units, qk.blocks, n, 3);
+  const int splits = (qk.blocks + qk.per - 1) / qk.per;
   p.lds = (p.S + 31) & ~31;
   const int tiles = (p.S + PTC_SFX_KEYS - 1) / PTC_SFX_KEYS;
   MoeArena a;
   const size_t o_sc = a.take<int32_t>(rows * p.lds), o_e = a.take<uint16_t>(int64_t(units) * p.Pp * PTC_ROWS),
-               o_part = a.take<int64_t>(int64_t(sv) * units * HD * PTC_ROWS),
+               o_part = a.take<int64_t>(int64_t(splits) * units * HD * PTC_ROWS),
                o_sfx = a.take<int32_t>(int64_t(tiles) * rows * HD);
   TRY(ensure(ctx->pfx, a.off));
   uint8_t* ws = static_cast<uint8_t*>(ctx->pfx.p);
@@ -213,32 +186,31 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix* pf, P
     CUDA_TRY(cudaLaunchKernelEx(&l0.cfg, prefix_suffix_kernel, p));
     qk.early = 1;
   }
-  LaunchCfg l1(ctx, dim3(unsigned(sq), unsigned(units)), dim3(PTC_QK_THREADS), Cfg::QK_SMEM, st);
-  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 0>, pf->tm_kh, pf->tm_kl, p, qk));
+  LaunchCfg l1(ctx, dim3(unsigned(splits), unsigned(units)), dim3(PTC_QK_THREADS), Cfg::QK_SMEM, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 0>, p, qk));
   qk.early = 1;
-  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 1>, pf->tm_kh, pf->tm_kl, p, qk));
+  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 1>, p, qk));
   if (p.S > 0) {
     LaunchCfg l(ctx, suffix, dim3(PFX_THREADS), 0, st);
     CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_suffix_values_kernel<HD>, p, sums, rows));
   }
-  LaunchCfg l2(ctx, dim3(unsigned(sv), unsigned(units)), dim3(PTC_PV_THREADS), Cfg::PV_SMEM, st);
-  CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_pv_kernel<HD>, pf->tm_vh, pf->tm_vl, p, pv));
+  LaunchCfg l2(ctx, dim3(unsigned(splits), unsigned(units)), dim3(PTC_PV_THREADS), Cfg::PV_SMEM, st);
+  CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_pv_kernel<HD>, p, pv));
   LaunchCfg l3(ctx, dim3(PTC_ROWS / PFX_ROWS, unsigned(units), HD / PTC_JOIN_DIMS), dim3(PFX_THREADS), 0, st);
-  CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_join_kernel, p, pv, units, sv, static_cast<const int32_t*>(sums)));
+  CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_join_kernel, p, pv, units, splits, static_cast<const int32_t*>(sums)));
   ctx->launches += p.S > 0 ? 6 : 4;
   return MYL_OK;
 }
 
 // The attention of `p` (pointers, shapes and plan filled in) with the
 // context's workspace, which the caller holds.
-int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix* pf, PrefixParams& p,
-                         cudaStream_t st) {
+int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaStream_t st) {
   const int64_t rows = int64_t(p.nkv) * p.R;
   p.err = ctx->d_err;
   const unsigned gy = unsigned(p.nkv * ((p.R + PFX_ROWS - 1) / PFX_ROWS));
   if (gy > 65535u) return fail(MYL_ERR_UNSUPPORTED, "%d query rows per KV head", p.R);
   if (pl->tc && p.P > 0 && p.R >= PTC_MIN_ROWS && (p.hd == 64 || p.hd == 128))
-    return p.hd == 128 ? run_prefix_tc<128>(ctx, pl, pf, p, st) : run_prefix_tc<64>(ctx, pl, pf, p, st);
+    return p.hd == 128 ? run_prefix_tc<128>(ctx, pl, p, st) : run_prefix_tc<64>(ctx, pl, p, st);
   p.lds = p.Pp + ((p.S + 31) & ~31);
   const size_t o_max = size_t(rows) * size_t(p.hd) * 8, o_sum = o_max + size_t(rows) * 4,
                o_sc = (o_sum + size_t(rows) * 4 + 255) & ~size_t(255);
@@ -274,10 +246,8 @@ int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, const myl_prefix
 void prefix_params(PrefixParams& p, const myl_attn_plan* pl, const myl_prefix* pf) {
   p.nkv = int(pf->nkv);
   p.hd = int(pf->hd);
-  p.kh = pf->kh;
-  p.kl = pf->kl;
-  p.vth = pf->vth;
-  p.vtl = pf->vtl;
+  p.k = pf->k;
+  p.v = pf->v;
   p.P = int(pf->P);
   p.Pp = int(pf->Pp);
   p.score_mult = pl->score_mult;
@@ -451,7 +421,7 @@ int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_
   TRY(ws_acquire(ctx, st));
   {
     PdlScope pdl(ctx);
-    TRY(run_prefix_attention(ctx, plan, prefix, p, st));
+    TRY(run_prefix_attention(ctx, plan, p, st));
   }
   return ws_release(ctx, st);
 }
