@@ -650,7 +650,7 @@ int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_
  *   y = clamp_i16(linear(x) + clamp_i16(rescale(dot(B[a][n], h), b_shifts + h_frac, out_frac)))
  * with the primitives of linear.rs:43-70 and :132-145; linear(x) is
  * myl_linear_dev of the same weight and requant plan (bias included). An
- * adapter of a smaller rank is padded with zero rows and columns. rank <= 256. */
+ * adapter of a smaller rank is padded with zero rows and columns. rank <= 256, in_features <= 2^18. */
 typedef struct myl_adapters myl_adapters;
 int myl_adapters_register(myl_ctx* ctx, int64_t num, int64_t rank, int64_t in_features,
                           int64_t out_features, const int8_t* A, const uint8_t* a_shifts,

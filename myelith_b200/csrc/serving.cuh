@@ -259,23 +259,40 @@ void prefix_params(PrefixParams& p, const myl_attn_plan* pl, const myl_prefix* p
   p.out_shift = pl->out_shift;
 }
 
-// y (int16, the projection's output) += the rows' adapters; the workspace is held.
+// Rows up to which a call counts as a decode batch: rows spread over as many
+// blocks as adapters, outputs by single threads.
+constexpr int64_t AD_FEW = 128;
+
+// h of the rows' adapters, then their share of y (int16, the projection's
+// output); the workspace is held.
 int run_adapter_shrink(myl_ctx* ctx, const myl_adapters* ad, AdapterParams& p, const int16_t* x, int64_t M,
                        int64_t ldx, const int32_t* ids, cudaStream_t st) {
   TRY(ensure(ctx->ad_h, size_t(M) * size_t(ad->ldb) * 2));
   p = AdapterParams{ad->A, ad->B, ad->sa, ad->sb, int(ad->num), int(ad->rank), ad->K, ad->N, ad->lda, int(ad->ldb),
                     ids, M, static_cast<int16_t*>(ctx->ad_h.p), ctx->d_err};
   const int aligned = aligned16(x) && ldx % 8 == 0;
-  const unsigned blocks = unsigned(std::min<int64_t>((M * ad->ldb + 7) / 8, int64_t(ctx->num_sms) * 64));
-  LaunchCfg lc(ctx, dim3(blocks), dim3(256), 0, st);
-  CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_shrink_kernel, x, ldx, aligned, p));
+  if (M <= AD_FEW) {
+    LaunchCfg lc(ctx, dim3(unsigned((M + 7) / 8), unsigned((ad->rank + 15) / 16), unsigned(std::min<int64_t>(8, std::min(ad->num, M)))),
+                 dim3(32 * 16), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_shrink_kernel<1, 1, 16>, x, ldx, aligned, p));
+  } else {
+    LaunchCfg lc(ctx, dim3(unsigned((M + 15) / 16), unsigned((ad->rank + 31) / 32)), dim3(32 * 8), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_shrink_kernel<2, 2, 8>, x, ldx, aligned, p));
+  }
   ctx->launches++;
   return MYL_OK;
 }
 
 int run_adapter_expand(myl_ctx* ctx, const AdapterParams& p, int16_t* y, int64_t ldy, cudaStream_t st) {
-  LaunchCfg lc(ctx, dim3(unsigned((p.N + 255) / 256), unsigned(std::min<int64_t>(p.M, 65535))), dim3(256), 0, st);
-  CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_expand_kernel, p, y, ldy));
+  const unsigned gx = unsigned((p.N + AD_ETHREADS - 1) / AD_ETHREADS);
+  if (p.M <= AD_FEW) {
+    LaunchCfg lc(ctx, dim3(gx, unsigned(p.M)), dim3(AD_ETHREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_expand_few_kernel, p, y, ldy));
+  } else {
+    const int aligned = aligned16(y) && ldy % 8 == 0;
+    LaunchCfg lc(ctx, dim3(gx, unsigned((p.M + AD_EROWS - 1) / AD_EROWS)), dim3(AD_ETHREADS), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, adapter_expand_kernel, p, y, ldy, aligned));
+  }
   ctx->launches++;
   return MYL_OK;
 }
@@ -434,8 +451,8 @@ int myl_adapters_register(myl_ctx* ctx, int64_t num, int64_t rank, int64_t in_fe
   if (num <= 0 || rank <= 0 || in_features <= 0 || out_features <= 0)
     return fail(MYL_ERR_SHAPE, "adapters: %lld of rank %lld over [%lld][%lld]", (long long)num, (long long)rank,
                 (long long)out_features, (long long)in_features);
-  if (rank > 256 || num > (1 << 20) || in_features > (int64_t(1) << 31) || out_features > (int64_t(1) << 31))
-    return fail(MYL_ERR_UNSUPPORTED, "adapters: rank at most 256, at most 2^20 adapters");
+  if (rank > 256 || num > (1 << 20) || in_features > AD_MAX_K || out_features > (int64_t(1) << 31))
+    return fail(MYL_ERR_UNSUPPORTED, "adapters: rank at most 256, 2^18 input features, 2^20 adapters");
   std::vector<int8_t> sa, sb;
   try {
     sa.resize(size_t(num * rank));
@@ -488,6 +505,7 @@ int myl_linear_adapters_dev(myl_ctx* ctx, const myl_weight* w, const myl_requant
                 (long long)w->N, (long long)w->K);
   if (M < 0 || ldx < w->K || ldy < w->N) return fail(MYL_ERR_SHAPE, "bad M/ldx/ldy");
   if (M == 0) return MYL_OK;
+  if (M > (1 << 20) - AD_EROWS) return fail(MYL_ERR_UNSUPPORTED, "%lld rows in one call", (long long)M);
   CUDA_TRY(cudaSetDevice(ctx->device));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   TRY(ws_acquire(ctx, st));
