@@ -56,9 +56,11 @@ struct PrefixParams {
   int lut_shift, prob_frac, out_shift;
   int32_t* scores;  // [nkv * R][lds]
   int64_t lds;
-  unsigned* rowmax;  // [nkv * R] as max (score ^ 0x80000000)
-  int32_t* rowsum;
+  // zero between calls
+  unsigned* rowmax;         // [nkv * R] as max (score ^ 0x80000000)
+  int32_t* rowsum;          // [nkv * R]
   unsigned long long* acc;  // [nkv * R][hd] int64 sums (two's complement)
+  unsigned* arrived;        // [nkv] blocks of the values pass that are done
   int16_t* out;
   int64_t ldo;
   int* err;
@@ -140,17 +142,6 @@ __global__ void __launch_bounds__(256)
     const int16_t vv = tile[x][r];
     vp[pfx_value_at(Pp, hd, g, j0 + x, 0, d)] = uint8_t((uint16_t(vv) >> 8) ^ 0x80);
     vp[pfx_value_at(Pp, hd, g, j0 + x, 1, d)] = uint8_t(vv & 255);
-  }
-}
-
-// ---- pass 0: empty maxima and sums -----------------------------------------------------
-__global__ void prefix_init_kernel(PrefixParams p, int64_t rows) {
-  pdl_wait();
-  pdl_launch();
-  const int64_t n = rows * p.hd;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
-    p.acc[i] = 0;
-    if (i < rows) p.rowmax[i] = 0;
   }
 }
 
@@ -267,7 +258,13 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_sum_kernel(PrefixParams p)
   const int32_t m = int32_t(p.rowmax[row] ^ 0x80000000u);
   const int32_t* sc = p.scores + row * p.lds;
   int32_t s = 0;  // the host bounds the keys so that the i32 sum cannot overflow
-  for (int j = threadIdx.x; j < p.P; j += PFX_THREADS) s += pfx_exp(p, m, sc[j]);
+  for (int j0 = threadIdx.x; j0 < p.P; j0 += 8 * PFX_THREADS) {
+    int32_t v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = j0 + u * PFX_THREADS < p.P ? sc[j0 + u * PFX_THREADS] : m;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += j0 + u * PFX_THREADS < p.P ? pfx_exp(p, m, v[u]) : 0;
+  }
   for (int j = threadIdx.x; j < n; j += PFX_THREADS) s += pfx_exp(p, m, sc[p.Pp + j]);
   s = __reduce_add_sync(0xffffffffu, s);
   if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = s;
@@ -304,11 +301,8 @@ __device__ __forceinline__ int dp2a_hi_uu(uint32_t a, uint32_t b, int c) {
 // 16-key groups of dimension d. p <= 2^prob_frac <= 2^15 is an unsigned 16-bit
 // operand; the sum of a row's probabilities is at most 2^prob_frac plus half a
 // unit per key, below 2^17, so sum p*vh and sum p*vl stay inside int32.
-__global__ void __launch_bounds__(PFX_THREADS) prefix_values_kernel(PrefixParams p, int nbp, int tiles) {
-  pdl_wait();
-  pdl_launch();
-  __shared__ __align__(16) uint16_t s_p[PFX_ROWS][PFX_VKEYS];
-  const int g = int(blockIdx.y) % p.nkv, rg = int(blockIdx.y) / p.nkv;
+__device__ __forceinline__ void prefix_values_block(const PrefixParams& p, int nbp, int tiles, int g, int rg,
+                                                    uint16_t (*s_p)[PFX_VKEYS]) {
   const bool suffix = int(blockIdx.x) >= nbp;
   const int per = suffix ? p.T * p.G : p.R;
   if (rg * PFX_ROWS >= per) return;
@@ -377,19 +371,45 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_values_kernel(PrefixParams
   }
 }
 
-// ---- pass 4: rounding and rescale ---------------------------------------------------------
-__global__ void prefix_finish_kernel(PrefixParams p, int64_t rows) {
-  pdl_wait();
-  pdl_launch();
-  const int64_t n = rows * p.hd;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
-    const int64_t row = i / p.hd;
+// Outputs [i0, ...) step `step` of the rows [row0, row0 + rows) from their sums,
+// which go back to zero, the row statistics too.
+__device__ __forceinline__ void prefix_finish(const PrefixParams& p, int64_t row0, int64_t rows, int64_t i0, int64_t step) {
+  for (int64_t i = i0; i < rows * p.hd; i += step) {
+    const int64_t row = row0 + i / p.hd;
     const int d = int(i % p.hd), g = int(row / p.R), rho = int(row % p.R);
-    const int64_t tot = int64_t(p.acc[i]);
+    const int64_t tot = int64_t(__ldcg(p.acc + row0 * p.hd + i));
     int32_t o = clamp16(p.prob_frac > 0 ? rshift_rne_i64(tot, p.prob_frac) : tot);
     if (p.out_shift != 0) o = clamp16(rescale_i32_s(o, p.out_shift));
     p.out[int64_t(rho / p.G) * p.ldo + int64_t(g * p.G + rho % p.G) * p.hd + d] = int16_t(o);
+    p.acc[row0 * p.hd + i] = 0;
+    if (d == 0) p.rowmax[row] = 0, p.rowsum[row] = 0;
   }
+}
+
+// merge: the last block of a KV head to finish also writes that head's outputs.
+__global__ void __launch_bounds__(PFX_THREADS) prefix_values_kernel(PrefixParams p, int nbp, int tiles, int merge) {
+  pdl_wait();
+  pdl_launch();
+  __shared__ __align__(16) uint16_t s_p[PFX_ROWS][PFX_VKEYS];
+  __shared__ bool s_last;
+  const int g = int(blockIdx.y) % p.nkv, rg = int(blockIdx.y) / p.nkv;
+  prefix_values_block(p, nbp, tiles, g, rg, s_p);
+  if (!merge) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(p.arrived + g, 1u) + 1 == gridDim.x * (gridDim.y / unsigned(p.nkv));
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  prefix_finish(p, int64_t(g) * p.R, p.R, threadIdx.x, PFX_THREADS);
+  if (threadIdx.x == 0) p.arrived[g] = 0;
+}
+
+// ---- pass 4 (many outputs a head): rounding and rescale -----------------------------------
+__global__ void prefix_finish_kernel(PrefixParams p, int64_t rows) {
+  pdl_wait();
+  pdl_launch();
+  prefix_finish(p, 0, rows, int64_t(blockIdx.x) * blockDim.x + threadIdx.x, int64_t(gridDim.x) * blockDim.x);
 }
 
 }  // namespace myl

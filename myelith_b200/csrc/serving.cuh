@@ -70,8 +70,15 @@ void free_handle(myl_ctx* ctx, T* h) {
   delete h;
 }
 
-// Query rows per KV head from which the prefix runs on the tensor cores.
-const int PTC_MIN_ROWS = std::getenv("MYL_PTC_MIN") ? std::atoi(std::getenv("MYL_PTC_MIN")) : 16;
+// Whether the prefix runs on the tensor cores: long enough for their five or six
+// launches, and enough rows to fill a tile's share of them. Measured (us, few-row
+// kernels / tensor cores; R rows per KV head, nkv heads, P positions):
+//   R 14, 4 heads, 2048: 22 / 25    R 28, 4, 2048: 29 / 27    R 56, 4, 500: 27 / 25
+//   R 7, 4 heads, 8192: 28 / 34     R 7, 4, 32749: 69 / 63    R 7, 2, 32749: 40 / 46
+//   R 105, 2 heads, 300: 20 / 25
+bool prefix_on_tensor_cores(const PrefixParams& p) {
+  return p.P >= 512 && int64_t(p.R) * p.R * p.nkv * p.P >= int64_t(1) << 22;
+}
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -209,23 +216,22 @@ int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p,
   p.err = ctx->d_err;
   const unsigned gy = unsigned(p.nkv * ((p.R + PFX_ROWS - 1) / PFX_ROWS));
   if (gy > 65535u) return fail(MYL_ERR_UNSUPPORTED, "%d query rows per KV head", p.R);
-  if (pl->tc && p.P > 0 && p.R >= PTC_MIN_ROWS && (p.hd == 64 || p.hd == 128))
+  if (pl->tc && (p.hd == 64 || p.hd == 128) && prefix_on_tensor_cores(p))
     return p.hd == 128 ? run_prefix_tc<128>(ctx, pl, p, st) : run_prefix_tc<64>(ctx, pl, p, st);
   p.lds = p.Pp + ((p.S + 31) & ~31);
-  const size_t o_max = size_t(rows) * size_t(p.hd) * 8, o_sum = o_max + size_t(rows) * 4,
-               o_sc = (o_sum + size_t(rows) * 4 + 255) & ~size_t(255);
-  TRY(ensure(ctx->pfx, o_sc + size_t(rows) * size_t(p.lds) * 4));
-  uint8_t* ws = static_cast<uint8_t*>(ctx->pfx.p);
-  p.acc = reinterpret_cast<unsigned long long*>(ws);
-  p.rowmax = reinterpret_cast<unsigned*>(ws + o_max);
-  p.rowsum = reinterpret_cast<int32_t*>(ws + o_sum);
-  p.scores = reinterpret_cast<int32_t*>(ws + o_sc);
-  const unsigned flat = unsigned(std::min<int64_t>((rows * p.hd + 255) / 256, int64_t(ctx->num_sms) * 8));
-  {
-    LaunchCfg lc(ctx, dim3(flat), dim3(256), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, prefix_init_kernel, p, rows));
-    ctx->launches++;
-  }
+  TRY(ensure(ctx->pfx, size_t(rows) * size_t(p.lds) * 4));
+  p.scores = static_cast<int32_t*>(ctx->pfx.p);
+  const size_t o_acc = size_t(rows) * 8;
+  TRY(zero_kept(ctx->pfx_stat, o_acc + size_t(rows) * size_t(p.hd) * 8 + size_t(p.nkv) * 4, st));
+  uint8_t* stat = static_cast<uint8_t*>(ctx->pfx_stat.p);
+  p.rowmax = reinterpret_cast<unsigned*>(stat);
+  p.rowsum = reinterpret_cast<int32_t*>(p.rowmax + rows);
+  p.acc = reinterpret_cast<unsigned long long*>(stat + o_acc);
+  p.arrived = reinterpret_cast<unsigned*>(p.acc + rows * p.hd);
+  // a head's outputs that one block writes in a few steps cost less there than
+  // another launch (7 rows of 128: 21 us with, 19 without, but a launch less to
+  // issue; 56 rows: 46 / 27)
+  const int merge = int64_t(p.R) * p.hd <= 4 * PFX_THREADS && (p.P > 0 || p.S > 0);
   if (p.P > 0 || p.S > 0) {
     const int nb1 = (p.P + PFX_SKEYS - 1) / PFX_SKEYS, t1 = (p.S + PFX_SKEYS - 1) / PFX_SKEYS;
     LaunchCfg l1(ctx, dim3(unsigned(nb1 + p.B * t1), gy), dim3(PFX_THREADS), 0, st);
@@ -234,12 +240,14 @@ int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p,
     CUDA_TRY(cudaLaunchKernelEx(&l2.cfg, prefix_sum_kernel, p));
     const int nb3 = (p.P + PFX_VKEYS - 1) / PFX_VKEYS, t3 = (p.S + PFX_VKEYS - 1) / PFX_VKEYS;
     LaunchCfg l3(ctx, dim3(unsigned(nb3 + p.B * t3), gy), dim3(PFX_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_values_kernel, p, nb3, t3));
+    CUDA_TRY(cudaLaunchKernelEx(&l3.cfg, prefix_values_kernel, p, nb3, t3, merge));
     ctx->launches += 3;
   }
-  LaunchCfg l4(ctx, dim3(flat), dim3(256), 0, st);
-  CUDA_TRY(cudaLaunchKernelEx(&l4.cfg, prefix_finish_kernel, p, rows));
-  ctx->launches++;
+  if (!merge) {
+    LaunchCfg l4(ctx, dim3(unsigned(std::min<int64_t>((rows * p.hd + 255) / 256, int64_t(ctx->num_sms) * 8))), dim3(256), 0, st);
+    CUDA_TRY(cudaLaunchKernelEx(&l4.cfg, prefix_finish_kernel, p, rows));
+    ctx->launches++;
+  }
   return MYL_OK;
 }
 

@@ -77,6 +77,11 @@ def check_attention(ctx, x, lens, c=PLAN):
     (1, 2, 6, 2, 248, 300, 35),
     (1, 1, 28, 4, 128, 4099, 3),      # longer prefixes
     (2, 9, 14, 2, 64, 2500, 77),
+    # many rows and a long enough prefix: whole and ragged row tiles, prefixes
+    # that end inside, at and just past a 128-position block
+    (16, 2, 7, 1, 128, 512, 9), (16, 2, 7, 1, 128, 513, 130), (32, 4, 4, 4, 128, 639, 5),
+    (37, 1, 28, 4, 128, 640, 17), (21, 3, 14, 2, 64, 641, 40), (64, 1, 14, 2, 64, 767, 0),
+    (9, 5, 28, 4, 128, 1025, 260), (130, 1, 2, 1, 64, 3001, 3), (1, 40, 14, 2, 64, 1500, 300),
 ])
 def test_prefix_attention(ctx, B, T, nq, nkv, hd, P, S):
     rng = np.random.default_rng(B * 1000 + P + hd)
@@ -91,7 +96,7 @@ def test_prefix_attention(ctx, B, T, nq, nkv, hd, P, S):
 def test_prefix_attention_extreme_values(ctx, hd, rows):
     """Rows of the type's lowest and highest values, scores that wrap i32, ties and equal rows."""
     rng = np.random.default_rng(hd + rows)
-    x = attention_problem(rng, rows, 1, 2, 1, hd, 200, 8)
+    x = attention_problem(rng, rows, 1, 2, 1, hd, 600, 8)
     x["q"][0] = -32768
     x["k"][0, :50] = -32768
     x["k"][0, 50:60] = 32767
@@ -117,7 +122,7 @@ def test_prefix_attention_extreme_values(ctx, hd, rows):
 @pytest.mark.parametrize("B", [1, 70])
 def test_prefix_attention_plans(ctx, change, B):
     rng = np.random.default_rng(7)
-    x = attention_problem(rng, B, 2, 4, 2, 64, 190, 12)
+    x = attention_problem(rng, B, 2, 4, 2, 64, 590, 12)
     check_attention(ctx, x, rng.integers(2, 13, size=B), {**PLAN, **change})
 
 
@@ -128,6 +133,9 @@ def test_prefix_attention_empty_rows_and_lengths(ctx):
     check_attention(ctx, x, [0, 1, 2, 6])  # rows without any key give zeros
     x = attention_problem(rng, 4, 3, 4, 2, 64, 65, 6)
     check_attention(ctx, x, [0, 1, 3, 6])
+    x = attention_problem(rng, 70, 3, 4, 2, 64, 565, 6)  # on the tensor cores
+    check_attention(ctx, x, rng.integers(0, 7, size=70))
+    check_attention(ctx, x, np.zeros(70))
     x = attention_problem(rng, 2, 1, 4, 2, 64, 65, 0)
     check_attention(ctx, x, [0, 0])
     x = attention_problem(rng, 2, 1, 4, 2, 64, 0, 0)
@@ -145,7 +153,7 @@ def test_prefix_attention_strides_and_streams(ctx, B):
     """Queries inside fused q/k/v rows, caches inside larger ones, position-major
     prefixes, a padded output, a stream of its own."""
     rng = np.random.default_rng(11)
-    T, nq, nkv, hd, P, S = 2, 4, 2, 64, 150, 10
+    T, nq, nkv, hd, P, S = 2, 4, 2, 64, 550, 10
     x = attention_problem(rng, B, T, nq, nkv, hd, P, S)
     lens = rng.integers(T, S + 1, size=B)
     ref = R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **PLAN)
@@ -217,6 +225,12 @@ def test_prefix_attention_rejects(ctx):
     with pytest.raises(myl.MylError):  # queries off 16-byte boundaries
         prefix.attention_dev(plan, wide.view(-1)[4:4 + 512].view(2, 1, 4, 64), ks, vs, lens, out)
     # lengths outside the capacity: clamped, and reported at the next check
+    big = attention_problem(rng, 70, 2, 4, 2, 64, 600, 8)
+    odd = rng.integers(-3, 12, size=70)
+    got = run_attention(ctx, big, odd, PLAN)
+    with pytest.raises(myl.MylError):
+        ctx.synchronize()
+    assert np.array_equal(got, R.prefix_attention(big["q"], big["k"], big["v"], big["ks"], big["vs"], odd, **PLAN))
     prefix.attention_dev(plan, q, ks, vs, dev(np.array([9, -1], np.int32)), out)
     with pytest.raises(myl.MylError) as e:
         torch.cuda.synchronize()
