@@ -214,6 +214,7 @@ struct KvCache {
   int64_t seq_stride;   // elements between sequences: L * n_kv * max_pos * hd
   int64_t layer_stride; // n_kv * max_pos * hd
   int64_t head_stride;  // max_pos * hd
+  int64_t pos_base;     // position of the first entry (a forked session: its prefix's length)
 };
 
 __device__ __forceinline__ int16_t rope_out(int32_t a, int frac) {
@@ -238,7 +239,7 @@ __global__ void rope_kv_kernel(int16_t* __restrict__ qkv, int64_t ldq, int64_t r
     const int64_t b = r / T, t = r % T;
     const int64_t pos = pos0_dev[0] + t;
     int16_t* row = qkv + r * ldq;
-    const int64_t cache_off = b * kc.seq_stride + int64_t(layer) * kc.layer_stride + pos * hd;
+    const int64_t cache_off = b * kc.seq_stride + int64_t(layer) * kc.layer_stride + (pos - kc.pos_base) * hd;
     if (e < n_rot) {
       const int h = e / half, j = e % half;
       const int64_t idx = pos % n_pos;

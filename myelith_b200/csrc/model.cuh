@@ -117,8 +117,25 @@ struct myl_session {
   int64_t* key_slots = nullptr;
   TpPeers peers{};
   unsigned long long* d_epoch = nullptr;
+  // a forked session: its sequences share the first prefix_len positions (one
+  // prefix and attention plan per layer); its own caches start after them
+  int64_t prefix_len = 0;
+  std::vector<myl_prefix*> prefixes;
+  std::vector<myl_attn_plan*> plans;
+  int32_t* d_lens = nullptr;  // [B] entries of the own caches, the new tokens included
+  // low-rank adapters by layer (may be null) and the sequences' adapter ids
+  std::vector<const myl_adapters*> ad_qkv, ad_o;
+  int32_t *d_seq_ids = nullptr, *d_row_ids = nullptr;  // [B], [rows_cap]
+  int16_t* xf_all = nullptr;  // final norms of every row (myl_forward_logits_dev)
   std::vector<void*> allocs;
 };
+
+// defined in serving.cuh
+static int session_prefix_attention(myl_ctx* ctx, myl_session* s, int64_t layer, int64_t T, cudaStream_t st);
+static int session_adapters(myl_ctx* ctx, myl_session* s, const myl_adapters* ad, const int16_t* x, int64_t ldx,
+                            int64_t rows, int16_t* y, int64_t ldy, cudaStream_t st);
+static int session_step(myl_ctx* ctx, myl_session* s, int64_t T, cudaStream_t st);
+static void session_unfork(myl_ctx* ctx, myl_session* s);
 
 namespace {
 
@@ -306,7 +323,10 @@ int session_alloc(myl_ctx* ctx, myl_session* s) {
   const myl_model* m = s->m;
   auto& A = s->allocs;
   const int64_t B = s->B, R = s->rows_cap, H = m->H;
-  s->cache.head_stride = s->max_pos * m->hd;
+  const bool fork = !s->prefixes.empty();
+  const int64_t cap = s->max_pos - s->prefix_len;  // entries of a sequence's own cache
+  s->cache.pos_base = s->prefix_len;
+  s->cache.head_stride = cap * m->hd;
   s->cache.layer_stride = m->nkv * s->cache.head_stride;
   s->cache.seq_stride = m->L * s->cache.layer_stride;
   const size_t cache_elems = size_t(B) * size_t(s->cache.seq_stride);
@@ -326,9 +346,11 @@ int session_alloc(myl_ctx* ctx, myl_session* s) {
   TRY(dev_alloc(A, &s->qkv, size_t(R * m->ldq)));
   TRY(dev_alloc(A, &s->attn, size_t(R * m->QD)));
   TRY(dev_alloc(A, &s->xf, size_t(B * H)));
-  TRY(dev_alloc(A, &s->scores, size_t(R * m->nq) * size_t(s->max_pos)));
+  // (a forked session's attention works in the context's workspace)
+  TRY(dev_alloc(A, &s->scores, fork ? 1 : size_t(R * m->nq) * size_t(s->max_pos)));
   s->max_chunks = int((s->max_pos + ATT_CHUNK - 1) / ATT_CHUNK);
-  TRY(dev_alloc(A, &s->part, size_t(s->part_rows * m->nq) * size_t(s->max_chunks) * size_t(m->hd)));
+  TRY(dev_alloc(A, &s->part, fork ? 1 : size_t(s->part_rows * m->nq) * size_t(s->max_chunks) * size_t(m->hd)));
+  if (fork) TRY(dev_alloc(A, &s->d_lens, size_t(B)));
   TRY(dev_alloc(A, &s->counters, size_t(s->part_rows * m->nq)));
   CUDA_TRY(cudaMemset(s->counters, 0, size_t(s->part_rows * m->nq) * sizeof(unsigned)));
   TRY(dev_alloc(A, &s->rowmax, size_t(R * m->nq)));
@@ -350,6 +372,7 @@ int session_alloc(myl_ctx* ctx, myl_session* s) {
 void release_session(myl_ctx* ctx, myl_session* s) {
   if (ctx) cudaSetDevice(ctx->device);
   if (s->graph) cudaGraphExecDestroy(s->graph);
+  session_unfork(ctx, s);
   for (auto& e : s->ev)
     if (e) cudaEventDestroy(e);
   for (void* p : s->allocs) cudaFree(p);
@@ -535,8 +558,9 @@ void tp_parts(const myl_session* s, int which, const int8_t* shift, ResidParams*
 // positions from s->d_pos). want_logits: the last token's logits into
 // s->logits. lds_len bounds the keys any row reads (the attention grids cover
 // it; a decode step captured once for all positions passes max_pos).
+// all_logits (world 1): instead, every row's logits into that [rows][V] array.
 int model_forward(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_t* tokens, int64_t T,
-                  bool want_logits, int64_t lds_len, cudaStream_t st) {
+                  bool want_logits, int64_t lds_len, cudaStream_t st, int32_t* all_logits = nullptr) {
   const int64_t rows = s->B * T, H = m->H;
   {
     LaunchCfg lc(ctx, dim3(unsigned(std::min<int64_t>(rows, 65535))), dim3(256), 0, st);
@@ -546,7 +570,8 @@ int model_forward(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_
                                 ctx->d_err));
   }
   ctx->launches++;
-  const bool tp = m->world > 1;
+  const bool tp = m->world > 1, fork = !s->prefixes.empty();
+  TRY(session_step(ctx, s, T, st));
   for (int64_t l = 0; l < m->L; ++l) {
     const ModelLayer& L = m->layers[size_t(l)];
     ResidParams rp{};
@@ -564,7 +589,9 @@ int model_forward(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_
     }
     TRY(launch_norm(ctx, m, x1, rows, rp, L.norm1, s->xn, nullptr, 0, st));
     TRY(dispatch_linear(ctx, L.w_qkv, s->xn, rows, H, make_ep(L.rq_qkv, s->qkv, m->ldq), st));
-    if (T > 1) {  // decode (T == 1): the RoPE runs inside the scores kernel
+    if (!s->ad_qkv.empty())
+      TRY(session_adapters(ctx, s, s->ad_qkv[size_t(l)], s->xn, H, rows, s->qkv, m->ldq, st));
+    if (T > 1 || fork) {  // decode (T == 1): the RoPE runs inside the scores kernel
       const int64_t items = (m->nq + m->nkv) * (m->hd / 2) + m->nkv * m->hd / ((m->hd % 8) ? 1 : 8);
       LaunchCfg lc(ctx, dim3(unsigned(std::min<int64_t>(rows, 65535)), unsigned((items + 255) / 256)),
                    dim3(256), 0, st);
@@ -575,7 +602,8 @@ int model_forward(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_
                                   s->cache, int(l)));
       ctx->launches++;
     }
-    TRY(run_attention(ctx, m, s, L, int(l), rows, T, lds_len, st));
+    if (fork) TRY(session_prefix_attention(ctx, s, l, T, st));
+    else TRY(run_attention(ctx, m, s, L, int(l), rows, T, lds_len, st));
     ResidParams ra{};
     ra.ld_add = H;
     ra.s1 = L.add_attn.s1;
@@ -589,6 +617,7 @@ int model_forward(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_
       tp_parts(s, 0, L.rq_o->d_shift, &ra);
     } else {
       TRY(dispatch_linear(ctx, L.w_o, s->attn, rows, m->QD, make_ep(L.rq_o, s->o, H), st));
+      if (!s->ad_o.empty()) TRY(session_adapters(ctx, s, s->ad_o[size_t(l)], s->attn, m->QD, rows, s->o, H, st));
       ra.add = s->o;
     }
     TRY(launch_norm(ctx, m, s->hid, rows, ra, L.norm2, s->xn, nullptr, 0, st));
@@ -608,6 +637,10 @@ int model_forward(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_
     rp.s1 = P.add_mlp.s1;
     rp.s2 = P.add_mlp.s2;
     if (tp) tp_parts(s, 1, P.mlp->d_shift_down, &rp);
+    if (all_logits) {
+      TRY(launch_norm(ctx, m, s->mid, rows, rp, m->final_norm, s->xf_all, nullptr, 0, st));
+      return dispatch_linear(ctx, m->head, s->xf_all, rows, H, make_ep(m->rq_head, all_logits, m->V), st);
+    }
     const int64_t* sel = nullptr;
     if (T > 1) {
       if (s->last_rows_T != T) {
@@ -895,7 +928,7 @@ int myl_session_release(myl_ctx* ctx, myl_session* s) {
 int myl_session_reset(myl_ctx* ctx, myl_session* s) {
   if (!ctx || !s) return fail(MYL_ERR_ARG, "null argument");
   CUDA_TRY(cudaSetDevice(ctx->device));
-  return set_pos(s, 0, ctx->stream);
+  return set_pos(s, s->prefix_len, ctx->stream);
 }
 
 int64_t myl_session_position(const myl_session* s) { return s ? s->pos : -1; }
@@ -1060,6 +1093,8 @@ int myl_generate(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_t
     return fail(MYL_ERR_ARG, "null argument");
   if (P <= 0 || max_new < 0) return fail(MYL_ERR_SHAPE, "P = %lld, max_new = %lld", (long long)P,
                                          (long long)max_new);
+  if (!s->prefixes.empty())
+    return fail(MYL_ERR_ARG, "a forked session continues its prefix: use myl_forward and myl_decode_greedy");
   if (P + max_new > s->max_pos)
     return fail(MYL_ERR_SHAPE, "%lld positions beyond the session's %lld", (long long)(P + max_new),
                 (long long)s->max_pos);

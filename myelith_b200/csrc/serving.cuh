@@ -342,7 +342,218 @@ int run_verify(myl_ctx* ctx, VerifyParams& p, cudaStream_t st) {
   return MYL_OK;
 }
 
+// Per-step state of a session's serving parts: the own caches' lengths and each
+// row's adapter id, from the device position (a captured step replays it).
+__global__ void session_step_kernel(const int64_t* __restrict__ pos, int64_t prefix_len, int64_t B, int64_t T,
+                                    int32_t* __restrict__ lens, const int32_t* __restrict__ seq_ids,
+                                    int32_t* __restrict__ row_ids) {
+  pdl_wait();
+  pdl_launch();
+  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < B * T; i += int64_t(gridDim.x) * blockDim.x) {
+    if (lens && i < B) lens[i] = int32_t(pos[0] + T - prefix_len);
+    if (row_ids) row_ids[i] = seq_ids[i / T];
+  }
+}
+
 }  // namespace
+
+static int session_step(myl_ctx* ctx, myl_session* s, int64_t T, cudaStream_t st) {
+  if (!s->d_lens && !s->d_row_ids) return MYL_OK;
+  LaunchCfg lc(ctx, dim3(unsigned(std::min<int64_t>((s->B * T + 255) / 256, 64))), dim3(256), 0, st);
+  CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, session_step_kernel, static_cast<const int64_t*>(s->d_pos), s->prefix_len, s->B, T,
+                              s->d_lens, static_cast<const int32_t*>(s->d_seq_ids), s->d_row_ids));
+  ctx->launches++;
+  return MYL_OK;
+}
+
+static int session_adapters(myl_ctx* ctx, myl_session* s, const myl_adapters* ad, const int16_t* x, int64_t ldx,
+                            int64_t rows, int16_t* y, int64_t ldy, cudaStream_t st) {
+  if (!ad) return MYL_OK;
+  AdapterParams p;
+  TRY(run_adapter_shrink(ctx, ad, p, x, rows, ldx, s->d_row_ids, st));
+  return run_adapter_expand(ctx, p, y, ldy, st);
+}
+
+// Attention of one layer of a forked session over B * T rotated query rows.
+static int session_prefix_attention(myl_ctx* ctx, myl_session* s, int64_t layer, int64_t T, cudaStream_t st) {
+  const myl_model* m = s->m;
+  PrefixParams p{};
+  prefix_params(p, s->plans[size_t(layer)], s->prefixes[size_t(layer)]);
+  p.q = s->qkv;
+  p.ldq = m->ldq;
+  p.B = int(s->B);
+  p.T = int(T);
+  p.nq = int(m->nq);
+  p.G = int(m->G);
+  p.R = int(s->B * T * m->G);
+  p.ks = s->cache.k + layer * s->cache.layer_stride;
+  p.vs = s->cache.v + layer * s->cache.layer_stride;
+  p.seq_stride = s->cache.seq_stride;
+  p.head_stride = s->cache.head_stride;
+  p.pos_stride = m->hd;
+  p.S = int(s->max_pos - s->prefix_len);
+  p.lens = s->d_lens;
+  p.out = s->attn;
+  p.ldo = m->QD;
+  return run_prefix_attention(ctx, s->plans[size_t(layer)], p, st);
+}
+
+static void session_unfork(myl_ctx* ctx, myl_session* s) {
+  for (myl_prefix* p : s->prefixes)
+    if (p) free_handle(ctx, p);
+  for (myl_attn_plan* p : s->plans)
+    if (p) free_handle(ctx, p);
+  s->prefixes.clear();
+  s->plans.clear();
+}
+
+// The caches of sequence `seq` of `parent` as the new session's prefix.
+static int session_share(myl_ctx* ctx, myl_session* s, const myl_session* parent, int64_t seq) {
+  const myl_model* m = s->m;
+  std::vector<int16_t> lut;
+  try {
+    lut.resize(size_t(m->exp_len));
+    s->prefixes.assign(size_t(m->L), nullptr);
+    s->plans.assign(size_t(m->L), nullptr);
+  } catch (const std::exception&) {
+    return fail(MYL_ERR_UNSUPPORTED, "out of host memory");
+  }
+  CUDA_TRY(cudaMemcpy(lut.data(), m->d_exp, lut.size() * 2, cudaMemcpyDeviceToHost));
+  const KvCache& c = parent->cache;
+  for (int64_t l = 0; l < m->L; ++l) {
+    const ModelLayer& L = m->layers[size_t(l)];
+    TRY(myl_attn_plan_create(ctx, m->score_mult, uint8_t(L.score_shift), lut.data(), m->exp_len, uint8_t(m->lut_shift),
+                             m->prob_frac, L.out_shift, &s->plans[size_t(l)]));
+    const int64_t at = seq * c.seq_stride + l * c.layer_stride;
+    TRY(myl_prefix_create(ctx, c.k + at, c.v + at, parent->pos, m->nkv, m->hd, m->hd, c.head_stride, ctx->stream,
+                          &s->prefixes[size_t(l)]));
+  }
+  return MYL_OK;
+}
+
+extern "C" {
+
+int myl_session_fork(myl_ctx* ctx, const myl_model* m, const myl_session* parent, int64_t seq, int64_t batch,
+                     int64_t max_new, myl_session** out) {
+  if (!ctx || !m || !parent || !out || parent->m != m) return fail(MYL_ERR_ARG, "null argument or another model's session");
+  *out = nullptr;
+  if (m->world > 1) return fail(MYL_ERR_UNSUPPORTED, "forks of tensor-parallel sessions");
+  if (!parent->prefixes.empty()) return fail(MYL_ERR_UNSUPPORTED, "a fork of a forked session");
+  if (batch <= 0 || max_new <= 0 || seq < 0 || seq >= parent->B || parent->pos <= 0)
+    return fail(MYL_ERR_SHAPE, "fork of sequence %lld at position %lld into %lld sequences of %lld more positions",
+                (long long)seq, (long long)parent->pos, (long long)batch, (long long)max_new);
+  if (int64_t(m->exp_max) * (parent->pos + max_new) > INT32_MAX)
+    return fail(MYL_ERR_OVERFLOW, "%lld positions overflow the softmax's i32 sum", (long long)(parent->pos + max_new));
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  CUDA_TRY(cudaStreamSynchronize(ctx->stream));  // the parent's caches are complete
+  myl_session* s = new myl_session();
+  s->m = m;
+  s->B = batch;
+  s->prefix_len = parent->pos;
+  s->max_pos = parent->pos + max_new;
+  s->rows_cap = std::max<int64_t>(batch, std::min<int64_t>(1024, batch * max_new));
+  s->part_rows = batch;
+  int rc = session_share(ctx, s, parent, seq);
+  if (rc == MYL_OK) rc = session_alloc(ctx, s);
+  if (rc == MYL_OK) rc = set_pos(s, s->prefix_len, ctx->stream);
+  // the parent's last logits are every sequence's, so that decoding can start at once
+  for (int64_t b = 0; rc == MYL_OK && b < batch; ++b)
+    if (cudaMemcpyAsync(s->logits + b * m->V, parent->logits + seq * m->V, size_t(m->V) * 4, cudaMemcpyDeviceToDevice,
+                        ctx->stream) != cudaSuccess)
+      rc = fail(MYL_ERR_CUDA, "logits copy");
+  if (rc != MYL_OK) {
+    release_session(ctx, s);
+    return rc;
+  }
+  *out = s;
+  return MYL_OK;
+}
+
+int myl_session_rewind(myl_ctx* ctx, myl_session* s, int64_t position) {
+  if (!ctx || !s) return fail(MYL_ERR_ARG, "null argument");
+  if (position < s->prefix_len || position > s->pos)
+    return fail(MYL_ERR_SHAPE, "position %lld outside [%lld, %lld]", (long long)position, (long long)s->prefix_len,
+                (long long)s->pos);
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  return set_pos(s, position, ctx->stream);
+}
+
+int myl_session_set_adapters(myl_ctx* ctx, myl_session* s, int64_t layer, int projection, const myl_adapters* ad) {
+  if (!ctx || !s) return fail(MYL_ERR_ARG, "null argument");
+  const myl_model* m = s->m;
+  if (m->world > 1) return fail(MYL_ERR_UNSUPPORTED, "adapters of tensor-parallel sessions");
+  if (layer < 0 || layer >= m->L || (projection != MYL_PROJ_QKV && projection != MYL_PROJ_O))
+    return fail(MYL_ERR_SHAPE, "layer %lld, projection %d", (long long)layer, projection);
+  const bool o = projection == MYL_PROJ_O;
+  const int64_t N = o ? m->H : m->QD + 2 * m->KD, K = o ? m->QD : m->H;
+  if (ad && (ad->N != N || ad->K != K))
+    return fail(MYL_ERR_SHAPE, "adapters are [%lld][%lld], the projection [%lld][%lld]", (long long)ad->N,
+                (long long)ad->K, (long long)N, (long long)K);
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+  if (!s->d_row_ids) {
+    TRY(dev_alloc(s->allocs, &s->d_seq_ids, size_t(s->B)));
+    TRY(dev_alloc(s->allocs, &s->d_row_ids, size_t(s->rows_cap)));
+    CUDA_TRY(cudaMemset(s->d_seq_ids, 0xFF, size_t(s->B) * 4));  // -1: none
+  }
+  try {
+    std::vector<const myl_adapters*>& list = o ? s->ad_o : s->ad_qkv;
+    if (list.empty()) list.assign(size_t(m->L), nullptr);
+    list[size_t(layer)] = ad;
+  } catch (const std::exception&) {
+    return fail(MYL_ERR_UNSUPPORTED, "out of host memory");
+  }
+  if (s->graph) {  // the decode step is captured again
+    cudaGraphExecDestroy(s->graph);
+    s->graph = nullptr;
+  }
+  return MYL_OK;
+}
+
+int myl_session_set_adapter_ids(myl_ctx* ctx, myl_session* s, const int32_t* ids) {
+  if (!ctx || !s || !ids) return fail(MYL_ERR_ARG, "null argument");
+  if (!s->d_row_ids) return fail(MYL_ERR_ARG, "the session has no adapters");
+  for (int64_t b = 0; b < s->B; ++b) {
+    int64_t num = INT32_MAX;
+    for (const auto* list : {&s->ad_qkv, &s->ad_o})
+      for (const myl_adapters* ad : *list)
+        if (ad) num = std::min(num, ad->num);
+    if (ids[b] < -1 || ids[b] >= num) return fail(MYL_ERR_SHAPE, "adapter id %d", ids[b]);
+  }
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+  CUDA_TRY(cudaMemcpy(s->d_seq_ids, ids, size_t(s->B) * 4, cudaMemcpyHostToDevice));
+  return MYL_OK;
+}
+
+int myl_forward_logits_dev(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_t* tokens, int64_t T,
+                           int32_t* logits) {
+  if (!ctx || !m || !s || s->m != m || !tokens || !logits) return fail(MYL_ERR_ARG, "null argument");
+  if (m->world > 1) return fail(MYL_ERR_UNSUPPORTED, "logits of every position need the whole vocabulary (world 1)");
+  if (T <= 0 || s->B * T > s->rows_cap || s->pos + T > s->max_pos)
+    return fail(MYL_ERR_SHAPE, "%lld tokens at position %lld (at most %lld a call, %lld positions)", (long long)T,
+                (long long)s->pos, (long long)(s->rows_cap / s->B), (long long)s->max_pos);
+  for (int64_t i = 0; i < s->B * T; ++i)
+    if (tokens[i] < 0 || tokens[i] >= m->V_global)
+      return fail(MYL_ERR_SHAPE, "token id %d outside the vocabulary", tokens[i]);
+  CUDA_TRY(cudaSetDevice(ctx->device));
+  cudaStream_t st = ctx->stream;
+  if (!s->xf_all) TRY(dev_alloc(s->allocs, &s->xf_all, size_t(s->rows_cap * m->H)));
+  TRY(ws_acquire(ctx, st));
+  CUDA_TRY(cudaStreamSynchronize(st));  // the pinned token buffer is free again
+  std::memcpy(s->h_tokens, tokens, size_t(s->B * T) * 4);
+  CUDA_TRY(cudaMemcpyAsync(s->tok_in, s->h_tokens, size_t(s->B * T) * 4, cudaMemcpyHostToDevice, st));
+  TRY(set_pos(s, s->pos, st));
+  {
+    PdlScope pdl(ctx);
+    TRY(model_forward(ctx, m, s, s->tok_in, T, true, s->pos + T, st, logits));
+  }
+  TRY(set_pos(s, s->pos + T, st));
+  TRY(ws_release(ctx, st));
+  return check_device_error(ctx);
+}
+
+}  // extern "C"
 
 extern "C" {
 

@@ -8,6 +8,12 @@ libmyl_w8a16.so (``myl_model_*``, include/myl_w8a16.h):
   Session(model, batch, max_positions)     kv_cache.rs:13-36 KVCache::new
   Session.forward(tokens)                  model.rs:229-311 forward_token (T tokens)
   Session.decode(n, digest=...)            generate.rs:101-113 / :181-196 (greedy)
+  Session.fork(batch, max_new)             no counterpart: sequences that share the
+                                           session's positions as one prefix
+  Session.set_adapters / forward_logits_dev / rewind
+                                           no counterpart: low-rank adapters per
+                                           sequence; logits of every position and
+                                           the step back for drafted tokens
   IntegerModel.generate(prompt, n,         generate.rs:76-116 generate (greedy) and,
                         digest=True)       :161-200 dekodieren_mit_digest
 
@@ -203,6 +209,11 @@ def _lib():
                 ("myl_model_shard", [vp, C.POINTER(i64)], i32),
                 ("myl_session_tp_bytes", [vp], i64),
                 ("myl_session_set_tp", [vp, vp, C.POINTER(vp)], i32),
+                ("myl_session_fork", [vp, vp, vp, i64, i64, i64, C.POINTER(vp)], i32),
+                ("myl_session_rewind", [vp, vp, i64], i32),
+                ("myl_session_set_adapters", [vp, vp, i64, i32, vp], i32),
+                ("myl_session_set_adapter_ids", [vp, vp, vp], i32),
+                ("myl_forward_logits_dev", [vp, vp, vp, vp, i64, vp], i32),
                 ("myl_session_timing", [vp, C.POINTER(C.c_float), C.POINTER(C.c_float)], i32),
                 ("myl_rmsnorm_i16", [vp, vp, i64, i64, vp, vp, vp, vp, i64, C.c_uint8, C.c_uint8,
                                      i64, C.c_uint8, vp], i32),
@@ -340,6 +351,54 @@ class Session:
         self.model = model
         self.batch = batch
         self.max_positions = max_positions
+
+    @classmethod
+    def _forked(cls, parent: "Session", seq: int, batch: int, max_new: int) -> "Session":
+        h = C.c_void_p()
+        model = parent.model
+        _check("myl_session_fork", _lib().myl_session_fork(
+            model.ctx.handle, model.handle, parent.handle, seq, batch, max_new, C.byref(h)))
+        s = cls.__new__(cls)
+        s._h, s.model, s.batch = h, model, batch
+        s.max_positions = parent.position + max_new
+        return s
+
+    def fork(self, batch: int, max_new: int, seq: int = 0) -> "Session":
+        """`batch` sequences that continue sequence `seq` of this session for up
+        to max_new positions each, its positions shared as one prefix
+        (myl_session_fork); equal to sessions that hold the prompt themselves."""
+        return Session._forked(self, seq, batch, max_new)
+
+    def rewind(self, position: int) -> None:
+        """Forgets the positions from `position` on."""
+        _check("myl_session_rewind", _lib().myl_session_rewind(self.model.ctx.handle, self._h, position))
+
+    def set_adapters(self, layer: int, projection: str, adapters) -> None:
+        """Low-rank adapters (Adapters, or None) of a layer's "qkv" rows or "o"
+        projection; set_adapter_ids chooses each sequence's."""
+        _check("myl_session_set_adapters", _lib().myl_session_set_adapters(
+            self.model.ctx.handle, self._h, layer, {"qkv": 0, "o": 1}[projection],
+            None if adapters is None else adapters.handle))
+        self._adapters = {**getattr(self, "_adapters", {}), (layer, projection): adapters}
+
+    def set_adapter_ids(self, ids) -> None:
+        """Each sequence's adapter (-1: none)."""
+        a = np.ascontiguousarray(np.asarray(ids, np.int32)).reshape(self.batch)
+        _check("myl_session_set_adapter_ids", _lib().myl_session_set_adapter_ids(
+            self.model.ctx.handle, self._h, a.ctypes.data))
+
+    def forward_logits_dev(self, tokens, logits) -> None:
+        """forward() of tokens [batch][T] whose logits of every position go to the
+        torch CUDA tensor logits [batch, T, vocab] int32."""
+        from . import MYL_ERR_SHAPE, MylError
+
+        t = np.ascontiguousarray(np.asarray(tokens, np.int32)).reshape(self.batch, -1)
+        if str(logits.dtype) != "torch.int32" or not logits.is_cuda or not logits.is_contiguous() or \
+                tuple(logits.shape) != (self.batch, t.shape[1], self.model.vocab):
+            raise MylError("myl_forward_logits_dev", MYL_ERR_SHAPE,
+                           f"logits {tuple(logits.shape)} {logits.dtype} for tokens {t.shape}")
+        _check("myl_forward_logits_dev", _lib().myl_forward_logits_dev(
+            self.model.ctx.handle, self.model.handle, self._h, t.ctypes.data, t.shape[1], logits.data_ptr()))
 
     @property
     def handle(self):
