@@ -305,25 +305,27 @@ int run_adapter_expand(myl_ctx* ctx, const AdapterParams& p, int16_t* y, int64_t
   return MYL_OK;
 }
 
-// A cluster per position where the rows' slices fit its CTAs' shared memory,
-// a block per row otherwise.
+// A cluster per position where the rows' slices fit its CTAs' shared memory and
+// the table's reach 16 bits, a block per row otherwise.
 int run_verify(myl_ctx* ctx, VerifyParams& p, cudaStream_t st) {
   const int64_t units = int64_t(p.B) * (p.D + 1);
-  const int64_t logit_bytes = p.draft ? 8 : 4;
-  // slices of at most 78 KB, so that two CTAs share an SM and one loads while
-  // the other sweeps; smaller ones where that leaves SMs without a CTA
+  const int64_t logit_bytes = p.draft ? 4 : 2;
+  // Slices of at most 40 KB, so that four CTAs share an SM and some load while
+  // others sweep; smaller ones as long as the SMs hold the CTAs at once (us with 4,
+  // 8, 16 CTAs a position: 5 positions of 151936 30 / 20 / 14; 80 of 32000 17 / 13
+  // / 19; 384 of 32000 32 / 37 / 66; 384 of 152064 without draft logits 84 / 59 / 78).
   int cl = 1;
-  while (cl < VERIFY_MAX_CL && p.V * logit_bytes > int64_t(cl) * 78 * 1024) cl *= 2;
-  while (cl < VERIFY_MAX_CL && 2 * units * cl <= ctx->num_sms && p.V >= cl * 4096) cl *= 2;
+  while (cl < VERIFY_MAX_CL && p.V * logit_bytes > int64_t(cl) * 40 * 1024) cl *= 2;
+  while (cl < VERIFY_MAX_CL && 2 * units * cl <= 6 * int64_t(ctx->num_sms) && p.V >= cl * 4096) cl *= 2;
   p.per = int(((p.V + cl - 1) / cl + 3) & ~3);
   const int64_t smem = p.per * logit_bytes;
-  if (smem <= VERIFY_SMEM && units * cl <= INT32_MAX) {
+  if (p.per <= VERIFY_PIECES * VERIFY_PIECE && p.reach < VERIFY_FAR && units * cl <= INT32_MAX) {
     TRY(zero_kept(ctx->vfy_done, size_t(p.B) * 4, st));
     TRY(ensure(ctx->vfy, size_t(units) * 4));
     p.done = static_cast<unsigned*>(ctx->vfy_done.p);
     p.pos = static_cast<int32_t*>(ctx->vfy.p);
     const void* fn = reinterpret_cast<const void*>(&verify_cluster_kernel);
-    TRY(kernel_smem_occupancy(ctx->device, fn, VERIFY_THREADS, VERIFY_SMEM, nullptr));
+    TRY(kernel_smem_occupancy(ctx->device, fn, VERIFY_THREADS, 4 * VERIFY_PIECES * VERIFY_PIECE, nullptr));
     if (cl > 8) CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     LaunchCfg lc(ctx, dim3(unsigned(units * cl)), dim3(VERIFY_THREADS), size_t(smem), st, unsigned(cl));
     CUDA_TRY(cudaLaunchKernelEx(&lc.cfg, verify_cluster_kernel, p, cl));

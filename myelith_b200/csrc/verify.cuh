@@ -19,11 +19,13 @@
 
 namespace myl {
 
-constexpr int VERIFY_THREADS = 512;
+constexpr int VERIFY_THREADS = 256;
 constexpr int VERIFY_WARPS = VERIFY_THREADS / 32;
-constexpr int VERIFY_MAX_CL = 16;         // CTAs per cluster (16 is the opt-in size)
-constexpr int VERIFY_SMEM = 220 * 1024;   // bytes of logits a CTA may hold
-constexpr int VERIFY_U = 5;               // 16-byte loads in flight per thread and row
+constexpr int VERIFY_MAX_CL = 16;                  // CTAs per cluster (16 is the opt-in size)
+constexpr int VERIFY_U = 5;                        // 16-byte loads in flight per thread and row
+constexpr int VERIFY_PIECE = 4 * VERIFY_U * VERIFY_THREADS;  // logits of a CTA's batch
+constexpr int VERIFY_PIECES = 10;                  // batches a CTA may hold: 2 rows x 2 bytes x 51200
+constexpr int VERIFY_FAR = 65535;                  // differences are kept in 16 bits
 
 struct VerifyParams {
   const int32_t* target;  // [B][D + 1][V] with strides
@@ -81,134 +83,143 @@ __device__ __forceinline__ int verify_count(const VerifyParams& p, int b) {
 // ---- one pass: a cluster per position --------------------------------------------------
 // Position i of request b is one cluster: its CTAs hold the target row and the
 // draft row in shared memory, a slice each, so that every logit is read from
-// HBM once. Maxima and weight sums cross the cluster through distributed
-// shared memory (two cluster barriers), the draw of a rejected position takes
-// a third; accepted positions stop after the second. All CTAs of a cluster
-// reach the same decisions from the same words. Weights past `reach` are zero,
-// so a slice is swept with one comparison per logit against max - reach, and a
-// warp looks the table up only where one of its logits passes. Positions past
-// the drafted ones are not read. The last position of a request to finish (a
-// counter per request) writes its output.
+// HBM once. A logit is kept as its 16-bit distance to the maximum of the 640 that
+// a warp loaded together (farther ones saturate; the host sends only tables
+// whose reach is below that here): half the bytes, twice the clusters on the
+// GPU, whose latency - loads, two or three cluster barriers - is what bounds a
+// batch (64 requests x 5 drafts: 142 us with 32-bit logits and half the
+// clusters). Maxima and weight sums cross the cluster through distributed shared
+// memory, the draw of a rejected position takes a third barrier; accepted
+// positions stop after the second. All CTAs of a cluster reach the same
+// decisions from the same words. Weights past `reach` are zero, so a warp looks
+// the table up only where one of its logits comes that near to the maximum.
+// Positions past the drafted ones are not read. The last position of a request to
+// finish (a counter per request) writes its output. (Clusters that stay and take
+// positions in turn were slower, 132 us: the hardware spreads uneven positions
+// better.)
 struct VerifyShared {
   int32_t mx[2][VERIFY_MAX_CL];              // slice maxima by CTA: target, draft
   unsigned long long sum[2][VERIFY_MAX_CL];  // slice weight sums
   unsigned long long rho[VERIFY_MAX_CL];     // slice sums of the residual weights
   int32_t wmax[2][VERIFY_WARPS];
   unsigned long long wsum[2][VERIFY_WARPS];
+  int32_t ref[2][VERIFY_PIECES][VERIFY_WARPS];  // what the distances are measured from
 };
 
 __device__ __forceinline__ void verify_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void verify_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// Copies n logits of each row (ROWS = 1: the first alone) to shared memory,
-// all rows' loads of a batch in flight together; m: this thread's maxima.
-// Rows off 16-byte boundaries are read by single words.
+// Loads n logits of each row (ROWS = 1: the first alone), all rows' loads of a
+// batch in flight together, and keeps their distances; m: the warp's maxima.
+// Thread t has the vectors t, t + VERIFY_THREADS, ... of four logits.
 template <int ROWS>
-__device__ __forceinline__ void verify_load(const int32_t* const (&row)[2], int n, int32_t* const (&s)[2],
-                                            int32_t (&m)[2]) {
-  bool vec = true;
+__device__ __forceinline__ void verify_load(const int32_t* const (&row)[2], int n, uint16_t* const (&s)[2],
+                                            VerifyShared& sm, int32_t (&m)[2]) {
+  const int warp = threadIdx.x >> 5;
+  for (int p0 = 0; p0 * VERIFY_PIECE < n; ++p0) {
+    int4 x[ROWS][VERIFY_U];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) vec = vec && (reinterpret_cast<uintptr_t>(row[r]) & 15) == 0;
-  int done = 0;
-  if (vec) {
-    const int nv = n / 4;
-    done = 4 * nv;
-    for (int v0 = threadIdx.x; v0 < nv; v0 += VERIFY_U * VERIFY_THREADS) {
-      int4 x[ROWS][VERIFY_U];
+    for (int r = 0; r < ROWS; ++r) {
+      const bool vec = (reinterpret_cast<uintptr_t>(row[r]) & 15) == 0;
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-        for (int u = 0; u < VERIFY_U; ++u) {
-          const int v = v0 + u * VERIFY_THREADS;
-          if (v < nv) x[r][u] = __ldcs(reinterpret_cast<const int4*>(row[r]) + v);
+      for (int u = 0; u < VERIFY_U; ++u) {
+        const int j = p0 * VERIFY_PIECE + 4 * (u * VERIFY_THREADS + int(threadIdx.x));
+        const int32_t* at = row[r] + j;
+        if (vec && j + 4 <= n) {
+          x[r][u] = __ldcs(reinterpret_cast<const int4*>(at));
+        } else {
+          x[r][u].x = j < n ? __ldg(at) : INT32_MIN;
+          x[r][u].y = j + 1 < n ? __ldg(at + 1) : INT32_MIN;
+          x[r][u].z = j + 2 < n ? __ldg(at + 2) : INT32_MIN;
+          x[r][u].w = j + 3 < n ? __ldg(at + 3) : INT32_MIN;
         }
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-        for (int u = 0; u < VERIFY_U; ++u) {
-          const int v = v0 + u * VERIFY_THREADS;
-          if (v < nv) {
-            const int4 y = x[r][u];
-            reinterpret_cast<int4*>(s[r])[v] = y;
-            m[r] = max(m[r], max(max(y.x, y.y), max(y.z, y.w)));
-          }
-        }
+      }
     }
-  }
-  for (int j0 = done + int(threadIdx.x); j0 < n; j0 += 4 * VERIFY_U * VERIFY_THREADS) {
-    int32_t x[ROWS][4 * VERIFY_U];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
+    for (int r = 0; r < ROWS; ++r) {
+      int32_t t = INT32_MIN;
 #pragma unroll
-      for (int u = 0; u < 4 * VERIFY_U; ++u) {
-        const int j = j0 + u * VERIFY_THREADS;
-        if (j < n) x[r][u] = __ldcs(row[r] + j);
+      for (int u = 0; u < VERIFY_U; ++u) t = max(t, max(max(x[r][u].x, x[r][u].y), max(x[r][u].z, x[r][u].w)));
+      t = __reduce_max_sync(0xffffffffu, t);
+      if ((threadIdx.x & 31) == 0) sm.ref[r][p0][warp] = t;
+      m[r] = max(m[r], t);
+      auto far = [t](int32_t l) { return min(uint32_t(t) - uint32_t(l), uint32_t(VERIFY_FAR)); };
+#pragma unroll
+      for (int u = 0; u < VERIFY_U; ++u) {
+        const int j = p0 * VERIFY_PIECE + 4 * (u * VERIFY_THREADS + int(threadIdx.x));
+        if (j < n)
+          *reinterpret_cast<uint2*>(s[r] + j) = make_uint2(far(x[r][u].x) | far(x[r][u].y) << 16, far(x[r][u].z) | far(x[r][u].w) << 16);
       }
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-      for (int u = 0; u < 4 * VERIFY_U; ++u) {
-        const int j = j0 + u * VERIFY_THREADS;
-        if (j < n) m[r] = max(m[r], s[r][j] = x[r][u]);
-      }
+    }
   }
 }
 
-// Replaces n logits in shared memory by their weights and returns this
-// thread's sum (S < 2^32 over all slices). A warp whose vectors hold no logit
-// at the floor or above writes zeros without looking the table up.
-__device__ __forceinline__ uint32_t verify_sum(const VerifyParams& p, int32_t* s, int n, int32_t m) {
-  const int32_t t = verify_floor(p, m);
+// The weight at distance d from the maximum (d <= VERIFY_FAR plus a bounded rest).
+__device__ __forceinline__ uint32_t verify_weight_at(const VerifyParams& p, uint32_t d) {
+  const uint32_t idx = __umulhi(d << p.pre, p.scaled) >> p.post;
+  return uint32_t(uint16_t(__ldg(p.lut + (d <= uint32_t(p.reach) ? idx : uint32_t(p.lut_len)))));
+}
+
+// Replaces n distances of row r by their weights (at most 32767) and returns
+// this thread's sum (S < 2^32 over all slices).
+__device__ __forceinline__ uint32_t verify_sum(const VerifyParams& p, uint16_t* s, int n, int r, const VerifyShared& sm,
+                                               int32_t m) {
+  const int warp = threadIdx.x >> 5;
   uint32_t w = 0;
-  for (int v0 = 0; 4 * v0 < n; v0 += VERIFY_THREADS) {
-    const int v = v0 + int(threadIdx.x);
-    const int left = n - 4 * v;  // logits of the vector inside the slice
-    int4 x = make_int4(0, 0, 0, 0);
-    if (left > 0) x = reinterpret_cast<const int4*>(s)[v];
-    if (__any_sync(0xffffffffu, left > 0 && max(max(x.x, x.y), max(x.z, x.w)) >= t)) {
-      x.x = int32_t(verify_weight(p, m, x.x));
-      x.y = left > 1 ? int32_t(verify_weight(p, m, x.y)) : 0;
-      x.z = left > 2 ? int32_t(verify_weight(p, m, x.z)) : 0;
-      x.w = left > 3 ? int32_t(verify_weight(p, m, x.w)) : 0;
-      w += left > 0 ? uint32_t(x.x) + uint32_t(x.y) + uint32_t(x.z) + uint32_t(x.w) : 0u;
-    } else {
-      x = make_int4(0, 0, 0, 0);
+  for (int p0 = 0; p0 * VERIFY_PIECE < n; ++p0) {
+    const uint32_t base = uint32_t(m) - uint32_t(sm.ref[r][p0][warp]);  // m >= ref
+    // distances that still carry weight; a piece too far away has none
+    const bool near = base <= uint32_t(p.reach);
+    const uint32_t left = uint32_t(p.reach) - base;
+#pragma unroll
+    for (int u = 0; u < VERIFY_U; ++u) {
+      const int j = p0 * VERIFY_PIECE + 4 * (u * VERIFY_THREADS + int(threadIdx.x));
+      uint2 x = make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
+      if (near && j < n) x = *reinterpret_cast<const uint2*>(s + j);
+      const uint32_t d[4] = {x.x & 0xFFFFu, x.x >> 16, x.y & 0xFFFFu, x.y >> 16};
+      const bool any = near && min(min(d[0], d[1]), min(d[2], d[3])) <= left;
+      uint32_t v[4] = {0, 0, 0, 0};
+      if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = verify_weight_at(p, base + d[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = j + e < n ? v[e] : 0u;
+      }
+      w += v[0] + v[1] + v[2] + v[3];
+      if (j < n) *reinterpret_cast<uint2*>(s + j) = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
     }
-    if (left > 0) reinterpret_cast<int4*>(s)[v] = x;
   }
   return w;
 }
 
-__global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_cluster_kernel(VerifyParams p, int cl) {
+__global__ void __launch_bounds__(VERIFY_THREADS, 4) verify_cluster_kernel(VerifyParams p, int cl) {
   verify_arrive();
   pdl_wait();
   pdl_launch();
-  extern __shared__ __align__(16) int32_t s_logit[];  // target slice [per], draft slice [per]
+  extern __shared__ __align__(16) uint16_t s_logit[];  // target slice [per], draft slice [per]
   __shared__ VerifyShared sm;
   const int rank = int(cluster_ctarank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int unit = int(blockIdx.x) / cl, b = unit / (p.D + 1), i = unit % (p.D + 1);
+  const int unit = int(blockIdx.x) / cl;
+  const int b = unit / (p.D + 1), i = unit % (p.D + 1);
+  const uint64_t word = p.rand[int64_t(b) * (p.D + 1) + i];
+  const int token = i < p.D ? p.tokens[int64_t(b) * p.D + i] : -1;
   const int cnt = verify_count(p, b);
   const int j0 = min(p.V, rank * p.per), n = min(p.per, p.V - j0);
   const bool need = i <= cnt;  // later positions are not reached
   const bool drafted = i < cnt, pair = drafted && p.draft;
-  int32_t *s_t = s_logit, *s_d = s_logit + p.per;
+  uint16_t *s_t = s_logit, *s_d = s_logit + p.per;
   const int32_t* trow = p.target + b * p.ts_b + i * p.ts_d;
   const int32_t* drow = pair ? p.draft + b * p.ds_b + i * p.ds_d : trow;
-  int x = -1;
-  uint64_t word = 0;
   if (need) {
-    if (drafted) x = p.tokens[int64_t(b) * p.D + i];
-    word = p.rand[int64_t(b) * (p.D + 1) + i];
     int32_t m[2] = {INT32_MIN, INT32_MIN};
-    if (pair) verify_load<2>({trow + j0, drow + j0}, n, {s_t, s_d}, m);
-    else verify_load<1>({trow + j0, trow + j0}, n, {s_t, s_d}, m);
-    m[0] = __reduce_max_sync(0xffffffffu, m[0]);
-    m[1] = __reduce_max_sync(0xffffffffu, m[1]);
+    if (pair) verify_load<2>({trow + j0, drow + j0}, n, {s_t, s_d}, sm, m);
+    else verify_load<1>({trow + j0, trow + j0}, n, {s_t, s_d}, sm, m);
     if (lane == 0) sm.wmax[0][warp] = m[0], sm.wmax[1][warp] = m[1];
   }
   __syncthreads();
   verify_wait();  // every CTA of the cluster runs: its shared memory may be written
   if (!need) return;
+  const int x = drafted ? token : -1;
   const bool inside = x >= 0 && x < p.V;
   const int32_t lt = inside ? trow[x] : 0, ld = inside ? drow[x] : 0;
   // warp 0 joins the warps' values; thread k < cl writes them into CTA k
@@ -223,6 +234,9 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_cluster_kernel(Verif
   cluster_sync_all();
   const int32_t mt = __reduce_max_sync(0xffffffffu, sm.mx[0][lane % cl]);
   const int32_t md = __reduce_max_sync(0xffffffffu, sm.mx[1][lane % cl]);
+  // the drafted token's weights, in flight during the sums
+  const uint64_t wx = inside ? verify_weight(p, mt, lt) : 0;
+  const uint64_t zx = inside ? (pair ? verify_weight(p, md, ld) : 1) : 0;
   auto join = [&](const unsigned long long* w) {  // warp 0: the sum of the warps' values
     unsigned long long v = lane < VERIFY_WARPS ? w[lane] : 0;
 #pragma unroll
@@ -230,8 +244,8 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_cluster_kernel(Verif
     return v;
   };
   {
-    const uint32_t a = __reduce_add_sync(0xffffffffu, verify_sum(p, s_t, n, mt));
-    const uint32_t c = pair ? __reduce_add_sync(0xffffffffu, verify_sum(p, s_d, n, md)) : 0;
+    const uint32_t a = __reduce_add_sync(0xffffffffu, verify_sum(p, s_t, n, 0, sm, mt));
+    const uint32_t c = pair ? __reduce_add_sync(0xffffffffu, verify_sum(p, s_d, n, 1, sm, md)) : 0;
     if (lane == 0) sm.wsum[0][warp] = a, sm.wsum[1][warp] = c;
   }
   __syncthreads();
@@ -250,13 +264,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_cluster_kernel(Verif
   }
   bool accept = false;
   if (drafted) {
-    uint64_t wx = 0, zx = 0;
-    if (inside) {
-      wx = verify_weight(p, mt, lt);
-      zx = pair ? verify_weight(p, md, ld) : 1;
-    } else if (rank == 0 && threadIdx.x == 0) {
-      atomicCAS(p.err, 0, DEV_BAD_TOKEN);
-    }
+    if (!inside && rank == 0 && threadIdx.x == 0) atomicCAS(p.err, 0, DEV_BAD_TOKEN);
     // u X < 2^32 Y iff floor(u X / 2^32) < Y
     accept = __umul64hi((word >> 32) << 32, zx * sw) < wx * sz;
   }
@@ -267,18 +275,18 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_cluster_kernel(Verif
     // the slice's vector v: target weights, or what the draft leaves of them
     auto left4 = [&](int v, unsigned long long (&r)[4]) -> unsigned long long {
       if (4 * v >= n) return r[0] = r[1] = r[2] = r[3] = 0;
-      const int4 w = reinterpret_cast<const int4*>(s_t)[v];
-      r[0] = uint32_t(w.x), r[1] = uint32_t(w.y), r[2] = uint32_t(w.z), r[3] = uint32_t(w.w);
+      const uint2 w = reinterpret_cast<const uint2*>(s_t)[v];
+      r[0] = w.x & 0xFFFFu, r[1] = w.x >> 16, r[2] = w.y & 0xFFFFu, r[3] = w.y >> 16;
       const unsigned long long any = r[0] | r[1] | r[2] | r[3];
       if (rest && any) {
-        int4 z = make_int4(0, 0, 0, 0);
+        uint2 z = make_uint2(0u, 0u);
         if (pair) {
-          z = reinterpret_cast<const int4*>(s_d)[v];
+          z = reinterpret_cast<const uint2*>(s_d)[v];
         } else if (unsigned(x - j0 - 4 * v) < 4u) {
           const int e = x - j0 - 4 * v;
-          z = make_int4(e == 0, e == 1, e == 2, e == 3);
+          z = make_uint2(e == 0 ? 1u : e == 1 ? 1u << 16 : 0u, e == 2 ? 1u : e == 3 ? 1u << 16 : 0u);
         }
-        const uint32_t q[4] = {uint32_t(z.x), uint32_t(z.y), uint32_t(z.z), uint32_t(z.w)};
+        const uint32_t q[4] = {z.x & 0xFFFFu, z.x >> 16, z.y & 0xFFFFu, z.y >> 16};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint64_t a = r[e] * sz, c = q[e] * sw;
@@ -370,7 +378,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_cluster_kernel(Verif
   }
 }
 
-// ---- vocabularies beyond a cluster's shared memory ----------------------------------------
+// ---- vocabularies beyond a cluster's shared memory, tables of a longer reach ----------------------------------------
 // Row statistics: one block per logit row, its maximum and weight sum.
 __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(VerifyParams p) {
   pdl_wait();

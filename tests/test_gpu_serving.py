@@ -460,6 +460,8 @@ def test_verify_extreme_logits_and_tables(ctx):
     p["draft"][2, 1, 5] = 2**31 - 1
     check_verify(ctx, p)
     check_verify(ctx, p, mult=2**32 - 1, shift=62)  # nearly flat
+    check_verify(ctx, p, mult=1, shift=2)           # a reach of 16 bits and a little less
+    check_verify(ctx, p, mult=(1 << 20) // 65534 + 1, shift=6)
     check_verify(ctx, p, mult=2**32 - 1, shift=0)   # the maximum alone
     check_verify(ctx, p, lut=np.array([1], np.int16))
     check_verify(ctx, p, lut=np.array([3, 32767, 0, 5], np.int16), mult=1, shift=5)
