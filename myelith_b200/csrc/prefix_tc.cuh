@@ -544,164 +544,171 @@ __global__ void __launch_bounds__(PTC_PV_THREADS, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
+// 16 int16 values as byte planes, words of four consecutive values.
+__device__ __forceinline__ void ptc_planes(const uint4& u, const uint4& v, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  hi[0] = __byte_perm(u.x, u.y, 0x7531), hi[1] = __byte_perm(u.z, u.w, 0x7531);
+  hi[2] = __byte_perm(v.x, v.y, 0x7531), hi[3] = __byte_perm(v.z, v.w, 0x7531);
+  lo[0] = __byte_perm(u.x, u.y, 0x6420), lo[1] = __byte_perm(u.z, u.w, 0x6420);
+  lo[2] = __byte_perm(v.x, v.y, 0x6420), lo[3] = __byte_perm(v.z, v.w, 0x6420);
+}
+
 // The suffixes' scores and row maxima: a block per (PTC_SFX_KEYS keys, KV head
-// and PFX_ROWS query rows, request). 8 threads a key (part s: the 8-element
-// chunks s, s + 8, ...); a thread ends up with one row's scores of its keys.
+// and PFX_ROWS query rows, request), a warp per 16 keys. A request's few rows fit
+// the 8 columns of an m16n8k32 MMA whose rows are keys: both operands come
+// straight from global memory as byte planes (a lane takes 16 consecutive values
+// of its key and of its query row for two k halves; the order inside a dot is
+// free). A tenth of the instructions of two-value dot products, which took 14 us
+// of a 64-request call.
+template <int HD>
 __global__ void __launch_bounds__(PFX_THREADS) prefix_suffix_kernel(PrefixParams p) {
   pdl_wait();
   pdl_launch();
-  constexpr int KEYS = PFX_THREADS / 8, ITER = PTC_SFX_KEYS / KEYS;
-  __shared__ __align__(16) int16_t s_q[PFX_ROWS * 128];
   __shared__ int32_t s_mx[PFX_THREADS / 32][PFX_ROWS];
-  const int b = int(blockIdx.z), g = int(blockIdx.y) % p.nkv, r0 = int(blockIdx.y) / p.nkv * PFX_ROWS;
-  const int n = pfx_len(p, b), nc8 = p.hd / 8, j0 = int(blockIdx.x) * PTC_SFX_KEYS;
+  const int b = int(blockIdx.z), h = int(blockIdx.y) % p.nkv, r0 = int(blockIdx.y) / p.nkv * PFX_ROWS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int n = pfx_len(p, b), j0 = int(blockIdx.x) * PTC_SFX_KEYS;
   if (j0 >= n) return;
-  const int jj = int(threadIdx.x) / 8, part = int(threadIdx.x) % 8;
-  const int16_t* kbase = p.ks + b * p.seq_stride + g * p.head_stride + 8 * part;
-  uint4 kv[ITER][2];
-#pragma unroll
-  for (int t = 0; t < ITER; ++t)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int j = j0 + t * KEYS + jj;
-      kv[t][i] = j < n && part + 8 * i < nc8 ? *reinterpret_cast<const uint4*>(kbase + j * p.pos_stride + 64 * i)
-                                             : make_uint4(0u, 0u, 0u, 0u);
-    }
   const int per = p.T * p.G, nrow = min(PFX_ROWS, per - r0), rho0 = b * per + r0;
-  for (int e = threadIdx.x; e < PFX_ROWS * nc8; e += PFX_THREADS) {
-    const int rho = rho0 + e / nc8;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (e / nc8 < nrow)
-      v = *reinterpret_cast<const uint4*>(p.q + int64_t(rho / p.G) * p.ldq + int64_t(g * p.G + rho % p.G) * p.hd + 8 * (e % nc8));
-    reinterpret_cast<uint4*>(s_q)[e] = v;
-  }
-  __syncthreads();
-  const int rho = rho0 + part;  // this thread's row after the reduce-scatter
-  const int seen = part < nrow ? pfx_seen(p, n, (rho / p.G) % p.T) : 0;
-  int32_t* dst = p.scores + (int64_t(g) * p.R + rho) * p.lds;
-  int32_t mx = INT32_MIN;
+  const int ja = j0 + 16 * warp + g, jb = ja + 8;
+  const int16_t* kbase = p.ks + b * p.seq_stride + h * p.head_stride + 16 * c;
+  const int rho = rho0 + min(g, nrow - 1);  // columns past the rows repeat the last
+  const int16_t* qrow = p.q + int64_t(rho / p.G) * p.ldq + int64_t(h * p.G + rho % p.G) * HD + 16 * c;
+  constexpr int KS = HD / 64;
+  uint4 ka[KS][2], kb[KS][2], q[KS][2];
 #pragma unroll
-  for (int t = 0; t < ITER; ++t) {
-    if (j0 + t * KEYS >= n) break;
-    int ah[PFX_ROWS], al[PFX_ROWS];
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
-    for (int r = 0; r < PFX_ROWS; ++r) ah[r] = al[r] = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 w = kv[t][i];
-      const uint32_t hx = __byte_perm(w.x, w.y, 0x7531), hy = __byte_perm(w.z, w.w, 0x7531);
-      const uint32_t lx = __byte_perm(w.x, w.y, 0x6420), ly = __byte_perm(w.z, w.w, 0x6420);
-      const int c = part + 8 * i;
-      if (c < nc8) {
-#pragma unroll
-        for (int r = 0; r < PFX_ROWS; ++r) {
-          const uint4 q = reinterpret_cast<const uint4*>(s_q)[r * nc8 + c];
-          ah[r] = dp2a_hi_ss(q.y, hx, dp2a_lo_ss(q.x, hx, ah[r]));
-          ah[r] = dp2a_hi_ss(q.w, hy, dp2a_lo_ss(q.z, hy, ah[r]));
-          al[r] = dp2a_hi_su(q.y, lx, dp2a_lo_su(q.x, lx, al[r]));
-          al[r] = dp2a_hi_su(q.w, ly, dp2a_lo_su(q.z, ly, al[r]));
-        }
-      }
+    for (int u = 0; u < 2; ++u) {
+      ka[s][u] = kb[s][u] = make_uint4(0u, 0u, 0u, 0u);
+      if (ja < n) ka[s][u] = *reinterpret_cast<const uint4*>(kbase + ja * p.pos_stride + 64 * s + 8 * u);
+      if (jb < n) kb[s][u] = *reinterpret_cast<const uint4*>(kbase + jb * p.pos_stride + 64 * s + 8 * u);
+      q[s][u] = *reinterpret_cast<const uint4*>(qrow + 64 * s + 8 * u);
     }
-    const int sh = att_reduce_scatter8(ah, part), sl = att_reduce_scatter8(al, part);
-    const int j = j0 + t * KEYS + jj;
-    if (j < seen) {
-      const int32_t sc = pfx_score(p, int64_t(sh) * 256 + int64_t(sl));
-      dst[j] = sc;
-      mx = max(mx, sc);
+  int hh[4] = {0, 0, 0, 0}, x[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    uint32_t ah[4], al[4], bh[4], bl[4], qh[4], ql[4];
+    ptc_planes(ka[s][0], ka[s][1], ah, al);
+    ptc_planes(kb[s][0], kb[s][1], bh, bl);
+    ptc_planes(q[s][0], q[s][1], qh, ql);
+#pragma unroll
+    for (int u = 0; u < 4; u += 2) {
+      mma_i8_16832<true, true>(hh, ah[u], bh[u], ah[u + 1], bh[u + 1], qh[u], qh[u + 1]);
+      mma_i8_16832<true, false>(x, ah[u], bh[u], ah[u + 1], bh[u + 1], ql[u], ql[u + 1]);
+      mma_i8_16832<false, true>(x, al[u], bl[u], al[u + 1], bl[u + 1], qh[u], qh[u + 1]);
+      mma_i8_16832<false, false>(ll, al[u], bl[u], al[u + 1], bl[u + 1], ql[u], ql[u + 1]);
+    }
+  }
+  int32_t mx[2] = {INT32_MIN, INT32_MIN};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {  // key ja (e 0, 1) or jb (2, 3), row 2 c + (e & 1)
+    const int r = 2 * c + (e & 1), j = e < 2 ? ja : jb;
+    if (r < nrow && j < pfx_seen(p, n, ((rho0 + r) / p.G) % p.T)) {
+      const int32_t sc = pfx_score(p, int64_t(hh[e]) * 65536 + int64_t(x[e]) * 256 + int64_t(ll[e]));
+      p.scores[(int64_t(h) * p.R + rho0 + r) * p.lds + j] = sc;
+      mx[e & 1] = max(mx[e & 1], sc);
     }
   }
 #pragma unroll
-  for (int o = 8; o < 32; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if ((threadIdx.x & 31) < 8) s_mx[threadIdx.x >> 5][part] = mx;
+  for (int u = 0; u < 2; ++u) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) mx[u] = max(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], o));
+    if (g == 0) s_mx[warp][2 * c + u] = mx[u];
+  }
   __syncthreads();
   if (int(threadIdx.x) < nrow) {
     int32_t m = s_mx[0][threadIdx.x];
 #pragma unroll
     for (int w = 1; w < PFX_THREADS / 32; ++w) m = max(m, s_mx[w][threadIdx.x]);
-    if (m != INT32_MIN) atomicMax(p.rowmax + int64_t(g) * p.R + rho0 + threadIdx.x, uint32_t(m) ^ 0x80000000u);
+    if (m != INT32_MIN) atomicMax(p.rowmax + int64_t(h) * p.R + rho0 + threadIdx.x, uint32_t(m) ^ 0x80000000u);
   }
 }
 
-// The suffixes' probability-weighted values: a block per (PTC_SFX_KEYS keys, KV
-// head and PFX_ROWS query rows, request), its value rows in registers (a thread
-// 8 dimensions of PTC_SFX_KEYS * hd / 2048 keys). The
-// int32 sums hold: the keys carry at most 2^15 + 64 of probability. They go to
-// sums [tile][row][hd].
+// The suffixes' probability-weighted values, blocks as above, on the same MMA:
+// rows are dimensions, columns the query rows, k the keys. A warp has 32 keys and
+// 64 dimensions; lane (g, c) loads dimensions 8 g.. of keys 8 c.. and turns each
+// four keys' words into plane words of one dimension with byte permutations; tile
+// t of the four MMA tiles has dimension 8 g + 2 t in row g and the next in row g
+// + 8. A block's sums fit int32 (its keys carry at most 2^15 + 64 of probability),
+// so the plane sums join in wrapping 32-bit arithmetic. They go to sums
+// [tile][row][hd].
 template <int HD>
-__global__ void __launch_bounds__(PFX_THREADS) prefix_suffix_values_kernel(PrefixParams p, int32_t* sums, int64_t rows) {
+__global__ void __launch_bounds__(2 * HD) prefix_suffix_values_kernel(PrefixParams p, int32_t* sums, int64_t rows) {
   pdl_launch();
-  constexpr int TPK = HD / 8, GROUPS = PFX_THREADS / TPK, PER = PTC_SFX_KEYS / GROUPS, WARPS = PFX_THREADS / 32;
-  __shared__ __align__(16) uint16_t s_p[PTC_SFX_KEYS][PFX_ROWS];
-  __shared__ __align__(16) int32_t s_part[WARPS][PFX_ROWS][HD];
-  const int b = int(blockIdx.z), g = int(blockIdx.y) % p.nkv, r0 = int(blockIdx.y) / p.nkv * PFX_ROWS, j0 = int(blockIdx.x) * PTC_SFX_KEYS;
-  const int n = pfx_len(p, b);
-  if (j0 >= n) return;
-  const int kg = int(threadIdx.x) / TPK, d8 = int(threadIdx.x) % TPK, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int16_t* vbase = p.vs + b * p.seq_stride + g * p.head_stride + 8 * d8;
-  uint4 v[PER];
+  constexpr int HALVES = HD / 64, KGROUPS = PTC_SFX_KEYS / 32, WARPS = HALVES * KGROUPS;
+  constexpr int LD = PTC_SFX_KEYS + 16;  // padded rows of the probability planes
+  __shared__ __align__(16) uint8_t s_ph[PFX_ROWS][LD], s_pl[PFX_ROWS][LD];
+  __shared__ int32_t s_part[KGROUPS][PFX_ROWS][HD];
+  const int b = int(blockIdx.z), h = int(blockIdx.y) % p.nkv, r0 = int(blockIdx.y) / p.nkv * PFX_ROWS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int n = pfx_len(p, b), j0 = int(blockIdx.x) * PTC_SFX_KEYS;
+  if (j0 >= n) {
+    pdl_wait();  // the grid ends after the kernel before it even if no request has a suffix
+    return;
+  }
+  const int kgroup = warp / HALVES, d0 = 64 * (warp % HALVES);
+  const int16_t* vbase = p.vs + b * p.seq_stride + h * p.head_stride + d0 + 8 * g;
+  uint4 v[8];
 #pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    const int j = j0 + kg + u * GROUPS;
+  for (int u = 0; u < 8; ++u) {
+    const int j = j0 + 32 * kgroup + 8 * c + u;
     v[u] = j < n ? *reinterpret_cast<const uint4*>(vbase + j * p.pos_stride) : make_uint4(0u, 0u, 0u, 0u);
   }
   pdl_wait();  // the row sums (never a call's first kernel: the inputs are in place)
   const int32_t one = int32_t(1) << p.prob_frac;
-  const int per = p.T * p.G;
-  const int nrow = min(PFX_ROWS, per - r0), rho0 = b * per + r0;
-  const int64_t row0 = int64_t(g) * p.R + rho0;
-  {  // probabilities: a warp's 32 lanes take 4 keys of each of the 8 rows
-    const int r = lane % PFX_ROWS;
+  const int per = p.T * p.G, nrow = min(PFX_ROWS, per - r0), rho0 = b * per + r0;
+  const int64_t row0 = int64_t(h) * p.R + rho0;
+  {  // probabilities: a thread has one row and every (2 HD / PFX_ROWS)th key
+    const int r = int(threadIdx.x) % PFX_ROWS;
     const bool live = r < nrow;
     const int seen = live ? pfx_seen(p, n, ((rho0 + r) / p.G) % p.T) - j0 : 0;
     const int32_t S = live ? p.rowsum[row0 + r] : 1;
     const int32_t top = live ? int32_t(p.rowmax[row0 + r] ^ 0x80000000u) : 0;
     const uint64_t recip = softmax_recip(S);
     const int32_t* sc = p.scores + (row0 + r) * p.lds + j0;
+    constexpr int STEP = 32 * WARPS / PFX_ROWS;
 #pragma unroll
-    for (int u = 0; u < PTC_SFX_KEYS * PFX_ROWS / PFX_THREADS; ++u) {
-      const int jj = (u * WARPS + warp) * (32 / PFX_ROWS) + lane / PFX_ROWS;
-      const int32_t ex = jj < seen ? pfx_exp(p, top, sc[jj]) : 0;
-      s_p[jj][r] = uint16_t(softmax_prob_r(ex, S, recip, 0, 1, one));
+    for (int u = 0; u < PTC_SFX_KEYS / STEP; ++u) {
+      const int jj = int(threadIdx.x) / PFX_ROWS + u * STEP;
+      const uint32_t pr = jj < seen ? uint32_t(softmax_prob_r(pfx_exp(p, top, sc[jj]), S, recip, 0, 1, one)) : 0u;
+      s_ph[r][jj] = uint8_t(pr >> 8);
+      s_pl[r][jj] = uint8_t(pr);
     }
   }
   __syncthreads();
-  int32_t acc[PFX_ROWS][8];
+  const uint2 ph = *reinterpret_cast<const uint2*>(&s_ph[g][32 * kgroup + 8 * c]);
+  const uint2 pl = *reinterpret_cast<const uint2*>(&s_pl[g][32 * kgroup + 8 * c]);
 #pragma unroll
-  for (int r = 0; r < PFX_ROWS; ++r)
+  for (int t = 0; t < 4; ++t) {
+    uint32_t even_h[2], even_l[2], odd_h[2], odd_l[2];  // plane words of keys 8 c + 4 s..
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[r][e] = 0;
+    for (int s = 0; s < 2; ++s) {
+      uint32_t w[4];
 #pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    const uint4 pw = *reinterpret_cast<const uint4*>(&s_p[kg + u * GROUPS][0]);
-    const uint32_t pr[4] = {pw.x, pw.y, pw.z, pw.w};
-    int32_t ve[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ve[e] = lane16(v[u], e);
-#pragma unroll
-    for (int r = 0; r < PFX_ROWS; ++r) {
-      const int32_t pj = int32_t((r & 1) ? pr[r / 2] >> 16 : pr[r / 2] & 0xFFFFu);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[r][e] += pj * ve[e];
+      for (int u = 0; u < 4; ++u) {
+        const uint4 y = v[4 * s + u];
+        w[u] = t == 0 ? y.x : t == 1 ? y.y : t == 2 ? y.z : y.w;
+      }
+      const uint32_t e01 = __byte_perm(w[0], w[1], 0x5140), e23 = __byte_perm(w[2], w[3], 0x5140);
+      const uint32_t o01 = __byte_perm(w[0], w[1], 0x7362), o23 = __byte_perm(w[2], w[3], 0x7362);
+      even_l[s] = __byte_perm(e01, e23, 0x5410), even_h[s] = __byte_perm(e01, e23, 0x7632);
+      odd_l[s] = __byte_perm(o01, o23, 0x5410), odd_h[s] = __byte_perm(o01, o23, 0x7632);
     }
-  }
-  // the warp's key groups (32 / TPK of them), then the warps'
+    int hh[4] = {0, 0, 0, 0}, x1[4] = {0, 0, 0, 0}, x2[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
+    mma_i8_16832<true, false>(hh, even_h[0], odd_h[0], even_h[1], odd_h[1], ph.x, ph.y);
+    mma_i8_16832<true, false>(x1, even_h[0], odd_h[0], even_h[1], odd_h[1], pl.x, pl.y);
+    mma_i8_16832<false, false>(x2, even_l[0], odd_l[0], even_l[1], odd_l[1], ph.x, ph.y);
+    mma_i8_16832<false, false>(ll, even_l[0], odd_l[0], even_l[1], odd_l[1], pl.x, pl.y);
 #pragma unroll
-  for (int r = 0; r < PFX_ROWS; ++r) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-      for (int o = TPK; o < 32; o <<= 1) acc[r][e] += __shfl_xor_sync(0xffffffffu, acc[r][e], o);
-    if (lane < TPK) {
-      *reinterpret_cast<int4*>(&s_part[warp][r][8 * d8]) = make_int4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-      *reinterpret_cast<int4*>(&s_part[warp][r][8 * d8 + 4]) = make_int4(acc[r][4], acc[r][5], acc[r][6], acc[r][7]);
-    }
+    for (int e = 0; e < 4; ++e)
+      s_part[kgroup][2 * c + (e & 1)][d0 + 8 * g + 2 * t + (e >> 1)] =
+          int32_t(uint32_t(hh[e]) * 65536u + uint32_t(x1[e] + x2[e]) * 256u + uint32_t(ll[e]));
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < nrow * HD; e += PFX_THREADS) {
+  for (int e = threadIdx.x; e < nrow * HD; e += 32 * WARPS) {
     int32_t t = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) t += s_part[w][e / HD][e % HD];
+    for (int w = 0; w < KGROUPS; ++w) t += s_part[w][e / HD][e % HD];
     sums[(int64_t(blockIdx.x) * rows + row0 + e / HD) * HD + e % HD] = t;
   }
 }

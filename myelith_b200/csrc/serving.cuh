@@ -190,7 +190,7 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaSt
   const dim3 suffix(unsigned(tiles), unsigned(p.nkv * ((p.T * p.G + PFX_ROWS - 1) / PFX_ROWS)), unsigned(p.B));
   if (p.S > 0) {
     LaunchCfg l0(ctx, suffix, dim3(PFX_THREADS), 0, st);
-    CUDA_TRY(cudaLaunchKernelEx(&l0.cfg, prefix_suffix_kernel, p));
+    CUDA_TRY(cudaLaunchKernelEx(&l0.cfg, prefix_suffix_kernel<HD>, p));
     qk.early = 1;
   }
   LaunchCfg l1(ctx, dim3(unsigned(splits), unsigned(units)), dim3(PTC_QK_THREADS), Cfg::QK_SMEM, st);
@@ -198,7 +198,7 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaSt
   qk.early = 1;
   CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 1>, p, qk));
   if (p.S > 0) {
-    LaunchCfg l(ctx, suffix, dim3(PFX_THREADS), 0, st);
+    LaunchCfg l(ctx, suffix, dim3(2 * HD), 0, st);
     CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_suffix_values_kernel<HD>, p, sums, rows));
   }
   LaunchCfg l2(ctx, dim3(unsigned(splits), unsigned(units)), dim3(PTC_PV_THREADS), Cfg::PV_SMEM, st);
