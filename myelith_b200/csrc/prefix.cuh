@@ -17,7 +17,7 @@
 // The prefix is laid out once, when it is registered, as unsigned byte planes
 // (x + 32768 = 256 hi + lo) in the order in which the tensor cores read them from
 // shared memory, so that one bulk copy brings a block of positions: keys as
-// [kv head][32 positions][hi 32 rows, lo 32 rows][hd], values transposed as
+// [kv head][64 positions][hi 64 rows, lo 64 rows][hd], values transposed as
 // [kv head][128 positions][hi hd rows, lo hd rows][128], the 16-byte pieces of a
 // row swapped by the 128-byte (64-byte for key rows of 64) swizzle; positions
 // padded with zeros to a multiple of PFX_PAD. Rows of a KV head g are numbered
@@ -97,9 +97,9 @@ __host__ __device__ __forceinline__ int pfx_piece(int hd, int row, int c16) {
 }
 // Offset of bytes d.. (inside one piece) of plane `lo` of position j of head g.
 __device__ __forceinline__ int64_t pfx_key_at(int64_t Pp, int hd, int64_t g, int64_t j, int lo, int d) {
-  const int row = 32 * lo + int(j & 31);
+  const int row = 64 * lo + int(j & 63);
   const int at = hd % 16 ? row * hd + d : pfx_piece(hd, row, d >> 4) + (d & 15);
-  return (g * (Pp / 32) + (j >> 5)) * 64 * hd + at;
+  return (g * (Pp / 64) + (j >> 6)) * 128 * hd + at;
 }
 // Offset of positions j.. (inside one piece) of plane `lo` of dimension d of head g.
 __device__ __forceinline__ int64_t pfx_value_at(int64_t Pp, int hd, int64_t g, int64_t j, int lo, int d) {

@@ -3,27 +3,34 @@
 //
 // A tile is 128 query rows of one KV head (TMEM lane = row). Operands are
 // bytes: q = 256 qh + ql (qh signed), k + 32768 = 256 kh + kl (both unsigned,
-// as the prefix stores them), so for 32 keys one kind::i8 MMA of qh and one of
-// ql against the 64 stacked byte rows [kh | kl] give hh, hl, lh, ll and
+// as the prefix stores them), so for 64 keys one kind::i8 MMA of qh and one of
+// ql against the 128 stacked byte rows [kh | kl] give hh, hl, lh, ll and
 //   dot = 256 (256 hh + hl + lh) + ll - 32768 sum(q)
-// with every int32 sum exact (|hh| <= 128 * 128 * 255 at hd = 128). In the same
+// with every int32 sum exact (each below 128 * 255 * 255 at hd = 128). In the same
 // way p = 256 ph + pl and v + 32768 = 256 vh + vl give the weighted values. A
 // row's probabilities sum to less than 2^17, so the value sums stay inside
 // int32 over a whole row and TMEM accumulates them without a flush.
 //
-// The score needs no integer rounding: the 64-bit pattern of the double
-// 1.5 * 2^52 is added to dot with two wide multiply-adds, which makes the bits
-// the double X = 1.5 * 2^52 + dot (|dot| < 2^38), and
+// Scores, in either of two forms that the plan's constants decide. If M = mult *
+// 2^(32 - shift) is an integer below 2^23, two wide multiply-adds make
+//   Y = dot * M + 2^31
+// whose high word is the score, rounded half up; a low word of zero marks a tie,
+// whose odd score loses one. As |dot * M| < 2^60 such a score does not wrap around
+// i32, so a row's largest dot has its largest score. Otherwise, for 0 <=
+// mult <= 2^shift and shift <= 51, the multiply-adds put dot below the bits of the
+// double X = 1.5 * 2^52 + dot (|dot| < 2^38), and
 //   fma(X, mult * 2^-shift, 1.5 * 2^52 * (1 - mult * 2^-shift))
 // is dot * mult * 2^-shift + 1.5 * 2^52 rounded once, to an integer with ties to
-// even: its low word is the score as i32, wrap-around included. The constant is
-// an exact integer for 0 <= mult <= 2^shift, shift <= 51.
+// even, its low word the score; the constant is an exact integer. Double
+// multiply-adds hold up the tensor cores: 448 rows per head x 32749 positions take
+// 40 us and 60 us (maxima, exponentials) in the first form, 44 and 77 in the
+// second.
 //
 // The maximum of a row must be known before the first exponential, and the sum
 // before the first probability, so the keys pass three times:
 //   prefix_suffix_kernel     suffix scores and maxima
-//   prefix_qk_kernel<HD, 0>  scores -> row maxima
-//   prefix_qk_kernel<HD, 1>  scores again -> exponentials (16 bits) and row sums
+//   prefix_qk_kernel<.., 0>  scores -> row maxima
+//   prefix_qk_kernel<.., 1>  scores again -> exponentials (16 bits) and row sums
 //                            (the suffix's included)
 //   prefix_suffix_values_kernel  the suffix's weighted values
 //   prefix_pv_kernel<HD>     exponentials -> probabilities -> weighted values
@@ -37,10 +44,11 @@
 namespace myl {
 
 constexpr int PTC_ROWS = 128;
-constexpr int PTC_KEYS = 32;        // keys per scores step
+constexpr int PTC_KEYS = 64;        // keys per scores step
 constexpr int PTC_BLOCK = 128;      // keys per bulk copy
-constexpr int PTC_BUFS = 3;         // TMEM score buffers
-constexpr int PTC_QK_WARPS = 4 * PTC_BUFS;  // worker warps: buffer x TMEM lane quarter
+constexpr int PTC_BUFS = 2;         // TMEM score buffers
+constexpr int PTC_COLS = 3 * PTC_KEYS;  // TMEM columns of one: hh | hl + lh | ll
+constexpr int PTC_QK_WARPS = 8 * PTC_BUFS;  // worker warps: buffer x half of a step's keys x TMEM lane quarter
 constexpr int PTC_PV_WARPS = 16;    // TMEM lane quarter x column quarter
 constexpr int PTC_QK_THREADS = 64 + 32 * PTC_QK_WARPS;
 constexpr int PTC_PV_THREADS = 64 + 32 * PTC_PV_WARPS;
@@ -52,8 +60,11 @@ struct PrefixTc {
   int RT;      // row tiles per KV head
   int blocks;  // 128-key blocks of the prefix
   int per;     // of these per thread block
-  double scale, offset;  // of a score, see above
-  int k256, k1;          // 256 and 1, kept from being folded: one multiply-add beats shifts and carries
+  double scale, offset;  // of a score, see above (second form)
+  // factors of 256 hh + hl + lh and of ll: 256 M and M, or 256 and 1 (kept from
+  // being folded: one wide multiply-add beats shifts and carries)
+  int k_mid, k_low;
+  int k256;
   int early;   // the scores kernel does not have to wait before its set-up
   int cap;     // largest table index looked up
   int lut_n;   // entries copied to shared memory (the one at cap included)
@@ -154,19 +165,25 @@ __device__ __forceinline__ void ptc_drain(PrefixCtl& ctl, int issued, int stages
   }
 }
 
+// The score of the first form: half up, a tie's odd result one less.
+__device__ __forceinline__ int32_t ptc_wide_score(int64_t y) {
+  const int32_t s = int32_t(y >> 32);
+  return uint32_t(y) == 0 ? s & ~1 : s;
+}
+
 // MODE 0: row maxima; MODE 1: exponentials and row sums. grid.x: key range,
 // grid.y: unit (kv head * RT + row tile). The query planes lie in TMEM, so an MMA
-// reads only its 64 key byte rows from shared memory (operand bytes from shared
-// memory, about 70 a clock here, set the pace of small MMAs: with the queries
-// there too, steps of 64 keys took 930 clocks instead of the 512 of the pipe).
-// Warp 0 copies key planes in blocks of 128 positions (tiled copies of 32 or 64
-// rows cost about 400 clocks each whatever their size, one bulk copy of a block
-// no more than that), warp 1 issues the MMAs into three score
-// buffers [hh | hl | lh | ll] of 32 columns each, and each buffer has four warps
-// that turn its scores into their output, so that three steps are worked on at
-// a time: warp (buffer, q) has rows 32 q.. of every third step, a thread one
-// row. In MODE 1 the blocks of a unit also share out its rows' suffix sums.
-template <int HD, int MODE>
+// reads only key byte rows from shared memory. Warp 0 copies key planes in blocks
+// of 128 positions, warp 1 issues the MMAs of 64 keys at a time into two score
+// buffers [hh | hl + lh | ll]: the products with qh end where those with ql
+// begin, so that TMEM adds the middle planes. Each buffer has eight warps that
+// turn its scores into their output: TMEM lane quarter x half of the keys, a
+// thread one row. One elected lane of the converged warp issues (from a divergent
+// lane each MMA costs about 100 clocks). 448 rows per head x 32749 positions of 4
+// heads: 40 us without, 60 us with the exponentials; the MMAs alone take 28, the
+// rest is the wide multiply-adds and the table look-ups between them. In MODE 1
+// the blocks of a unit also share out its rows' suffix sums.
+template <int HD, int MODE, bool WIDE>
 __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
     prefix_qk_kernel(PrefixParams p, PrefixTc tc) {
   // early: the kernel before this one belongs to the same call, so everything
@@ -186,11 +203,11 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
   const int i0 = int(blockIdx.x) * tc.per, n = min(tc.per, tc.blocks - i0);  // 128-key blocks
   constexpr int SUB = PTC_BLOCK / PTC_KEYS;                                  // steps each
 
-  ptc_setup(ctl, ST, 1, 4);
+  ptc_setup(ctl, ST, 1, 8);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl.tmem_base, a_hi = tmem + PTC_BUFS * 128, a_lo = a_hi + HD / 4;
+  const uint32_t tmem = ctl.tmem_base, a_hi = tmem + PTC_BUFS * PTC_COLS, a_lo = a_hi + HD / 4;
   // query planes and sums, a thread of the first worker group a row; rows past R are zero
   if (warp >= 2 && warp < 6) {
     const int r = 32 * (warp & 3) + lane, rho = row0 + r;
@@ -239,7 +256,8 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
     // The whole warp walks the steps and one elected lane issues: operands that
     // the compiler can see are warp-uniform need no move into uniform registers
     // before every MMA.
-    constexpr uint32_t id_h = idesc_i8(128, 2 * PTC_KEYS, true, false), id_l = idesc_i8(128, 2 * PTC_KEYS, false, false);
+    constexpr uint32_t id_h = idesc_i8(128, 2 * PTC_KEYS, true, false), id_l = idesc_i8(128, 2 * PTC_KEYS, false, false),
+                       id_half = idesc_i8(128, PTC_KEYS, true, false);
     int i = 0, b = 0;  // step, its buffer
     uint32_t use = 0;  // parity of the buffers' use
     for (; i < n * SUB; ++i) {
@@ -250,13 +268,18 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
         break;
       }
       tc_fence_after();
-      const uint32_t d = tmem + uint32_t(b * 128);
+      const uint32_t d = tmem + uint32_t(b * PTC_COLS);
       const uint64_t db = ptc_desc<HD>(ring + uint32_t(s * Cfg::K_STAGE + i % SUB * (Cfg::K_STAGE / SUB)));
       if (elect_lane()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 32; ++kk) {
-          mma_i8_ts(d, a_hi + 8 * kk, db + 2 * kk, id_h, kk > 0);
-          mma_i8_ts(d + 64, a_lo + 8 * kk, db + 2 * kk, id_l, kk > 0);
+          mma_i8_ts(d + PTC_KEYS, a_lo + 8 * kk, db + 2 * kk, id_l, kk > 0);
+          if (kk > 0) {
+            mma_i8_ts(d, a_hi + 8 * kk, db + 2 * kk, id_h, true);
+          } else {  // hh starts, the middle sum goes on
+            mma_i8_ts(d, a_hi, db, id_half, false);
+            mma_i8_ts(d + PTC_KEYS, a_hi, db + PTC_KEYS * HD / 16, id_half, true);
+          }
         }
         if (i % SUB == SUB - 1) mma_commit(smem_addr(&ctl.empty[s]));
         mma_commit(smem_addr(&ctl.tfull[b]));
@@ -268,14 +291,15 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
     if (i > 0 && !mbar_wait_bounded(smem_addr(&ctl.tfull[(i - 1) % PTC_BUFS]), uint32_t((i - 1) / PTC_BUFS) & 1u, tc.timeout_ns, nullptr))
       atomicCAS(p.err, 0, DEV_WAIT_DRAIN);
   } else {
-    const int q = warp & 3, b = (warp - 2) >> 2;
+    const int q = warp & 3, b = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1;
     const int r = 32 * q + lane, rho = row0 + r;
     const bool live = rho < p.R, warp_live = row0 + 32 * q < p.R;
     const int64_t row = int64_t(g) * p.R + rho;
-    // the pattern of 1.5 * 2^52, less the unsigned key bytes' share of the dot
-    const int64_t pattern = 0x4338000000000000ll - int64_t(ctl.rowval[r]) * 32768;
+    // 2^31 or the pattern of 1.5 * 2^52, less the unsigned key bytes' share of the dot
+    const int64_t start = (WIDE ? int64_t(1) << 31 : 0x4338000000000000ll) - int64_t(ctl.rowval[r]) * 32768 * tc.k_low;
     pdl_wait();
     int32_t mx = INT32_MIN, sum = 0;
+    int64_t mxd = INT64_MIN;  // largest dot + 32768 sum(q)
     if (MODE == 1 && live) mx = int32_t(p.rowmax[row] ^ 0x80000000u);
     uint32_t use = 0;
     for (int i = b; i < n * SUB; i += PTC_BUFS, use ^= 1u) {
@@ -285,16 +309,15 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
       }
       if (*abort) break;
       tc_fence_after();
-      const int kb = i0 * SUB + i;
-      const uint32_t t0 = tmem + (uint32_t(32 * q) << 16) + uint32_t(b * 128);
+      const int group0 = (i0 * SUB + i) * (PTC_KEYS / 16) + 2 * half;  // of 16 keys
+      const uint32_t t0 = tmem + (uint32_t(32 * q) << 16) + uint32_t(b * PTC_COLS + 32 * half);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t hh[16], hl[16], lh[16], ll[16];
+        uint32_t hh[16], mid[16], ll[16];
         if (warp_live) {
           tmem_ld_32x32b_x16(t0 + 16 * h, hh);
-          tmem_ld_32x32b_x16(t0 + 16 * h + 32, hl);
-          tmem_ld_32x32b_x16(t0 + 16 * h + 64, lh);
-          tmem_ld_32x32b_x16(t0 + 16 * h + 96, ll);
+          tmem_ld_32x32b_x16(t0 + 16 * h + PTC_KEYS, mid);
+          tmem_ld_32x32b_x16(t0 + 16 * h + 2 * PTC_KEYS, ll);
           tmem_ld_wait();
         }
         if (h == 1) {
@@ -303,42 +326,57 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
           if (lane == 0) mbar_arrive(smem_addr(&ctl.tempty[b]));
         }
         if (!warp_live) continue;
-        const int left = p.P - kb * PTC_KEYS - 16 * h;  // keys of this group inside the prefix
-        int32_t sc[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int32_t t = int32_t(hh[j]) * tc.k256 + (int32_t(hl[j]) + int32_t(lh[j]));
-          const double x = __longlong_as_double(mad_wide(t, tc.k256, mad_wide(int32_t(ll[j]), tc.k1, pattern)));
-          sc[j] = __double2loint(fma(x, tc.scale, tc.offset));
-        }
-        if (MODE == 0) {
-          if (left < 16) {
+        for (int e = 0; e < 16; e += 8) {  // eight at a time stay in registers
+          const int left = p.P - 16 * (group0 + h) - e;  // keys of these inside the prefix
+          if constexpr (MODE == 0 && WIDE) {
+            int64_t d[8];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sc[j] = j < left ? sc[j] : INT32_MIN;
+            for (int j = 0; j < 8; ++j) d[j] = mad_wide(int32_t((hh[e + j] << 8) + mid[e + j]), tc.k256, int64_t(ll[e + j]));
+            if (left < 8) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) d[j] = j < left ? d[j] : INT64_MIN;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mxd = max(mxd, d[j]);
+          } else {
+            int32_t sc[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int32_t t = int32_t((hh[e + j] << 8) + mid[e + j]);
+              const int64_t y = mad_wide(t, tc.k_mid, mad_wide(int32_t(ll[e + j]), tc.k_low, start));
+              sc[j] = WIDE ? ptc_wide_score(y) : __double2loint(fma(__longlong_as_double(y), tc.scale, tc.offset));
+            }
+            if constexpr (MODE == 0) {
+              if (left < 8) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sc[j] = j < left ? sc[j] : INT32_MIN;
+              }
+#pragma unroll
+              for (int j = 0; j < 8; j += 2) mx = max(max(sc[j], sc[j + 1]), mx);
+            } else {
+              uint32_t ex[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                ex[j] = s_lut[min((uint32_t(mx) - uint32_t(sc[j])) >> p.lut_shift, uint32_t(tc.cap))];
+              if (left < 8) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ex[j] = j < left ? ex[j] : 0u;
+              }
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                sum += int32_t(ex[2 * j] + ex[2 * j + 1]);
+                w[j] = ex[2 * j] | (ex[2 * j + 1] << 16);
+              }
+              tc.e[((int64_t(unit) * tc.blocks * (PTC_BLOCK / 16) + group0 + h) * PTC_ROWS + r) * 2 + e / 8] =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
-#pragma unroll
-          for (int j = 0; j < 16; j += 2) mx = max(max(sc[j], sc[j + 1]), mx);
-        } else {
-          uint32_t ex[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            ex[j] = s_lut[min((uint32_t(mx) - uint32_t(sc[j])) >> p.lut_shift, uint32_t(tc.cap))];
-          if (left < 16) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) ex[j] = j < left ? ex[j] : 0u;
-          }
-          uint32_t w[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            sum += int32_t(ex[2 * j] + ex[2 * j + 1]);
-            w[j] = ex[2 * j] | (ex[2 * j + 1] << 16);
-          }
-          uint4* dst = tc.e + (((int64_t(unit) * tc.blocks * SUB + kb) * 2 + h) * PTC_ROWS + r) * 2;
-          dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-          dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
       }
     }
+    if (MODE == 0 && WIDE && mxd != INT64_MIN) mx = ptc_wide_score(mxd * tc.k_low + start);
     if (live) {
       if (MODE == 0) atomicMax(p.rowmax + row, uint32_t(mx) ^ 0x80000000u);
       else atomicAdd(p.rowsum + row, sum);
@@ -370,7 +408,10 @@ __global__ void __launch_bounds__(PTC_QK_THREADS, 1)
 // from one float multiply-add, exact unless the quotient lies within its error
 // of a half; w = 2 e one - 2 S p + S - 1 lies in [0, 2 S - 2] exactly when p is
 // the nearest integer and no tie, and anything else is redone in integers. The
-// byte planes of p go to shared memory as the MMA's A operand.
+// byte planes of p go to shared memory as the MMA's A operand. 448 rows per head x
+// 32749 positions of 4 heads: 42 us; the MMAs alone would take about 14, reading
+// the 117 MB of exponentials 15: the probabilities' instructions (about 14 a
+// value in 16 warps) are what is left.
 template <int HD>
 __global__ void __launch_bounds__(PTC_PV_THREADS, 1)
     prefix_pv_kernel(PrefixParams p, PrefixTc tc) {
@@ -557,8 +598,8 @@ __device__ __forceinline__ void ptc_planes(const uint4& u, const uint4& v, uint3
 // the 8 columns of an m16n8k32 MMA whose rows are keys: both operands come
 // straight from global memory as byte planes (a lane takes 16 consecutive values
 // of its key and of its query row for two k halves; the order inside a dot is
-// free). A tenth of the instructions of two-value dot products, which took 14 us
-// of a 64-request call.
+// free). 64 requests x 512 positions (34 MB of keys): 7.6 us with the launch; two
+// products at a time on the integer units took 14.
 template <int HD>
 __global__ void __launch_bounds__(PFX_THREADS) prefix_suffix_kernel(PrefixParams p) {
   pdl_wait();
@@ -631,7 +672,8 @@ __global__ void __launch_bounds__(PFX_THREADS) prefix_suffix_kernel(PrefixParams
 // t of the four MMA tiles has dimension 8 g + 2 t in row g and the next in row g
 // + 8. A block's sums fit int32 (its keys carry at most 2^15 + 64 of probability),
 // so the plane sums join in wrapping 32-bit arithmetic. They go to sums
-// [tile][row][hd].
+// [tile][row][hd]. 64 requests x 512 positions: 15 us, of which reading the values
+// once more is 5; two products at a time took 20.
 template <int HD>
 __global__ void __launch_bounds__(2 * HD) prefix_suffix_values_kernel(PrefixParams p, int32_t* sums, int64_t rows) {
   pdl_launch();

@@ -15,6 +15,7 @@ struct myl_attn_plan {
   int64_t score_mult = 0;
   int score_shift = 0, lut_shift = 0, prob_frac = 0, out_shift = 0;
   int cap = 0, lut_n = 0;  // see PrefixTc
+  int wide = -1;  // M of the integer score form, -1: the double form (prefix_tc.cuh)
   double scale = 0, offset = 0;
   bool tc = false;  // the constants fit the tensor-core kernels
   std::vector<void*> allocs;
@@ -105,10 +106,12 @@ int attn_plan_build(myl_attn_plan* pl, int64_t score_mult, uint8_t score_shift, 
   const int64_t top = INT32_MAX >> lut_shift;
   pl->cap = int(std::min(n, top));
   pl->lut_n = pl->cap + 1;
-  // the tensor-core path's score is one double multiply-add, see prefix_tc.cuh
+  // the tensor-core path's two forms of a score, see prefix_tc.cuh
   pl->tc = score_shift <= 51 && score_mult >= 0 && score_mult < (1 << 25) && score_mult <= int64_t(1) << score_shift &&
            pl->lut_n <= PTC_LUT_MAX;
   pl->scale = std::ldexp(double(score_mult), -int(score_shift));
+  const double m32 = std::ldexp(pl->scale, 32);
+  pl->wide = m32 >= 0 && m32 < (1 << 23) && m32 == std::floor(m32) ? int32_t(m32) : -1;
   pl->offset = std::ldexp(1.5, 52) - std::ldexp(1.5 * double(score_mult), 52 - int(score_shift));
   return dev_upload(pl->allocs, &pl->d_lut, exp_lut, size_t(exp_len));
 }
@@ -149,7 +152,7 @@ int prefix_split(int units, int steps, int sms, int fixed) {
   return best;
 }
 
-template <int HD>
+template <int HD, bool WIDE>
 int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaStream_t st) {
   const int64_t rows = int64_t(p.nkv) * p.R;
   const int RT = (p.R + PTC_ROWS - 1) / PTC_ROWS, units = p.nkv * RT, n = sms(ctx);
@@ -160,7 +163,8 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaSt
   qk.scale = pl->scale;
   qk.offset = pl->offset;
   qk.k256 = 256;
-  qk.k1 = 1;
+  qk.k_low = WIDE ? pl->wide : 1;
+  qk.k_mid = 256 * qk.k_low;
   qk.timeout_ns = pv.timeout_ns = ctx->timeout_ns;
   qk.blocks = pv.blocks = p.Pp / PTC_BLOCK;
   qk.per = pv.per = prefix_split(units, qk.blocks, n, 3);
@@ -180,8 +184,8 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaSt
   qk.e = pv.e = reinterpret_cast<uint4*>(ws + o_e);
   pv.part = reinterpret_cast<int64_t*>(ws + o_part);
   using Cfg = PtcCfg<HD>;
-  const void *f0 = reinterpret_cast<const void*>(&prefix_qk_kernel<HD, 0>),
-             *f1 = reinterpret_cast<const void*>(&prefix_qk_kernel<HD, 1>),
+  const void *f0 = reinterpret_cast<const void*>(&prefix_qk_kernel<HD, 0, WIDE>),
+             *f1 = reinterpret_cast<const void*>(&prefix_qk_kernel<HD, 1, WIDE>),
              *f2 = reinterpret_cast<const void*>(&prefix_pv_kernel<HD>);
   TRY(kernel_smem_occupancy(ctx->device, f0, PTC_QK_THREADS, Cfg::QK_SMEM, nullptr));
   TRY(kernel_smem_occupancy(ctx->device, f1, PTC_QK_THREADS, Cfg::QK_SMEM, nullptr));
@@ -194,9 +198,9 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaSt
     qk.early = 1;
   }
   LaunchCfg l1(ctx, dim3(unsigned(splits), unsigned(units)), dim3(PTC_QK_THREADS), Cfg::QK_SMEM, st);
-  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 0>, p, qk));
+  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 0, WIDE>, p, qk));
   qk.early = 1;
-  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 1>, p, qk));
+  CUDA_TRY(cudaLaunchKernelEx(&l1.cfg, prefix_qk_kernel<HD, 1, WIDE>, p, qk));
   if (p.S > 0) {
     LaunchCfg l(ctx, suffix, dim3(2 * HD), 0, st);
     CUDA_TRY(cudaLaunchKernelEx(&l.cfg, prefix_suffix_values_kernel<HD>, p, sums, rows));
@@ -217,7 +221,8 @@ int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p,
   const unsigned gy = unsigned(p.nkv * ((p.R + PFX_ROWS - 1) / PFX_ROWS));
   if (gy > 65535u) return fail(MYL_ERR_UNSUPPORTED, "%d query rows per KV head", p.R);
   if (pl->tc && (p.hd == 64 || p.hd == 128) && prefix_on_tensor_cores(p))
-    return p.hd == 128 ? run_prefix_tc<128>(ctx, pl, p, st) : run_prefix_tc<64>(ctx, pl, p, st);
+    return p.hd == 128 ? (pl->wide >= 0 ? run_prefix_tc<128, true>(ctx, pl, p, st) : run_prefix_tc<128, false>(ctx, pl, p, st))
+                       : (pl->wide >= 0 ? run_prefix_tc<64, true>(ctx, pl, p, st) : run_prefix_tc<64, false>(ctx, pl, p, st));
   p.lds = p.Pp + ((p.S + 31) & ~31);
   TRY(ensure(ctx->pfx, size_t(rows) * size_t(p.lds) * 4));
   p.scores = static_cast<int32_t*>(ctx->pfx.p);

@@ -126,6 +126,20 @@ def test_prefix_attention_plans(ctx, change, B):
     check_attention(ctx, x, rng.integers(2, 13, size=B), {**PLAN, **change})
 
 
+@pytest.mark.parametrize("mult,shift", [(1, 10), (3, 11), (1, 9), (5, 13), (2896, 36), (5, 34), (0, 3)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefix_attention_score_ties(ctx, mult, shift, hd):
+    """Scores around both ends of the constants that the tensor-core forms take; a
+    thousandth of the scores lie half way between integers and change the exponentials."""
+    rng = np.random.default_rng(shift)
+    x = attention_problem(rng, 70, 2, 4, 2, hd, 590, 12)
+    for n in ("q", "k", "ks"):
+        x[n][:] = rng.integers(-60, 61, size=x[n].shape)
+    lut = (16000 >> np.arange(14)).astype(np.int16)
+    check_attention(ctx, x, rng.integers(2, 13, size=70),
+                    {**PLAN, "score_mult": mult, "score_shift": shift, "lut_shift": 0, "exp_lut": lut})
+
+
 def test_prefix_attention_empty_rows_and_lengths(ctx):
     """No prefix, no suffix entries, fewer entries than new tokens, neither."""
     rng = np.random.default_rng(3)
