@@ -273,8 +273,11 @@ void prefix_params(PrefixParams& p, const myl_attn_plan* pl, const myl_prefix* p
 }
 
 // Rows up to which a call counts as a decode batch: rows spread over as many
-// blocks as adapters, outputs by single threads.
-constexpr int64_t AD_FEW = 128;
+// blocks as adapters, outputs by single threads. With a 3584 x 3584 projection and
+// rank 32, this form / the one for many rows, us: 32 rows of one adapter 23 / 28, of
+// 32 adapters 24 / 145; 128 rows of one 32 / 37, of 128 38 / 158; 512 rows of one
+// 41 / 41, of 8 42 / 48, of 512 62 / 177. More rows read each adapter too often.
+constexpr int64_t AD_FEW = 512;
 
 // h of the rows' adapters, then their share of y (int16, the projection's
 // output); the workspace is held.
@@ -821,8 +824,6 @@ int myl_verify_dev(myl_ctx* ctx, const myl_verifier* v, const int32_t* target, i
   p.V = int(vocab);
   p.lut = v->d_lut;
   p.lut_len = int32_t(v->len);
-  p.mult = v->mult;
-  p.shift = v->shift;
   p.reach = v->reach;
   p.scaled = v->scaled;
   p.pre = v->pre;

@@ -38,8 +38,6 @@ struct VerifyParams {
   int B, D, V;
   const int16_t* lut;  // [lut_len + 1], entry lut_len = 0
   int32_t lut_len;
-  uint32_t mult;
-  int shift;
   int32_t reach;  // largest difference to the maximum with a table entry above zero; INT32_MAX: no bound
   // (d * mult) >> shift for d <= reach as umulhi(d << pre, scaled) >> post: d * mult < 2^(31 + shift)
   // there, so mult << (32 - shift - pre) fits 32 bits with reach << pre filling them
@@ -62,12 +60,6 @@ __device__ __forceinline__ uint32_t verify_weight(const VerifyParams& p, int32_t
   const uint32_t d = min(uint32_t(m) - uint32_t(l), uint32_t(INT32_MAX));  // m >= l
   const uint32_t idx = __umulhi(d << p.pre, p.scaled) >> p.post;
   return uint32_t(uint16_t(__ldg(p.lut + (d <= uint32_t(p.reach) ? idx : uint32_t(p.lut_len)))));
-}
-
-// The smallest logit that can carry weight below the maximum m.
-__device__ __forceinline__ int32_t verify_floor(const VerifyParams& p, int32_t m) {
-  const int64_t t = int64_t(m) - p.reach;
-  return p.reach == INT32_MAX || t < INT32_MIN ? INT32_MIN : int32_t(t);
 }
 
 __device__ __forceinline__ int verify_count(const VerifyParams& p, int b) {
