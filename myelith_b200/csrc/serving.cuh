@@ -635,8 +635,10 @@ int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_
     return fail(MYL_ERR_SHAPE, "%lld query heads over %lld KV heads", (long long)num_heads, (long long)nkv);
   if (ldq < num_heads * hd || ldo < num_heads * hd || (suffix_cap > 0 && (pos_stride < hd || head_stride < 0 || seq_stride < 0)))
     return fail(MYL_ERR_SHAPE, "row or cache strides shorter than a row");
-  if (!aligned16(q) || ldq % 8 || (suffix_cap > 0 && (!aligned16(k_suffix) || pos_stride % 8 || head_stride % 8 || seq_stride % 8)))
-    return fail(MYL_ERR_UNSUPPORTED, "queries and suffix keys must lie on 16-byte boundaries (strides in multiples of 8)");
+  if (!aligned16(q) || ldq % 8 ||
+      (suffix_cap > 0 && (!aligned16(k_suffix) || !aligned16(v_suffix) || pos_stride % 8 || head_stride % 8 || seq_stride % 8)))
+    return fail(MYL_ERR_UNSUPPORTED,
+                "queries, suffix keys and suffix values must lie on 16-byte boundaries (strides in multiples of 8)");
   const int64_t keys = prefix->P + suffix_cap;
   // softmax.rs:46: the i32 sum of up to `keys` exponentials
   if (keys > INT32_MAX / 2 || int64_t(plan->exp_max) * keys > INT32_MAX)

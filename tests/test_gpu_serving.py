@@ -255,6 +255,29 @@ def test_prefix_attention_rejects(ctx):
     ctx.synchronize()  # the context stays usable
 
 
+def off_boundary(t):
+    """The same values in a tensor that starts 2 bytes past a 16-byte boundary."""
+    flat = torch.zeros(t.numel() + 8, dtype=t.dtype, device=t.device)
+    flat[1:1 + t.numel()] = t.reshape(-1)
+    return flat[1:1 + t.numel()].view(t.shape)
+
+
+@pytest.mark.parametrize("which", ["q", "ks", "vs"])
+def test_prefix_attention_rejects_unaligned_operands(ctx, which):
+    """Refused on the host, whatever kernels the size would select."""
+    rng = np.random.default_rng(4)
+    x = attention_problem(rng, 2, 1, 4, 2, 64, 20, 8)
+    plan, prefix = make_plan(ctx, PLAN), myl.Prefix(ctx, dev(x["k"]), dev(x["v"]))
+    a = {n: dev(x[n]) for n in ("q", "ks", "vs")}
+    a[which] = off_boundary(a[which])
+    out = torch.full((2, 1, 256), 77, dtype=torch.int16, device="cuda")
+    with pytest.raises(myl.MylError) as e:
+        prefix.attention_dev(plan, a["q"], a["ks"], a["vs"], dev(np.array([3, 8], np.int32)), out)
+    assert e.value.code == myl.MYL_ERR_UNSUPPORTED
+    torch.cuda.synchronize()
+    assert (out == 77).all()
+
+
 # ---- low-rank adapters ----------------------------------------------------------------
 
 def adapter_problem(rng, M, K, N, r, num, full=False):
