@@ -700,12 +700,15 @@ int myl_verify_dev(myl_ctx* ctx, const myl_verifier* verifier, const int32_t* ta
  * continue sequence `seq` of `parent`, each for up to max_new more positions.
  * The parent's positions become a shared prefix (laid out once; the parent may
  * go on or be released) and the parent's last logits every sequence's, so that
- * myl_decode_greedy can follow at once; results equal separate sessions that hold
- * the prompt each. head_dim a multiple of 8 up to 248, prob_frac_bits <= 15; no
+ * myl_decode_greedy can follow at once, also after myl_session_reset or a rewind to
+ * the prefix's end (a parent that was itself rewound has no logits to give: the
+ * fork needs a forward first); results equal separate sessions that hold the
+ * prompt each. head_dim a multiple of 8 up to 248, prob_frac_bits <= 15; no
  * fork of a fork. */
 int myl_session_fork(myl_ctx* ctx, const myl_model* model, const myl_session* parent, int64_t seq,
                      int64_t batch, int64_t max_new, myl_session** out);
-/* Forgets the positions from `position` on (at least a fork's prefix). */
+/* Forgets the positions from `position` on (at least a fork's prefix). Where
+ * that leaves no logits for the position, myl_decode_greedy is refused until a forward. */
 int myl_session_rewind(myl_ctx* ctx, myl_session* s, int64_t position);
 /* Low-rank adapters of one layer's fused q/k/v rows (out_features = (heads + 2 *
  * kv_heads) * head_dim) or output projection, added after the projection and its
@@ -718,7 +721,8 @@ int myl_session_set_adapters(myl_ctx* ctx, myl_session* s, int64_t layer, int pr
 /* Each sequence's adapter (host array [batch], -1: none; all -1 at first). */
 int myl_session_set_adapter_ids(myl_ctx* ctx, myl_session* s, const int32_t* ids);
 /* myl_forward that leaves the logits of all T positions in device memory, logits
- * [batch][T][vocab] int32 (the input of myl_verify_dev). At most rows of one
+ * [batch][T][vocab] int32 (the input of myl_verify_dev), the last position's in the
+ * session too. At most rows of one
  * prefill call: batch * T <= max(batch, 1024) for a fork. */
 int myl_forward_logits_dev(myl_ctx* ctx, const myl_model* model, myl_session* s,
                            const int32_t* tokens, int64_t T, int32_t* logits);

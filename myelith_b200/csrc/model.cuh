@@ -94,6 +94,7 @@ struct myl_session {
   unsigned* rowmax = nullptr;  // [rows_cap * nq] attention row maxima, zero between calls
   int max_chunks = 0;
   int32_t* logits = nullptr;
+  int64_t logits_pos = -1;  // the position that `logits` select the token of, -1: none
   int64_t* keys = nullptr;
   int32_t* tok_in = nullptr;
   int32_t* next_tok = nullptr;
@@ -122,6 +123,7 @@ struct myl_session {
   int64_t prefix_len = 0;
   std::vector<myl_prefix*> prefixes;
   std::vector<myl_attn_plan*> plans;
+  int32_t* prompt_logits = nullptr;  // [V] after the prefix (null: the parent had none)
   int32_t* d_lens = nullptr;  // [B] entries of the own caches, the new tokens included
   // low-rank adapters by layer (may be null) and the sequences' adapter ids
   std::vector<const myl_adapters*> ad_qkv, ad_o;
@@ -136,6 +138,7 @@ static int session_adapters(myl_ctx* ctx, myl_session* s, const myl_adapters* ad
                             int64_t rows, int16_t* y, int64_t ldy, cudaStream_t st);
 static int session_step(myl_ctx* ctx, myl_session* s, int64_t T, cudaStream_t st);
 static void session_unfork(myl_ctx* ctx, myl_session* s);
+static int session_prompt_logits(myl_session* s, cudaStream_t st);
 
 namespace {
 
@@ -928,7 +931,8 @@ int myl_session_release(myl_ctx* ctx, myl_session* s) {
 int myl_session_reset(myl_ctx* ctx, myl_session* s) {
   if (!ctx || !s) return fail(MYL_ERR_ARG, "null argument");
   CUDA_TRY(cudaSetDevice(ctx->device));
-  return set_pos(s, s->prefix_len, ctx->stream);
+  TRY(set_pos(s, s->prefix_len, ctx->stream));
+  return session_prompt_logits(s, ctx->stream);
 }
 
 int64_t myl_session_position(const myl_session* s) { return s ? s->pos : -1; }
@@ -1005,7 +1009,9 @@ int myl_forward(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_t*
   cudaStream_t st = ctx->stream;
   TRY(ws_acquire(ctx, st));
   CUDA_TRY(cudaEventRecord(s->ev[0], st));
+  s->logits_pos = -1;
   TRY(prefill(ctx, m, s, tokens, T, true, st));
+  s->logits_pos = s->pos;
   CUDA_TRY(cudaEventRecord(s->ev[1], st));
   TRY(ws_release(ctx, st));
   if (logits)
@@ -1022,6 +1028,7 @@ static int decode_loop(myl_ctx* ctx, const myl_model* m, myl_session* s, int64_t
   if (m->world > 1 && (digests || step_logits))
     return fail(MYL_ERR_UNSUPPORTED, "digests and step logits need the whole vocabulary (world 1)");
   const int64_t P = s->pos;
+  if (max_new > 0) s->logits_pos = -1;
   CUDA_TRY(cudaMemsetAsync(s->d_step, 0, 8, st));
   const bool host_steps = digests || step_logits;
   std::vector<Sha256Stream> sha(digests ? size_t(s->B) : 0);
@@ -1078,6 +1085,7 @@ static int decode_loop(myl_ctx* ctx, const myl_model* m, myl_session* s, int64_t
   CUDA_TRY(cudaEventRecord(s->ev[3], st));
   s->pos = P + max_new;
   if (max_new > 0) {
+    s->logits_pos = s->pos;
     CUDA_TRY(cudaMemcpy2DAsync(out_tokens, size_t(max_new) * 4, s->out_tokens, size_t(s->max_pos) * 4,
                                size_t(max_new) * 4, size_t(s->B), cudaMemcpyDeviceToHost, st));
   }
@@ -1120,6 +1128,8 @@ int myl_decode_greedy(myl_ctx* ctx, const myl_model* m, myl_session* s, int64_t 
   if (!ctx || !m || !s || s->m != m || (max_new > 0 && !out_tokens))
     return fail(MYL_ERR_ARG, "null argument");
   if (s->pos <= 0) return fail(MYL_ERR_ARG, "the session holds no prompt (run myl_forward first)");
+  if (max_new > 0 && s->logits_pos != s->pos)
+    return fail(MYL_ERR_ARG, "the session has no logits for position %lld (run myl_forward first)", (long long)s->pos);
   if (max_new < 0 || s->pos + max_new > s->max_pos)
     return fail(MYL_ERR_SHAPE, "%lld positions beyond the session's %lld", (long long)(s->pos + max_new),
                 (long long)s->max_pos);

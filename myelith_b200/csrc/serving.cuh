@@ -441,6 +441,17 @@ static int session_share(myl_ctx* ctx, myl_session* s, const myl_session* parent
   return MYL_OK;
 }
 
+// Every sequence of a fork at the end of its prefix selects from the prompt's logits.
+static int session_prompt_logits(myl_session* s, cudaStream_t st) {
+  if (!s->prompt_logits || s->pos != s->prefix_len || s->logits_pos == s->pos) return MYL_OK;
+  s->logits_pos = -1;
+  const size_t row = size_t(s->m->V);
+  for (int64_t b = 0; b < s->B; ++b)
+    CUDA_TRY(cudaMemcpyAsync(s->logits + size_t(b) * row, s->prompt_logits, row * 4, cudaMemcpyDeviceToDevice, st));
+  s->logits_pos = s->pos;
+  return MYL_OK;
+}
+
 extern "C" {
 
 int myl_session_fork(myl_ctx* ctx, const myl_model* m, const myl_session* parent, int64_t seq, int64_t batch,
@@ -466,11 +477,15 @@ int myl_session_fork(myl_ctx* ctx, const myl_model* m, const myl_session* parent
   int rc = session_share(ctx, s, parent, seq);
   if (rc == MYL_OK) rc = session_alloc(ctx, s);
   if (rc == MYL_OK) rc = set_pos(s, s->prefix_len, ctx->stream);
-  // the parent's last logits are every sequence's, so that decoding can start at once
-  for (int64_t b = 0; rc == MYL_OK && b < batch; ++b)
-    if (cudaMemcpyAsync(s->logits + b * m->V, parent->logits + seq * m->V, size_t(m->V) * 4, cudaMemcpyDeviceToDevice,
-                        ctx->stream) != cudaSuccess)
+  // the parent's last logits are every sequence's, so that decoding can start at
+  // once (a parent that was rewound has none)
+  if (rc == MYL_OK && parent->logits_pos == parent->pos) {
+    rc = dev_alloc(s->allocs, &s->prompt_logits, size_t(m->V));
+    if (rc == MYL_OK && cudaMemcpyAsync(s->prompt_logits, parent->logits + seq * m->V, size_t(m->V) * 4,
+                                        cudaMemcpyDeviceToDevice, ctx->stream) != cudaSuccess)
       rc = fail(MYL_ERR_CUDA, "logits copy");
+    if (rc == MYL_OK) rc = session_prompt_logits(s, ctx->stream);
+  }
   if (rc != MYL_OK) {
     release_session(ctx, s);
     return rc;
@@ -485,7 +500,8 @@ int myl_session_rewind(myl_ctx* ctx, myl_session* s, int64_t position) {
     return fail(MYL_ERR_SHAPE, "position %lld outside [%lld, %lld]", (long long)position, (long long)s->prefix_len,
                 (long long)s->pos);
   CUDA_TRY(cudaSetDevice(ctx->device));
-  return set_pos(s, position, ctx->stream);
+  TRY(set_pos(s, position, ctx->stream));
+  return session_prompt_logits(s, ctx->stream);
 }
 
 int myl_session_set_adapters(myl_ctx* ctx, myl_session* s, int64_t layer, int projection, const myl_adapters* ad) {
@@ -554,11 +570,17 @@ int myl_forward_logits_dev(myl_ctx* ctx, const myl_model* m, myl_session* s, con
   std::memcpy(s->h_tokens, tokens, size_t(s->B * T) * 4);
   CUDA_TRY(cudaMemcpyAsync(s->tok_in, s->h_tokens, size_t(s->B * T) * 4, cudaMemcpyHostToDevice, st));
   TRY(set_pos(s, s->pos, st));
+  s->logits_pos = -1;
   {
     PdlScope pdl(ctx);
     TRY(model_forward(ctx, m, s, s->tok_in, T, true, s->pos + T, st, logits));
   }
+  // each sequence's last row, so that decoding can follow
+  const size_t row = size_t(m->V) * 4;
+  CUDA_TRY(cudaMemcpy2DAsync(s->logits, row, logits + (T - 1) * m->V, size_t(T) * row, row, size_t(s->B),
+                             cudaMemcpyDeviceToDevice, st));
   TRY(set_pos(s, s->pos + T, st));
+  s->logits_pos = s->pos;
   TRY(ws_release(ctx, st));
   return check_device_error(ctx);
 }

@@ -370,7 +370,8 @@ class Session:
         return Session._forked(self, seq, batch, max_new)
 
     def rewind(self, position: int) -> None:
-        """Forgets the positions from `position` on."""
+        """Forgets the positions from `position` on; decode() needs a forward() first
+        (a fork's prefix end still has the prompt's logits)."""
         _check("myl_session_rewind", _lib().myl_session_rewind(self.model.ctx.handle, self._h, position))
 
     def set_adapters(self, layer: int, projection: str, adapters) -> None:

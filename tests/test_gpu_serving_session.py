@@ -241,3 +241,80 @@ def test_example_serves_what_single_requests_sample(ctx, drafts):
             hist[b] += [int(t) for t in out[b][:n]]
         done += n
     assert np.array_equal(got, np.array([h[len(prompt):len(prompt) + new] for h in hist]))
+
+
+# ---- the logits that decode() starts from -------------------------------------------------
+
+
+def prompted(m, spec, B=2, P=9):
+    prompt = S.prompt_tokens(spec.vocab, P, seed=P)
+    s = m.session(B, P + 40)
+    s.forward(np.tile(prompt, (B, 1)))
+    return s, prompt
+
+
+def test_decode_after_forward_logits_goes_on_from_the_last_position(model):
+    spec, m = model
+    tokens = np.random.default_rng(1).integers(0, spec.vocab, size=(2, 5)).astype(np.int32)
+    plain, _ = prompted(m, spec)
+    plain.forward(tokens)
+    want = plain.decode(4, keep_logits=True)
+    for T in (5, 1):  # all five at once, or the last by itself
+        s, _ = prompted(m, spec)
+        parent = m.session(1, 30)
+        parent.forward(S.prompt_tokens(spec.vocab, 9, seed=9)[None])
+        for t in (s, parent.fork(2, 30)):
+            if T == 1:
+                t.forward(tokens[:, :4])
+            all_logits(t, tokens[:, 5 - T:])
+            got = t.decode(4, keep_logits=True)
+            assert np.array_equal(got[0], want[0]) and np.array_equal(got[2], want[2])
+
+
+def test_decode_is_refused_without_logits_for_the_position(model):
+    """After a step back the logits kept are another position's."""
+    spec, m = model
+    tokens = np.random.default_rng(2).integers(0, spec.vocab, size=(2, 6)).astype(np.int32)
+    s, prompt = prompted(m, spec)
+    s.forward(tokens)
+    s.rewind(s.position)  # forgets nothing
+    s.decode(1)
+    s.rewind(12)
+    with pytest.raises(myl.MylError) as e:
+        s.decode(1)
+    assert e.value.code == myl.MYL_ERR_ARG and s.position == 12
+    fork = s.fork(3, 20)  # the parent has none to give
+    with pytest.raises(myl.MylError):
+        fork.decode(2)
+    assert fork.position == 12
+    # a forward brings them back, in both
+    plain, _ = prompted(m, spec, B=3)
+    plain.forward(np.tile(tokens[:1, :3], (3, 1)))
+    want = plain.forward(np.tile(tokens[:1, 3:4], (3, 1)))
+    assert np.array_equal(fork.forward(np.tile(tokens[:1, 3:4], (3, 1))), want)
+    after = plain.decode(3)[0]
+    assert np.array_equal(fork.decode(3)[0], after)
+    s.forward(tokens[:, 3:4])
+    assert np.array_equal(s.decode(3)[0][0], after[0])
+    # a fork after forward() behind a step back decodes from that forward's logits
+    s.rewind(12)
+    s.forward(tokens[:, 3:4])
+    assert np.array_equal(s.fork(2, 5).decode(3)[0][1], after[0])
+
+
+def test_fork_goes_back_to_the_prompts_logits(model):
+    spec, m = model
+    parent = m.session(1, 30)
+    parent.forward(S.prompt_tokens(spec.vocab, 9, seed=9)[None])
+    fork = parent.fork(3, 20)
+    parent.forward(np.array([[1, 2]]))
+    parent.release()
+    first = fork.decode(6, keep_logits=True)
+    for back in (fork.reset, lambda: fork.rewind(9)):
+        fork.forward(np.full((3, 2), 5, np.int32))
+        back()
+        again = fork.decode(6, keep_logits=True)
+        assert np.array_equal(first[0], again[0]) and np.array_equal(first[2], again[2])
+    fork.reset()
+    fork.rewind(9)
+    assert np.array_equal(fork.decode(6)[0], first[0])
