@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define MYL_ABI_VERSION 1
+#define MYL_ABI_VERSION 2 /* 2: myl_forward_logits_dev takes a stream */
 
 enum myl_status {
   MYL_OK = 0,
@@ -722,10 +722,11 @@ int myl_session_set_adapters(myl_ctx* ctx, myl_session* s, int64_t layer, int pr
 int myl_session_set_adapter_ids(myl_ctx* ctx, myl_session* s, const int32_t* ids);
 /* myl_forward that leaves the logits of all T positions in device memory, logits
  * [batch][T][vocab] int32 (the input of myl_verify_dev), the last position's in the
- * session too. At most rows of one
+ * session too. They are written after the work that `stream` holds at the call
+ * (the buffer's last use); the call returns when they are complete. At most rows of one
  * prefill call: batch * T <= max(batch, 1024) for a fork. */
 int myl_forward_logits_dev(myl_ctx* ctx, const myl_model* model, myl_session* s,
-                           const int32_t* tokens, int64_t T, int32_t* logits);
+                           const int32_t* tokens, int64_t T, int32_t* logits, void* stream);
 
 /* --- Allocation-free variant ------------------------------------------------------
  * No counterpart in the reference: its CPU path never allocates device memory.

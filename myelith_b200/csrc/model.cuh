@@ -108,6 +108,7 @@ struct myl_session {
   // device time of the last prefill (myl_forward) and decode loop, CUDA
   // events on the launching stream
   cudaEvent_t ev[4] = {};
+  cudaEvent_t ev_out = nullptr;  // the last use of a caller's output buffer
   float prefill_ms = 0.f, decode_ms = 0.f;
   // tensor parallelism: one peer-memory region per rank (myl_session_set_tp)
   // holding two receive regions [world][rows_cap][H] int64 (o_proj and down
@@ -365,6 +366,7 @@ int session_alloc(myl_ctx* ctx, myl_session* s) {
   TRY(dev_alloc(A, &s->last_rows, size_t(B)));
   TRY(dev_alloc(A, &s->out_tokens, size_t(B * s->max_pos)));
   for (auto& e : s->ev) CUDA_TRY(cudaEventCreate(&e));
+  CUDA_TRY(cudaEventCreateWithFlags(&s->ev_out, cudaEventDisableTiming));
   CUDA_TRY(cudaMallocHost(&s->h_pos, sizeof(int64_t)));
   CUDA_TRY(cudaMallocHost(&s->h_tokens, size_t(R) * 4));
   CUDA_TRY(cudaMallocHost(&s->h_logits, size_t(B * m->V) * 4));
@@ -378,6 +380,7 @@ void release_session(myl_ctx* ctx, myl_session* s) {
   session_unfork(ctx, s);
   for (auto& e : s->ev)
     if (e) cudaEventDestroy(e);
+  if (s->ev_out) cudaEventDestroy(s->ev_out);
   for (void* p : s->allocs) cudaFree(p);
   if (s->h_pos) cudaFreeHost(s->h_pos);
   if (s->h_tokens) cudaFreeHost(s->h_tokens);

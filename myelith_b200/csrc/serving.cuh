@@ -553,7 +553,7 @@ int myl_session_set_adapter_ids(myl_ctx* ctx, myl_session* s, const int32_t* ids
 }
 
 int myl_forward_logits_dev(myl_ctx* ctx, const myl_model* m, myl_session* s, const int32_t* tokens, int64_t T,
-                           int32_t* logits) {
+                           int32_t* logits, void* stream) {
   if (!ctx || !m || !s || s->m != m || !tokens || !logits) return fail(MYL_ERR_ARG, "null argument");
   if (m->world > 1) return fail(MYL_ERR_UNSUPPORTED, "logits of every position need the whole vocabulary (world 1)");
   if (T <= 0 || s->B * T > s->rows_cap || s->pos + T > s->max_pos)
@@ -566,10 +566,13 @@ int myl_forward_logits_dev(myl_ctx* ctx, const myl_model* m, myl_session* s, con
   cudaStream_t st = ctx->stream;
   if (!s->xf_all) TRY(dev_alloc(s->allocs, &s->xf_all, size_t(s->rows_cap * m->H)));
   TRY(ws_acquire(ctx, st));
+  // the context's own stream does not wait for others by itself
+  CUDA_TRY(cudaEventRecord(s->ev_out, static_cast<cudaStream_t>(stream)));
   CUDA_TRY(cudaStreamSynchronize(st));  // the pinned token buffer is free again
   std::memcpy(s->h_tokens, tokens, size_t(s->B * T) * 4);
   CUDA_TRY(cudaMemcpyAsync(s->tok_in, s->h_tokens, size_t(s->B * T) * 4, cudaMemcpyHostToDevice, st));
   TRY(set_pos(s, s->pos, st));
+  CUDA_TRY(cudaStreamWaitEvent(st, s->ev_out, 0));
   s->logits_pos = -1;
   {
     PdlScope pdl(ctx);

@@ -213,7 +213,7 @@ def _lib():
                 ("myl_session_rewind", [vp, vp, i64], i32),
                 ("myl_session_set_adapters", [vp, vp, i64, i32, vp], i32),
                 ("myl_session_set_adapter_ids", [vp, vp, vp], i32),
-                ("myl_forward_logits_dev", [vp, vp, vp, vp, i64, vp], i32),
+                ("myl_forward_logits_dev", [vp, vp, vp, vp, i64, vp, vp], i32),
                 ("myl_session_timing", [vp, C.POINTER(C.c_float), C.POINTER(C.c_float)], i32),
                 ("myl_rmsnorm_i16", [vp, vp, i64, i64, vp, vp, vp, vp, i64, C.c_uint8, C.c_uint8,
                                      i64, C.c_uint8, vp], i32),
@@ -388,10 +388,12 @@ class Session:
         _check("myl_session_set_adapter_ids", _lib().myl_session_set_adapter_ids(
             self.model.ctx.handle, self._h, a.ctypes.data))
 
-    def forward_logits_dev(self, tokens, logits) -> None:
+    def forward_logits_dev(self, tokens, logits, stream=None) -> None:
         """forward() of tokens [batch][T] whose logits of every position go to the
-        torch CUDA tensor logits [batch, T, vocab] int32."""
+        torch CUDA tensor logits [batch, T, vocab] int32, after what the given
+        stream (default: torch's current one) holds; complete on return."""
         from . import MYL_ERR_SHAPE, MylError
+        from .serving import _stream
 
         t = np.ascontiguousarray(np.asarray(tokens, np.int32)).reshape(self.batch, -1)
         if str(logits.dtype) != "torch.int32" or not logits.is_cuda or not logits.is_contiguous() or \
@@ -399,7 +401,8 @@ class Session:
             raise MylError("myl_forward_logits_dev", MYL_ERR_SHAPE,
                            f"logits {tuple(logits.shape)} {logits.dtype} for tokens {t.shape}")
         _check("myl_forward_logits_dev", _lib().myl_forward_logits_dev(
-            self.model.ctx.handle, self.model.handle, self._h, t.ctypes.data, t.shape[1], logits.data_ptr()))
+            self.model.ctx.handle, self.model.handle, self._h, t.ctypes.data, t.shape[1], logits.data_ptr(),
+            _stream(self.model.ctx, stream)))
 
     @property
     def handle(self):

@@ -318,3 +318,26 @@ def test_fork_goes_back_to_the_prompts_logits(model):
     fork.reset()
     fork.rewind(9)
     assert np.array_equal(fork.decode(6)[0], first[0])
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_forward_logits_waits_for_the_buffers_last_use(model, own):
+    """Work that torch's stream still has to do on the logits tensor comes before them."""
+    spec, m = model
+    s, _ = prompted(m, spec)
+    tokens = np.random.default_rng(3).integers(0, spec.vocab, size=(2, 4)).astype(np.int32)
+    at = s.position
+    want = all_logits(s, tokens)
+    s.rewind(at)
+    out = torch.zeros((2, 4, spec.vocab), dtype=torch.int32, device="cuda")
+    read = torch.zeros_like(out)
+    stream = torch.cuda.Stream() if own else torch.cuda.current_stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(100_000_000)  # about 50 ms
+        out.fill_(7)
+        read.copy_(out)
+        s.forward_logits_dev(tokens, out)
+    torch.cuda.synchronize()
+    assert np.array_equal(out.cpu().numpy(), want)
+    assert (read == 7).all()
