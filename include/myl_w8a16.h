@@ -635,7 +635,9 @@ int64_t myl_prefix_positions(const myl_prefix* prefix);
  * out [batch * T][ldo] int16; a row that sees no key gives zeros. A length
  * outside [0, suffix_cap] is clamped and reported as MYL_ERR_DEVICE at the next
  * synchronising call. q, k_suffix and v_suffix are 16-byte aligned, strides
- * multiples of 8 elements. Equal to attention_int over the concatenated keys. */
+ * multiples of 8 elements. Equal to attention_int over the concatenated keys.
+ * The scores work in the context's workspace; a call that would need more than
+ * about 1 GiB of it runs in slices of its rows. */
 int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_prefix* prefix,
                              const int16_t* q, int64_t batch, int64_t T, int64_t num_heads,
                              int64_t ldq, const int16_t* k_suffix, const int16_t* v_suffix,

@@ -48,6 +48,7 @@ struct PrefixParams {
   const int16_t *ks, *vs;  // suffix caches
   int64_t seq_stride, head_stride, pos_stride;
   int S;  // suffix capacity
+  int after;  // new tokens of a request that follow these T (a call in slices)
   const int32_t* lens;
   int64_t score_mult;
   int score_shift;
@@ -77,7 +78,7 @@ __device__ __forceinline__ int pfx_len(const PrefixParams& p, int b) {
 }
 __device__ __forceinline__ int pfx_clamped(const PrefixParams& p, int b) { return min(max(p.lens[b], 0), p.S); }
 // Suffix entries that token t of a request with n entries sees.
-__device__ __forceinline__ int pfx_seen(const PrefixParams& p, int n, int t) { return max(0, n - p.T + t + 1); }
+__device__ __forceinline__ int pfx_seen(const PrefixParams& p, int n, int t) { return max(0, n - p.after - p.T + t + 1); }
 
 __device__ __forceinline__ int32_t pfx_score(const PrefixParams& p, int64_t dot) {
   const int64_t prod = int64_t(uint64_t(dot) * uint64_t(p.score_mult));

@@ -213,14 +213,16 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaSt
   return MYL_OK;
 }
 
-// The attention of `p` (pointers, shapes and plan filled in) with the
-// context's workspace, which the caller holds.
-int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaStream_t st) {
+bool prefix_tc_form(const myl_attn_plan* pl, const PrefixParams& p) {
+  return pl->tc && (p.hd == 64 || p.hd == 128) && prefix_on_tensor_cores(p);
+}
+
+int run_prefix_slice(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaStream_t st) {
   const int64_t rows = int64_t(p.nkv) * p.R;
   p.err = ctx->d_err;
   const unsigned gy = unsigned(p.nkv * ((p.R + PFX_ROWS - 1) / PFX_ROWS));
   if (gy > 65535u) return fail(MYL_ERR_UNSUPPORTED, "%d query rows per KV head", p.R);
-  if (pl->tc && (p.hd == 64 || p.hd == 128) && prefix_on_tensor_cores(p))
+  if (prefix_tc_form(pl, p))
     return p.hd == 128 ? (pl->wide >= 0 ? run_prefix_tc<128, true>(ctx, pl, p, st) : run_prefix_tc<128, false>(ctx, pl, p, st))
                        : (pl->wide >= 0 ? run_prefix_tc<64, true>(ctx, pl, p, st) : run_prefix_tc<64, false>(ctx, pl, p, st));
   p.lds = p.Pp + ((p.S + 31) & ~31);
@@ -253,6 +255,40 @@ int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p,
     CUDA_TRY(cudaLaunchKernelEx(&l4.cfg, prefix_finish_kernel, p, rows));
     ctx->launches++;
   }
+  return MYL_OK;
+}
+
+// Workspace of one slice of a call, in bytes: a session's score rows are kept near
+// this size too.
+constexpr int64_t PFX_WS_BYTES = int64_t(1) << 30;
+
+// The attention of `p` (pointers, shapes and plan filled in) with the
+// context's workspace, which the caller holds; in slices of whole requests, or of
+// one request's tokens, where the scores of all rows would take more than
+// PFX_WS_BYTES (each slice reads the prefix again).
+int run_prefix_attention(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaStream_t st) {
+  const int64_t sfx = (p.S + 31) & ~31;
+  const int64_t row = prefix_tc_form(pl, p)
+                          ? 2 * int64_t(p.Pp) + 4 * sfx + 4 * p.hd * int64_t((p.S + PTC_SFX_KEYS - 1) / PTC_SFX_KEYS)
+                          : 4 * (p.Pp + sfx) + 8 * p.hd;
+  const int64_t tokens = std::max<int64_t>(1, PFX_WS_BYTES / (row * p.nq));
+  if (int64_t(p.B) * p.T <= tokens) return run_prefix_slice(ctx, pl, p, st);
+  const int T = p.T, B = p.B;
+  const int reqs = int(std::max<int64_t>(1, tokens / T)), toks = int(std::min<int64_t>(T, tokens));
+  for (int b = 0; b < B; b += reqs)
+    for (int t = 0; t < T; t += toks) {
+      PrefixParams s = p;
+      s.B = std::min(reqs, B - b);
+      s.T = std::min(toks, T - t);
+      s.after = T - t - s.T;
+      s.R = s.B * s.T * s.G;
+      const int64_t at = int64_t(b) * T + t;
+      s.q += at * p.ldq;
+      s.out += at * p.ldo;
+      s.lens += b;
+      if (p.S > 0) s.ks += b * p.seq_stride, s.vs += b * p.seq_stride;
+      TRY(run_prefix_slice(ctx, pl, s, st));
+    }
   return MYL_OK;
 }
 

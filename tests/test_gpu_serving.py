@@ -278,6 +278,49 @@ def test_prefix_attention_rejects_unaligned_operands(ctx, which):
     assert (out == 77).all()
 
 
+@pytest.mark.parametrize("B,T,nq,nkv,hd,P,S,part", [
+    (1, 1024, 28, 4, 128, 32749, 1100, (1, 128)),  # one long prompt on the tensor cores
+    (3, 700, 14, 2, 64, 60001, 720, (1, 175)),
+    (48, 24, 28, 4, 128, 32749, 40, (8, 24)),      # many requests
+    (64, 32, 4, 1, 8, 65541, 33, (16, 32)),        # kernels for few rows
+    (2, 2100, 4, 1, 8, 65541, 2100, (1, 700)),
+])
+def test_prefix_attention_workspace_is_bounded(B, T, nq, nkv, hd, P, S, part):
+    """Calls whose scores would take 2 to 4 GB equal their parts of (requests, tokens) and keep the
+    context's workspace near 1 GiB."""
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    g = torch.Generator(device="cuda").manual_seed(B + T)
+
+    def normal(shape, sigma):
+        return torch.empty(shape, device="cuda").normal_(0, sigma, generator=g).round_().to(torch.int16)
+
+    q, k, v = normal((B, T, nq, hd), 3000), normal((nkv, P, hd), 3000), normal((nkv, P, hd), 9000)
+    ks, vs = normal((B, nkv, S, hd), 3000), normal((B, nkv, S, hd), 9000)
+    lens = torch.randint(T // 2, S + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    out, ref = (torch.full((B, T, nq * hd), 77, dtype=torch.int16, device="cuda") for _ in range(2))
+    c = myl.Context(0)
+    try:
+        plan, prefix = make_plan(c, PLAN), myl.Prefix(c, k, v)
+        torch.cuda.synchronize()
+        free = torch.cuda.mem_get_info()[0]
+        prefix.attention_dev(plan, q, ks, vs, lens, out)
+        torch.cuda.synchronize()
+        used = free - torch.cuda.mem_get_info()[0]
+        nb, nt = part
+        for b in range(0, B, nb):
+            for t in range(0, T, nt):
+                n = (lens[b:b + nb] - (T - t - min(nt, T - t))).clamp(min=0)  # entries as of the part's last token
+                prefix.attention_dev(plan, q[b:b + nb, t:t + nt], ks[b:b + nb], vs[b:b + nb], n, ref[b:b + nb, t:t + nt])
+        c.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)
+        assert len(out.unique()) > 100
+        assert used < 1.25 * 2**30
+    finally:
+        c.close()
+
+
 # ---- low-rank adapters ----------------------------------------------------------------
 
 def adapter_problem(rng, M, K, N, r, num, full=False):
