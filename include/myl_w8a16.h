@@ -637,7 +637,8 @@ int64_t myl_prefix_positions(const myl_prefix* prefix);
  * synchronising call. q, k_suffix and v_suffix are 16-byte aligned, strides
  * multiples of 8 elements. Equal to attention_int over the concatenated keys.
  * The scores work in the context's workspace; a call that would need more than
- * about 1 GiB of it runs in slices of its rows. */
+ * about 1 GiB of it runs in slices of its rows. Limits: batch <= 65535, batch * T * (num_heads /
+ * kv_heads) <= 2^24. */
 int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_prefix* prefix,
                              const int16_t* q, int64_t batch, int64_t T, int64_t num_heads,
                              int64_t ldq, const int16_t* k_suffix, const int16_t* v_suffix,
@@ -687,7 +688,7 @@ int myl_linear_adapters_dev(myl_ctx* ctx, const myl_weight* w, const myl_requant
  * token outside the vocabulary counts as having no weight, a count outside
  * [0, drafted] is clamped; both are reported as MYL_ERR_DEVICE at the next
  * synchronising call. Limits: vocab times the largest table entry below 2^32,
- * drafted <= 1024. */
+ * vocab < 2^31 - 1024, drafted <= 1024, batch <= 2^20, batch * (2 drafted + 1) < 2^31. */
 typedef struct myl_verifier myl_verifier;
 int myl_verifier_create(myl_ctx* ctx, const int16_t* exp_lut, int64_t exp_len, uint32_t temp_mult,
                         uint8_t temp_shift, myl_verifier** out);

@@ -903,7 +903,7 @@ int myl_session_create(myl_ctx* ctx, const myl_model* m, int64_t batch, int64_t 
   *out = nullptr;
   if (batch <= 0 || max_positions <= 0) return fail(MYL_ERR_SHAPE, "batch and max_positions must be positive");
   // softmax.rs:46: the i32 sum of up to max_positions exponentials
-  if (int64_t(m->exp_max) * max_positions > INT32_MAX)
+  if (max_positions > INT32_MAX || int64_t(m->exp_max) * max_positions > INT32_MAX)
     return fail(MYL_ERR_OVERFLOW, "%lld positions overflow the softmax's i32 sum", (long long)max_positions);
   CUDA_TRY(cudaSetDevice(ctx->device));
   myl_session* s = new myl_session();

@@ -38,6 +38,7 @@ constexpr int PFX_ROWS = 8;       // query rows per block
 constexpr int PFX_SKEYS = 32;     // keys per scores block (8 threads each)
 constexpr int PFX_VKEYS = 256;    // keys per values block
 constexpr int PFX_MAX_HD = 248;
+constexpr int PFX_MAX_BATCH = 65535;  // requests are a grid's z index
 
 struct PrefixParams {
   const int16_t* q;

@@ -499,8 +499,9 @@ int myl_session_fork(myl_ctx* ctx, const myl_model* m, const myl_session* parent
   if (batch <= 0 || max_new <= 0 || seq < 0 || seq >= parent->B || parent->pos <= 0)
     return fail(MYL_ERR_SHAPE, "fork of sequence %lld at position %lld into %lld sequences of %lld more positions",
                 (long long)seq, (long long)parent->pos, (long long)batch, (long long)max_new);
-  if (int64_t(m->exp_max) * (parent->pos + max_new) > INT32_MAX)
-    return fail(MYL_ERR_OVERFLOW, "%lld positions overflow the softmax's i32 sum", (long long)(parent->pos + max_new));
+  if (batch > PFX_MAX_BATCH) return fail(MYL_ERR_UNSUPPORTED, "%lld sequences in one fork", (long long)batch);
+  if (max_new > INT32_MAX || int64_t(m->exp_max) * (parent->pos + max_new) > INT32_MAX)
+    return fail(MYL_ERR_OVERFLOW, "%lld more positions overflow the softmax's i32 sum", (long long)max_new);
   CUDA_TRY(cudaSetDevice(ctx->device));
   CUDA_TRY(cudaStreamSynchronize(ctx->stream));  // the parent's caches are complete
   myl_session* s = new myl_session();
@@ -694,19 +695,24 @@ int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_
   const int64_t nkv = prefix->nkv, hd = prefix->hd;
   if (num_heads <= 0 || num_heads % nkv)
     return fail(MYL_ERR_SHAPE, "%lld query heads over %lld KV heads", (long long)num_heads, (long long)nkv);
+  // (no product below passes 64 bits)
+  if (batch > PFX_MAX_BATCH || T > (1 << 24) || num_heads > (1 << 20))
+    return fail(MYL_ERR_UNSUPPORTED, "%lld requests x %lld tokens x %lld heads in one call", (long long)batch,
+                (long long)T, (long long)num_heads);
   if (ldq < num_heads * hd || ldo < num_heads * hd || (suffix_cap > 0 && (pos_stride < hd || head_stride < 0 || seq_stride < 0)))
     return fail(MYL_ERR_SHAPE, "row or cache strides shorter than a row");
   if (!aligned16(q) || ldq % 8 ||
       (suffix_cap > 0 && (!aligned16(k_suffix) || !aligned16(v_suffix) || pos_stride % 8 || head_stride % 8 || seq_stride % 8)))
     return fail(MYL_ERR_UNSUPPORTED,
                 "queries, suffix keys and suffix values must lie on 16-byte boundaries (strides in multiples of 8)");
-  const int64_t keys = prefix->P + suffix_cap;
   // softmax.rs:46: the i32 sum of up to `keys` exponentials
+  const int64_t keys = prefix->P + std::min<int64_t>(suffix_cap, INT32_MAX);
   if (keys > INT32_MAX / 2 || int64_t(plan->exp_max) * keys > INT32_MAX)
-    return fail(MYL_ERR_OVERFLOW, "%lld keys overflow the softmax's i32 sum", (long long)keys);
-  const int64_t R = batch * T * (num_heads / nkv);
-  if (R > (1 << 24) || nkv * R > INT32_MAX || batch > 65535)
-    return fail(MYL_ERR_UNSUPPORTED, "%lld query rows in one call", (long long)(nkv * R));
+    return fail(MYL_ERR_OVERFLOW, "%lld + %lld keys overflow the softmax's i32 sum", (long long)prefix->P,
+                (long long)suffix_cap);
+  const int64_t G = num_heads / nkv;
+  if (batch * T * G > (1 << 24) || batch * T * num_heads > INT32_MAX)
+    return fail(MYL_ERR_UNSUPPORTED, "%lld query rows in one call", (long long)(batch * T * num_heads));
   CUDA_TRY(cudaSetDevice(ctx->device));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   PrefixParams p{};
@@ -716,8 +722,8 @@ int myl_prefix_attention_dev(myl_ctx* ctx, const myl_attn_plan* plan, const myl_
   p.B = int(batch);
   p.T = int(T);
   p.nq = int(num_heads);
-  p.G = int(num_heads / nkv);
-  p.R = int(R);
+  p.G = int(G);
+  p.R = int(batch * T * G);
   p.ks = k_suffix;
   p.vs = v_suffix;
   p.seq_stride = seq_stride;
@@ -866,9 +872,10 @@ int myl_verify_dev(myl_ctx* ctx, const myl_verifier* v, const int32_t* target, i
       (draft && (draft_pos_stride < vocab || draft_seq_stride < 0)))
     return fail(MYL_ERR_SHAPE, "logit rows shorter than the vocabulary");
   // weights sums below 2^32, so that products of two fit 64 bits
-  if (int64_t(v->max) * vocab >= (int64_t(1) << 32))
+  if (vocab >= (int64_t(1) << 32) || int64_t(v->max) * vocab >= (int64_t(1) << 32))
     return fail(MYL_ERR_OVERFLOW, "%lld table weights of up to %d overflow 32 bits", (long long)vocab, v->max);
-  if (drafted > 1024 || batch > (1 << 20)) return fail(MYL_ERR_UNSUPPORTED, "at most 1024 drafted tokens, 2^20 requests");
+  if (drafted > 1024 || batch > (1 << 20) || batch * (2 * drafted + 1) > INT32_MAX || vocab > INT32_MAX - 1024)
+    return fail(MYL_ERR_UNSUPPORTED, "at most 1024 drafted tokens, 2^20 requests, 2^31 logit rows, 2^31 - 1025 logits");
   CUDA_TRY(cudaSetDevice(ctx->device));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (drafted == 0) draft = nullptr;

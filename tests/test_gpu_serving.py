@@ -600,6 +600,34 @@ def test_verify_rejects(ctx):
     ctx.synchronize()
 
 
+@pytest.mark.parametrize("entry,sizes,code", [
+    # batch, T, heads, suffix capacity: products that pass 32 and 64 bits
+    ("attention", (65536, 1, 4, 8), myl.MYL_ERR_UNSUPPORTED), ("attention", (2**40, 2**40, 4, 8), myl.MYL_ERR_UNSUPPORTED),
+    ("attention", (4, 2**62, 4, 8), myl.MYL_ERR_UNSUPPORTED), ("attention", (1, 1, 2**62, 8), myl.MYL_ERR_UNSUPPORTED),
+    ("attention", (1, 1, 4, 2**31), myl.MYL_ERR_OVERFLOW), ("attention", (1, 1, 4, 2**63 - 1), myl.MYL_ERR_OVERFLOW),
+    # batch, drafted, vocab
+    ("verify", (2**20, 1024, 40), myl.MYL_ERR_UNSUPPORTED), ("verify", (2**62, 2, 40), myl.MYL_ERR_UNSUPPORTED),
+    ("verify", (1, 2, 2**31), myl.MYL_ERR_UNSUPPORTED), ("verify", (1, 2, 2**62), myl.MYL_ERR_OVERFLOW),
+])
+def test_serving_sizes_beyond_the_limits_are_refused(ctx, entry, sizes, code):
+    """By the C entry points themselves, before anything is launched."""
+    from myelith_b200 import serving
+
+    L, some = serving._lib(), torch.zeros(4096, dtype=torch.int64, device="cuda").data_ptr()
+    if entry == "attention":
+        kv = torch.zeros((2, 8, 64), dtype=torch.int16, device="cuda")
+        plan, prefix = make_plan(ctx, PLAN), myl.Prefix(ctx, kv, kv)
+        batch, T, heads, cap = sizes
+        rc = L.myl_prefix_attention_dev(ctx.handle, plan.handle, prefix.handle, some, batch, T, heads, 256, some, some,
+                                        cap, 1024, 512, 64, some, some, 256, None)
+    else:
+        v = myl.DraftVerifier(ctx, np.array([1], np.int16), 4, 0)  # a weight of one: the sum fits 32 bits longest
+        batch, drafted, vocab = sizes
+        rc = L.myl_verify_dev(ctx.handle, v.handle, some, 0, vocab, some, 0, vocab, batch, drafted, vocab, some, None,
+                              some, some, some, None)
+    assert rc == code
+
+
 # ---- captured in a CUDA graph ------------------------------------------------------------
 
 def test_serving_operators_in_a_graph(ctx):

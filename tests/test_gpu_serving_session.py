@@ -341,3 +341,20 @@ def test_forward_logits_waits_for_the_buffers_last_use(model, own):
     torch.cuda.synchronize()
     assert np.array_equal(out.cpu().numpy(), want)
     assert (read == 7).all()
+
+
+def test_session_sizes_beyond_the_limits_are_refused(model):
+    """Positions and sequences whose products pass 64 bits."""
+    spec, m = model
+    s, _ = prompted(m, spec)
+    for bad, code in ((dict(batch=1, max_new=2**62), myl.MYL_ERR_OVERFLOW), (dict(batch=1, max_new=2**50), myl.MYL_ERR_OVERFLOW),
+                      (dict(batch=65536, max_new=1), myl.MYL_ERR_UNSUPPORTED),
+                      (dict(batch=2**60, max_new=16), myl.MYL_ERR_UNSUPPORTED)):
+        with pytest.raises(myl.MylError) as e:
+            s.fork(**bad)
+        assert e.value.code == code
+    for n in (2**62, 2**50, 2**31):
+        with pytest.raises(myl.MylError) as e:
+            m.session(1, n)
+        assert e.value.code == myl.MYL_ERR_OVERFLOW
+    assert np.array_equal(s.fork(1, 2).decode(2)[0][0], s.decode(2)[0][0])
