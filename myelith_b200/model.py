@@ -384,7 +384,9 @@ class Session:
 
     def set_adapter_ids(self, ids) -> None:
         """Each sequence's adapter (-1: none)."""
-        a = np.ascontiguousarray(np.asarray(ids, np.int32)).reshape(self.batch)
+        from .serving import _array
+
+        a = _array("myl_session_set_adapter_ids", "ids", ids, np.int32).reshape(self.batch)
         _check("myl_session_set_adapter_ids", _lib().myl_session_set_adapter_ids(
             self.model.ctx.handle, self._h, a.ctypes.data))
 
@@ -393,9 +395,9 @@ class Session:
         torch CUDA tensor logits [batch, T, vocab] int32, after what the given
         stream (default: torch's current one) holds; complete on return."""
         from . import MYL_ERR_SHAPE, MylError
-        from .serving import _stream
+        from .serving import _array, _stream
 
-        t = np.ascontiguousarray(np.asarray(tokens, np.int32)).reshape(self.batch, -1)
+        t = _array("myl_forward_logits_dev", "tokens", tokens, np.int32).reshape(self.batch, -1)
         if str(logits.dtype) != "torch.int32" or not logits.is_cuda or not logits.is_contiguous() or \
                 tuple(logits.shape) != (self.batch, t.shape[1], self.model.vocab):
             raise MylError("myl_forward_logits_dev", MYL_ERR_SHAPE,

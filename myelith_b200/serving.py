@@ -67,6 +67,27 @@ def _bad(fn: str, msg: str):
     return MylError(fn, MYL_ERR_SHAPE, msg)
 
 
+def _array(fn: str, what: str, a, dtype) -> np.ndarray:
+    """a as a contiguous array of dtype; values that dtype does not hold are refused, not wrapped."""
+    a = np.asarray(a)
+    c = a.astype(dtype, order="C", copy=False)
+    if a.dtype != c.dtype and not np.array_equal(a, c):
+        from . import MYL_ERR_OVERFLOW, MylError
+
+        raise MylError(fn, MYL_ERR_OVERFLOW, f"{what}: values outside {np.dtype(dtype).name}")
+    return np.ascontiguousarray(c)
+
+
+def _value(fn: str, what: str, v, dtype) -> int:
+    """An integer argument that dtype holds."""
+    info = np.iinfo(dtype)
+    if v != int(v) or not info.min <= v <= info.max:
+        from . import MYL_ERR_OVERFLOW, MylError
+
+        raise MylError(fn, MYL_ERR_OVERFLOW, f"{what} {v}: outside {np.dtype(dtype).name}")
+    return int(v)
+
+
 def _need(fn: str, ctx, what: str, t, dtype: str, dim: int) -> None:
     """A CUDA tensor of the context's device with `dim` dimensions, the last one dense."""
     if not _DTYPES:
@@ -123,10 +144,13 @@ class AttentionPlan(_Handle):
     def __init__(self, ctx, score_mult: int, score_shift: int, exp_lut, lut_shift: int, prob_frac_bits: int,
                  out_shift: int = 0):
         self.ctx = ctx
-        lut = np.ascontiguousarray(np.asarray(exp_lut, np.int16))
+        fn = "myl_attn_plan_create"
+        lut = _array(fn, "exp_lut", exp_lut, np.int16)
         h = C.c_void_p()
-        _check("myl_attn_plan_create", _lib().myl_attn_plan_create(
-            ctx.handle, score_mult, score_shift, lut.ctypes.data, lut.size, lut_shift, prob_frac_bits, out_shift,
+        _check(fn, _lib().myl_attn_plan_create(
+            ctx.handle, _value(fn, "score_mult", score_mult, np.int64), _value(fn, "score_shift", score_shift, np.uint8),
+            lut.ctypes.data, lut.size, _value(fn, "lut_shift", lut_shift, np.uint8),
+            _value(fn, "prob_frac_bits", prob_frac_bits, np.uint8), _value(fn, "out_shift", out_shift, np.int32),
             C.byref(h)))
         self._h = h
 
@@ -196,8 +220,10 @@ class Adapters(_Handle):
     def __init__(self, ctx, A, a_shifts, B, b_shifts, act_frac: int, h_frac: int, out_frac: int):
         self.ctx = ctx
         fn = "myl_adapters_register"
-        A, B = (np.ascontiguousarray(np.asarray(a, np.int8)) for a in (A, B))
-        sa, sb = (np.ascontiguousarray(np.asarray(a, np.uint8)) for a in (a_shifts, b_shifts))
+        A, B = _array(fn, "A", A, np.int8), _array(fn, "B", B, np.int8)
+        sa, sb = _array(fn, "a_shifts", a_shifts, np.uint8), _array(fn, "b_shifts", b_shifts, np.uint8)
+        act_frac, h_frac, out_frac = (_value(fn, n, v, np.uint8) for n, v in (
+            ("act_frac", act_frac), ("h_frac", h_frac), ("out_frac", out_frac)))
         if A.ndim != 3 or B.ndim != 3 or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2] or \
                 sa.shape != A.shape[:2] or sb.shape != B.shape[:2]:
             raise _bad(fn, f"A {A.shape}, a_shifts {sa.shape}, B {B.shape}, b_shifts {sb.shape}")
@@ -238,12 +264,12 @@ class DraftVerifier(_Handle):
 
     def __init__(self, ctx, exp_lut, temp_mult: int, temp_shift: int):
         self.ctx = ctx
-        lut = np.ascontiguousarray(np.asarray(exp_lut, np.int16))
-        if not 0 <= temp_mult < 2**32:
-            raise _bad("myl_verifier_create", f"temp_mult {temp_mult} outside 32 bits")
+        fn = "myl_verifier_create"
+        lut = _array(fn, "exp_lut", exp_lut, np.int16)
         h = C.c_void_p()
-        _check("myl_verifier_create", _lib().myl_verifier_create(
-            ctx.handle, lut.ctypes.data, lut.size, temp_mult, temp_shift, C.byref(h)))
+        _check(fn, _lib().myl_verifier_create(
+            ctx.handle, lut.ctypes.data, lut.size, _value(fn, "temp_mult", temp_mult, np.uint32),
+            _value(fn, "temp_shift", temp_shift, np.uint8), C.byref(h)))
         self._h = h
 
     def verify_dev(self, target, draft, tokens, counts, rand, accepted, out_tokens, stream=None) -> None:

@@ -600,6 +600,35 @@ def test_verify_rejects(ctx):
     ctx.synchronize()
 
 
+@pytest.mark.parametrize("change", [
+    dict(score_shift=256 + 23), dict(score_shift=-233), dict(lut_shift=262), dict(prob_frac=270), dict(out_shift=2**32 - 1),
+    dict(score_mult=2**64 + 2896), dict(score_mult=2896.5), dict(exp_lut=R.EXP_LUT.astype(np.int64) + 2**16),
+])
+def test_plan_values_outside_their_types_are_refused(ctx, change):
+    """Not wrapped into another plan."""
+    with pytest.raises(myl.MylError) as e:
+        make_plan(ctx, {**PLAN, **change})
+    assert e.value.code == myl.MYL_ERR_OVERFLOW
+
+
+def test_adapter_and_verifier_values_outside_their_types_are_refused(ctx):
+    rng = np.random.default_rng(2)
+    p = adapter_problem(rng, 1, 64, 32, 4, 2)
+    good = dict(A=p["A"], a_shifts=p["sa"], B=p["B"], b_shifts=p["sb"], act_frac=8, h_frac=8, out_frac=8)
+    myl.Adapters(ctx, **{**good, "A": p["A"].astype(np.int64), "b_shifts": p["sb"].astype(float)})  # other types are fine
+    for bad in (dict(A=p["A"].astype(np.int64) + 256), dict(B=p["B"] + 0.5), dict(a_shifts=p["sa"].astype(int) - 256),
+                dict(b_shifts=p["sb"].astype(int) + 256), dict(act_frac=264), dict(h_frac=-248), dict(out_frac=264)):
+        with pytest.raises(myl.MylError) as e:
+            myl.Adapters(ctx, **{**good, **bad})
+        assert e.value.code == myl.MYL_ERR_OVERFLOW
+    for mult, shift in ((4, 256), (4, -1), (2**32 + 4, 0), (4.5, 0)):
+        with pytest.raises(myl.MylError) as e:
+            myl.DraftVerifier(ctx, R.EXP_LUT, mult, shift)
+        assert e.value.code == myl.MYL_ERR_OVERFLOW
+    with pytest.raises(myl.MylError):
+        myl.DraftVerifier(ctx, R.EXP_LUT.astype(np.int64) + 2**16, 4, 0)
+
+
 @pytest.mark.parametrize("entry,sizes,code", [
     # batch, T, heads, suffix capacity: products that pass 32 and 64 bits
     ("attention", (65536, 1, 4, 8), myl.MYL_ERR_UNSUPPORTED), ("attention", (2**40, 2**40, 4, 8), myl.MYL_ERR_UNSUPPORTED),

@@ -358,3 +358,16 @@ def test_session_sizes_beyond_the_limits_are_refused(model):
             m.session(1, n)
         assert e.value.code == myl.MYL_ERR_OVERFLOW
     assert np.array_equal(s.fork(1, 2).decode(2)[0][0], s.decode(2)[0][0])
+
+
+def test_ids_and_tokens_outside_32_bits_are_refused(ctx, model):
+    spec, m = model
+    s, _ = prompted(m, spec)
+    l, p, a = adapters(ctx, spec, np.random.default_rng(4))[0]
+    s.set_adapters(l, p, a)
+    with pytest.raises(myl.MylError):
+        s.set_adapter_ids(np.array([0, 2**32], np.int64))
+    with pytest.raises(myl.MylError):
+        s.forward_logits_dev(np.array([[0], [2**32]], np.int64),
+                             torch.zeros((2, 1, spec.vocab), dtype=torch.int32, device="cuda"))
+    assert s.position == 9
