@@ -104,6 +104,12 @@ def _need(fn: str, ctx, what: str, t, dtype: str, dim: int) -> None:
                        f"strides {t.stride()}")
 
 
+def _alike(a, b) -> bool:
+    """Equal strides over the dimensions that have any (longer than one)."""
+    x, y = a.stride(), b.stride()
+    return x == y or all(n <= 1 or i == j for n, i, j in zip(a.shape, x, y))
+
+
 def _stream(ctx, stream) -> int | None:
     """The stream's handle; by default torch's current stream on the context's device."""
     global _current_stream
@@ -166,7 +172,7 @@ class Prefix(_Handle):
         fn = "myl_prefix_create"
         _need(fn, ctx, "k", k, "int16", 3)
         _need(fn, ctx, "v", v, "int16", 3)
-        if k.shape != v.shape or (k.numel() and k.stride() != v.stride()):
+        if k.shape != v.shape or (k.numel() and not _alike(k, v)):
             raise _bad(fn, f"k {tuple(k.shape)} and v {tuple(v.shape)} differ in shape or strides")
         nkv, P, hd = k.shape
         h = C.c_void_p()
@@ -197,7 +203,7 @@ class Prefix(_Handle):
         if B == 0 or T == 0:
             return
         if (T > 1 and B > 1 and (q.stride(0) != T * q.stride(1) or out.stride(0) != T * out.stride(1))) or \
-                (nq > 1 and q.stride(2) != hd) or (S and k_suffix.stride() != v_suffix.stride()) or \
+                (nq > 1 and q.stride(2) != hd) or (S and not _alike(k_suffix, v_suffix)) or \
                 (B > 1 and lens.stride(0) != 1):
             raise _bad(fn, "q and out rows evenly spaced over (B, T) with dense heads, equal suffix strides and dense "
                            "lens are needed")

@@ -600,6 +600,37 @@ def test_verify_rejects(ctx):
     ctx.synchronize()
 
 
+@pytest.mark.parametrize("B,nkv,S", [(1, 2, 10), (3, 1, 10), (2, 2, 1)])
+def test_prefix_attention_takes_any_stride_of_single_entries(ctx, B, nkv, S):
+    """Keys and values whose strides differ in dimensions of length one alone."""
+    rng = np.random.default_rng(15)
+    x = attention_problem(rng, B, 1, 4, nkv, 64, 30, S)
+    big = torch.full((B, 3, nkv, 2, S, 64), 5, dtype=torch.int16, device="cuda")
+    if B == 1:  # another stride of the request
+        ks = big[:, 1, :, 0]
+        vs = torch.zeros((nkv, 2, S, 64), dtype=torch.int16, device="cuda")[None, :, 0]
+    elif nkv == 1:  # of the head
+        ks = big[:, 1, :, 0]
+        vs = torch.zeros((B, 6, S, 64), dtype=torch.int16, device="cuda")[:, :1]
+    else:  # of the position
+        ks = torch.zeros((B, nkv, 1, 64), dtype=torch.int16, device="cuda")
+        vs = torch.zeros((B, nkv, 64), dtype=torch.int16, device="cuda").unsqueeze(2)
+        vs = vs.as_strided(vs.shape, (nkv * 64, 64, 8, 1))
+    assert ks.stride() != vs.stride()
+    ks[:], vs[:] = dev(x["ks"]), dev(x["vs"])
+    # a prefix of one head likewise
+    k, v = dev(x["k"]), dev(x["v"])
+    if nkv == 1:
+        v = v.as_strided(v.shape, (7, 64, 1))
+    lens = np.arange(1, B + 1) % (S + 1)
+    out = torch.full((B, 1, 256), 77, dtype=torch.int16, device="cuda")
+    myl.Prefix(ctx, k, v).attention_dev(make_plan(ctx, PLAN), dev(x["q"]), ks, vs, dev(lens.astype(np.int32)), out)
+    ctx.synchronize()
+    torch.cuda.synchronize()
+    assert np.array_equal(out.cpu().numpy(),
+                          R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **PLAN))
+
+
 @pytest.mark.parametrize("change", [
     dict(score_shift=256 + 23), dict(score_shift=-233), dict(lut_shift=262), dict(prob_frac=270), dict(out_shift=2**32 - 1),
     dict(score_mult=2**64 + 2896), dict(score_mult=2896.5), dict(exp_lut=R.EXP_LUT.astype(np.int64) + 2**16),
