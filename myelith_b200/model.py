@@ -395,13 +395,13 @@ class Session:
         torch CUDA tensor logits [batch, T, vocab] int32, after what the given
         stream (default: torch's current one) holds; complete on return."""
         from . import MYL_ERR_SHAPE, MylError
-        from .serving import _array, _stream
+        from .serving import _array, _need, _stream
 
         t = _array("myl_forward_logits_dev", "tokens", tokens, np.int32).reshape(self.batch, -1)
-        if str(logits.dtype) != "torch.int32" or not logits.is_cuda or not logits.is_contiguous() or \
-                tuple(logits.shape) != (self.batch, t.shape[1], self.model.vocab):
+        _need("myl_forward_logits_dev", self.model.ctx, "logits", logits, "int32", 3)
+        if not logits.is_contiguous() or tuple(logits.shape) != (self.batch, t.shape[1], self.model.vocab):
             raise MylError("myl_forward_logits_dev", MYL_ERR_SHAPE,
-                           f"logits {tuple(logits.shape)} {logits.dtype} for tokens {t.shape}")
+                           f"logits {tuple(logits.shape)} for tokens {t.shape}")
         _check("myl_forward_logits_dev", _lib().myl_forward_logits_dev(
             self.model.ctx.handle, self.model.handle, self._h, t.ctypes.data, t.shape[1], logits.data_ptr(),
             _stream(self.model.ctx, stream)))
