@@ -377,8 +377,13 @@ class Session:
     def set_adapters(self, layer: int, projection: str, adapters) -> None:
         """Low-rank adapters (Adapters, or None) of a layer's "qkv" rows or "o"
         projection; set_adapter_ids chooses each sequence's."""
+        from . import MYL_ERR_SHAPE, MylError
+
+        which = {"qkv": 0, "o": 1}.get(projection)
+        if which is None:
+            raise MylError("myl_session_set_adapters", MYL_ERR_SHAPE, f"projection {projection!r}: qkv or o")
         _check("myl_session_set_adapters", _lib().myl_session_set_adapters(
-            self.model.ctx.handle, self._h, layer, {"qkv": 0, "o": 1}[projection],
+            self.model.ctx.handle, self._h, layer, which,
             None if adapters is None else adapters.handle))
         self._adapters = {**getattr(self, "_adapters", {}), (layer, projection): adapters}
 

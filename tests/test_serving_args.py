@@ -55,3 +55,8 @@ def session(monkeypatch):
 def test_forward_logits_takes_a_tensor_of_its_own_device(session, bad):
     with pytest.raises(myl.MylError):
         session.forward_logits_dev(np.zeros((1, 2), np.int32), Logits(**bad))
+
+
+def test_set_adapters_refuses_an_unknown_projection(session):
+    with pytest.raises(myl.MylError):
+        session.set_adapters(0, "mlp", None)
