@@ -602,7 +602,10 @@ int myl_attention_int(myl_ctx* ctx, const int16_t* q, int64_t q_len, const int16
 
 /* --- Serving many requests that share a prompt ---------------------------------------
  * No counterpart in the reference, which runs one sequence; each operator is
- * composed of its primitives, so every result is one exact integer.
+ * composed of its primitives, so every result is one exact integer. The device
+ * forms may be captured in a CUDA graph once a call of the same size has run (it
+ * sizes the context's workspaces; a larger call may move them, after which the
+ * graph has to be captured again).
  *
  * Attention plan: the constants of attention_int (attention.rs:42-94) and of
  * the rescale to the output projection's input (model.rs:563-567):

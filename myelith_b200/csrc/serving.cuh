@@ -131,11 +131,13 @@ int prefix_build(myl_ctx* ctx, myl_prefix* pf, const int16_t* k, const int16_t* 
   return MYL_OK;
 }
 
-// A workspace of words that every call leaves at zero.
+// A workspace of words that every call leaves at zero. A capture cannot make it:
+// its first zeros would come with the first replay, after calls that need them.
 int zero_kept(DevBuf& b, size_t bytes, cudaStream_t st) {
-  const size_t had = b.cap;
+  if (b.cap >= bytes) return MYL_OK;
+  if (capturing(st)) return fail(MYL_ERR_ARG, "a call of this size has to run once before it is captured");
   TRY(ensure(b, bytes));
-  if (b.cap != had) CUDA_TRY(cudaMemsetAsync(b.p, 0, b.cap, st));
+  CUDA_TRY(cudaMemsetAsync(b.p, 0, b.cap, st));
   return MYL_OK;
 }
 
@@ -175,9 +177,9 @@ int run_prefix_tc(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cudaSt
   const size_t o_sc = a.take<int32_t>(rows * p.lds), o_e = a.take<uint16_t>(int64_t(units) * p.Pp * PTC_ROWS),
                o_part = a.take<int64_t>(int64_t(splits) * units * HD * PTC_ROWS),
                o_sfx = a.take<int32_t>(int64_t(tiles) * rows * HD);
+  TRY(zero_kept(ctx->pfx_stat, size_t(rows) * 8, st));
   TRY(ensure(ctx->pfx, a.off));
   uint8_t* ws = static_cast<uint8_t*>(ctx->pfx.p);
-  TRY(zero_kept(ctx->pfx_stat, size_t(rows) * 8, st));
   p.rowmax = static_cast<unsigned*>(ctx->pfx_stat.p);
   p.rowsum = reinterpret_cast<int32_t*>(p.rowmax + rows);
   p.scores = reinterpret_cast<int32_t*>(ws + o_sc);
@@ -226,10 +228,10 @@ int run_prefix_slice(myl_ctx* ctx, const myl_attn_plan* pl, PrefixParams& p, cud
     return p.hd == 128 ? (pl->wide >= 0 ? run_prefix_tc<128, true>(ctx, pl, p, st) : run_prefix_tc<128, false>(ctx, pl, p, st))
                        : (pl->wide >= 0 ? run_prefix_tc<64, true>(ctx, pl, p, st) : run_prefix_tc<64, false>(ctx, pl, p, st));
   p.lds = p.Pp + ((p.S + 31) & ~31);
-  TRY(ensure(ctx->pfx, size_t(rows) * size_t(p.lds) * 4));
-  p.scores = static_cast<int32_t*>(ctx->pfx.p);
   const size_t o_acc = size_t(rows) * 8;
   TRY(zero_kept(ctx->pfx_stat, o_acc + size_t(rows) * size_t(p.hd) * 8 + size_t(p.nkv) * 4, st));
+  TRY(ensure(ctx->pfx, size_t(rows) * size_t(p.lds) * 4));
+  p.scores = static_cast<int32_t*>(ctx->pfx.p);
   uint8_t* stat = static_cast<uint8_t*>(ctx->pfx_stat.p);
   p.rowmax = reinterpret_cast<unsigned*>(stat);
   p.rowsum = reinterpret_cast<int32_t*>(p.rowmax + rows);

@@ -732,3 +732,45 @@ def test_serving_operators_in_a_graph(ctx):
     ref = R.verify(p["target"], p["draft"], p["tokens"], None, p["rand"], R.EXP_LUT, 4, 0)
     assert np.array_equal(acc.cpu().numpy(), ref[0]) and np.array_equal(toks.cpu().numpy(), ref[1])
     ctx.synchronize()
+
+
+@pytest.mark.parametrize("B", [2, 70])
+def test_first_calls_are_not_captured(B):
+    """The statistics that calls keep at zero have to be zero before the first replay."""
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    rng = np.random.default_rng(30)
+    x, p = attention_problem(rng, B, 2, 4, 2, 64, 565, 6), verify_problem(rng, B, 2, 60)
+    lens = rng.integers(2, 7, size=B)
+    want = R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **PLAN)
+    ver_want = R.verify(p["target"], p["draft"], p["tokens"], None, p["rand"], R.EXP_LUT, 4, 0)
+    c = myl.Context(0)
+    try:
+        plan, prefix, ver = make_plan(c, PLAN), myl.Prefix(c, dev(x["k"]), dev(x["v"])), myl.DraftVerifier(c, R.EXP_LUT, 4, 0)
+        a = [dev(x[n]) for n in ("q", "ks", "vs")] + [dev(lens.astype(np.int32))]
+        v = [dev(p[n]) for n in ("target", "draft", "tokens")] + [None, dev(p["rand"])]
+        out = torch.zeros((B, 2, 256), dtype=torch.int16, device="cuda")
+        acc, toks = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in ((B,), (B, 3)))
+        calls = [lambda: prefix.attention_dev(plan, *a, out), lambda: ver.verify_dev(*v, acc, toks)]
+        torch.cuda.synchronize()
+        for call in calls:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, capture_error_mode="relaxed"):  # a mode that lets a capture allocate
+                with pytest.raises(myl.MylError) as e:
+                    call()
+            assert e.value.code == myl.MYL_ERR_ARG
+        g = torch.cuda.CUDAGraph()
+        for repeat in range(2):  # eagerly, then captured and replayed
+            out.zero_(), acc.zero_(), toks.zero_()
+            if repeat:
+                with torch.cuda.graph(g):
+                    [call() for call in calls]
+                g.replay()
+            else:
+                [call() for call in calls]
+            torch.cuda.synchronize()
+            assert np.array_equal(out.cpu().numpy(), want)
+            assert np.array_equal(acc.cpu().numpy(), ver_want[0]) and np.array_equal(toks.cpu().numpy(), ver_want[1])
+        c.synchronize()
+    finally:
+        c.close()
