@@ -774,3 +774,146 @@ def test_first_calls_are_not_captured(B):
         c.synchronize()
     finally:
         c.close()
+
+
+# ---- many rows, streams that take turns, replays ---------------------------------------------
+
+
+def runs_of(rng, M, num, length):
+    """Adapter ids in runs of `length` rows, neighbouring runs of different adapters, some of none."""
+    ids = (np.arange(M) // length) % (num + 1) - 1
+    return np.roll(ids, int(rng.integers(0, M)))
+
+
+@pytest.mark.parametrize("M", [512, 513, 529, 1040])  # both sides of the decode form, ragged tiles
+@pytest.mark.parametrize("K,N,r", [(96, 64, 1), (203, 77, 17), (512, 264, 64), (130, 40, 256)])
+def test_linear_adapters_many_rows(ctx, M, K, N, r):
+    """Tiles of 16 rows with one, four, five and sixteen adapters in them."""
+    rng = np.random.default_rng(M + K)
+    p = adapter_problem(rng, M, K, N, r, 20)
+    for length in (100, 4, 3, 1):
+        ids = runs_of(rng, M, 20, length)
+        got = run_adapters(ctx, p, ids)
+        ctx.synchronize()
+        assert np.array_equal(got, adapter_ref(p, ids)), length
+
+
+@pytest.mark.parametrize("length", [60, 1])
+def test_linear_adapters_many_rows_extremes(ctx, length):
+    """Saturated rows, -128 weights, shifts of zero, to the left and beyond 30, ids outside the adapters."""
+    M, N = 530, 48
+    rng = np.random.default_rng(length)
+    p = adapter_problem(rng, M, 96, N, 16, 3, full=True)
+    p["x"][::7], p["x"][3::7] = 32767, -32768
+    p["A"][1], p["A"][2], p["B"][1, ::2], p["B"][2, 1::2] = 127, -128, -128, 127
+    ids = runs_of(rng, M, 3, length)
+    bias = (rng.integers(-30000, 30000, size=N).astype(np.int16), rng.integers(6, 10, size=N).astype(np.uint8))
+    assert np.array_equal(run_adapters(ctx, p, ids, bias=bias), adapter_ref(p, ids, bias=bias))
+    p["sb"][0, 3], p["sb"][1, 9] = 0, 40  # one lane's shifts of several kinds
+    assert np.array_equal(run_adapters(ctx, p, ids), adapter_ref(p, ids))
+    p["sa"][:], p["sb"][:] = 0, 0
+    for fr in ((8, 8, 8), (0, 6, 12), (20, 3, 3), (62, 0, 0), (0, 0, 40), (0, 35, 0)):
+        assert np.array_equal(run_adapters(ctx, p, ids, fr), adapter_ref(p, ids, fr)), fr
+    odd = ids.copy()
+    odd[::31], odd[5::31] = 3, -2
+    got = run_adapters(ctx, p, odd)
+    with pytest.raises(myl.MylError) as e:
+        ctx.synchronize()
+    assert e.value.code == DEVICE_ERR
+    assert np.array_equal(got, adapter_ref(p, np.where((odd >= 0) & (odd < 3), odd, -1)))
+
+
+@pytest.mark.parametrize("N", [90, 96])
+@pytest.mark.parametrize("length", [50, 2])
+def test_linear_adapters_many_rows_strides(ctx, N, length):
+    M, K = 517, 203
+    rng = np.random.default_rng(N + length)
+    p = adapter_problem(rng, M, K, N, 8, 4)
+    ids = runs_of(rng, M, 4, length)
+    ref = adapter_ref(p, ids)
+    for lead, pad in ((1, 5), (0, 5), (8, 13)):  # off 16-byte boundaries, odd row strides, rows on boundaries
+        xs = torch.full((M, K + lead + pad), 3, dtype=torch.int16, device="cuda")
+        xs[:, lead:lead + K] = dev(p["x"])
+        ys = torch.full((M, (N + lead + pad + 7) // 8 * 8 + (0 if lead == 8 else 1)), 77, dtype=torch.int16, device="cuda")
+        got = run_adapters(ctx, p, ids, x=xs[:, lead:lead + K], y=ys[:, lead:lead + N])
+        assert np.array_equal(got, ref)
+        assert (ys[:, :lead] == 77).all() and (ys[:, lead + N:] == 77).all()
+
+
+@pytest.mark.parametrize("B,T,nq,nkv,hd,P,S", [
+    (64, 1, 28, 4, 128, 300, 512), (16, 5, 28, 4, 128, 500, 260), (70, 2, 14, 2, 64, 511, 130), (3, 90, 4, 2, 64, 40, 300),
+    (40, 1, 6, 2, 48, 700, 200),  # a head size of the other kernels
+])
+def test_prefix_attention_many_rows_over_a_short_prefix(ctx, B, T, nq, nkv, hd, P, S):
+    rng = np.random.default_rng(B + P)
+    x = attention_problem(rng, B, T, nq, nkv, hd, P, S)
+    lens = rng.integers(0, S + 1, size=B)
+    lens[0], lens[1] = S, T - 1
+    check_attention(ctx, x, lens)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("S", [0, 6, 300])
+def test_many_row_attention_replayed(ctx, hd, S):
+    """The chain of kernels for many rows captured once; queries and lengths change between replays."""
+    rng = np.random.default_rng(hd + S)
+    B, T, nq, nkv, P = 70, 2, 4, 2, 565
+    plan = make_plan(ctx, PLAN)
+    x = attention_problem(rng, B, T, nq, nkv, hd, P, S)
+    prefix, ks, vs = myl.Prefix(ctx, dev(x["k"]), dev(x["v"])), dev(x["ks"]), dev(x["vs"])
+    q, lens = torch.zeros((B, T, nq, hd), dtype=torch.int16, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    out = torch.zeros((B, T, nq * hd), dtype=torch.int16, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        prefix.attention_dev(plan, q, ks, vs, lens, out)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        prefix.attention_dev(plan, q, ks, vs, lens, out)
+        prefix.attention_dev(plan, q, ks, vs, lens, out)  # the second finds the first's statistics at zero
+    for _ in range(4):
+        qn, ln = int16s(rng, (B, T, nq, hd), 3000.0), rng.integers(0, S + 1, size=B).astype(np.int32)
+        q.copy_(dev(qn)), lens.copy_(dev(ln))
+        g.replay(), g.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(out.cpu().numpy(), R.prefix_attention(qn, x["k"], x["v"], x["ks"], x["vs"], ln, **PLAN))
+    ctx.synchronize()
+
+
+def test_streams_take_turns_on_the_workspaces(ctx):
+    """Calls of every operator, of both sizes of attention, queued on two streams without a wait between them."""
+    rng = np.random.default_rng(31)
+    plan, jobs = make_plan(ctx, PLAN), []
+    for B, P in ((3, 150), (70, 565), (2, 40), (66, 700)):
+        x = attention_problem(rng, B, 2, 4, 2, 64, P, 9)
+        lens = rng.integers(2, 10, size=B).astype(np.int32)
+        prefix = myl.Prefix(ctx, dev(x["k"]), dev(x["v"]))
+        a = [dev(x[n]) for n in ("q", "ks", "vs")] + [dev(lens)]
+        jobs.append((lambda o, f=prefix, a=a: f.attention_dev(plan, *a, o[0]), [((B, 2, 256), torch.int16)],
+                     [R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **PLAN)]))
+    ver = myl.DraftVerifier(ctx, R.EXP_LUT, 4, 0)
+    for B, D, V in ((5, 3, 3000), (40, 1, 97)):
+        p = verify_problem(rng, B, D, V)
+        v = [dev(p[n]) for n in ("target", "draft", "tokens")] + [None, dev(p["rand"])]
+        jobs.append((lambda o, v=v: ver.verify_dev(*v, *o), [((B,), torch.int32), ((B, D + 1), torch.int32)],
+                     R.verify(p["target"], p["draft"], p["tokens"], None, p["rand"], R.EXP_LUT, 4, 0)))
+    for M in (5, 600):
+        p = adapter_problem(rng, M, 256, 64, 8, 3)
+        ids = rng.integers(-1, 3, size=M).astype(np.int32)
+        w = myl.Weight(ctx, p["W"], 256, p["ws"])
+        rq, ad = w.requant(myl.RQ_SHIFT_I16, 8, 8), myl.Adapters(ctx, p["A"], p["sa"], p["B"], p["sb"], 8, 8, 8)
+        a = [rq, ad, dev(p["x"]), dev(ids)]
+        jobs.append((lambda o, w=w, a=a: w.linear_adapters_dev(*a, o[0]), [((M, 64), torch.int16)], [adapter_ref(p, ids)]))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    order = [int(i) for i in rng.permutation(np.repeat(np.arange(len(jobs)), 6))]
+    outs = [[torch.full(s, 77, dtype=t, device="cuda") for s, t in jobs[i][1]] for i in order]
+    torch.cuda.synchronize()
+    for n, (i, o) in enumerate(zip(order, outs)):
+        with torch.cuda.stream(streams[n % 2]):
+            jobs[i][0](o)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    for i, o in zip(order, outs):
+        for got, want in zip(o, jobs[i][2]):
+            assert np.array_equal(got.cpu().numpy(), want), i

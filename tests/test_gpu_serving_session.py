@@ -371,3 +371,25 @@ def test_ids_and_tokens_outside_32_bits_are_refused(ctx, model):
         s.forward_logits_dev(np.array([[0], [2**32]], np.int64),
                              torch.zeros((2, 1, spec.vocab), dtype=torch.int32, device="cuda"))
     assert s.position == 9
+
+
+def test_fork_of_many_sequences_decodes_by_replays(model):
+    """Enough sequences for the many-row attention in the captured step, a workspace that moves between decodes."""
+    spec, m = model
+    P, B = 600, 60
+    prompt = S.prompt_tokens(spec.vocab, P, seed=3)
+    tokens = np.random.default_rng(5).integers(0, spec.vocab, size=(B, 3)).astype(np.int32)
+    plain, parent = m.session(B, P + 40), m.session(1, P)
+    plain.forward(np.tile(prompt, (B, 1)))
+    parent.forward(prompt[None])
+    fork, larger = parent.fork(B, 40), parent.fork(2 * B, 60)
+    assert np.array_equal(plain.forward(tokens), fork.forward(tokens))
+    a, b = plain.decode(6, keep_logits=True), fork.decode(6, keep_logits=True)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[2], b[2])
+    c, d = plain.decode(5)[0], fork.decode(5)[0]  # captured
+    assert np.array_equal(c, d)
+    larger.forward(np.tile(tokens, (2, 1)))
+    both = larger.decode(11)[0]
+    for half in (both[:B], both[B:]):
+        assert np.array_equal(half, np.concatenate((a[0], c), 1))
+    assert np.array_equal(plain.decode(5)[0], fork.decode(5)[0])
