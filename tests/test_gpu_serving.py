@@ -917,3 +917,81 @@ def test_streams_take_turns_on_the_workspaces(ctx):
     for i, o in zip(order, outs):
         for got, want in zip(o, jobs[i][2]):
             assert np.array_equal(got.cpu().numpy(), want), i
+
+
+# ---- long prefixes, offsets past 32 bits --------------------------------------------------
+
+
+@pytest.mark.parametrize("hd,P", [(64, 130900), (128, 65537)])
+def test_long_prefix_batch_equals_single_requests(ctx, hd, P):
+    """Near the most keys that the table allows: the many-row kernels against those for few rows."""
+    rng = np.random.default_rng(P)
+    B, nq, nkv, S = 24, 4, 2, 40
+    x = attention_problem(rng, B, 1, nq, nkv, hd, P, S)
+    lens = rng.integers(1, S + 1, size=B)
+    got = run_attention(ctx, x, lens, PLAN)
+    for b in range(0, B, 5):
+        one = {**x, "q": x["q"][b:b + 1], "ks": x["ks"][b:b + 1], "vs": x["vs"][b:b + 1]}
+        assert np.array_equal(run_attention(ctx, one, lens[b:b + 1], PLAN)[0], got[b])
+    assert np.array_equal(got[:1], R.prefix_attention(x["q"][:1], x["k"], x["v"], x["ks"][:1], x["vs"][:1], lens[:1],
+                                                      **PLAN))
+
+
+@pytest.mark.parametrize("lut", [[32767], [32767, 32767, 32766, 3]])
+def test_prefix_attention_of_sums_beyond_2_to_30(ctx, lut):
+    """Row sums above 2^30, where twice the sum passes 31 bits, on both kinds of kernels."""
+    rng = np.random.default_rng(len(lut))
+    c = {**PLAN, "exp_lut": np.array(lut, np.int16), "prob_frac": 15, "lut_shift": 8}
+    for B in (1, 12):
+        x = attention_problem(rng, B, 1, 4, 2, 64, 45000, 9)
+        check_attention(ctx, x, rng.integers(1, 10, size=B), c)
+
+
+def far_apart(t, dim, gap):
+    """The values of t in a tensor whose stride in `dim` is `gap` elements."""
+    strides, step = [0] * t.dim(), 1
+    for d in reversed(range(t.dim())):
+        if d != dim:
+            strides[d] = step
+            step *= t.shape[d]
+    strides[dim] = gap
+    assert step <= gap
+    flat = torch.empty(gap * (t.shape[dim] - 1) + step, dtype=t.dtype, device="cuda")
+    out = flat.as_strided(t.shape, strides)
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("B,dim", [(2, 0), (2, 1), (2, 2), (70, 1)])
+def test_attention_offsets_past_32_bits(ctx, B, dim):
+    """Suffix caches whose requests, heads or positions lie more than 2^31 elements apart."""
+    rng = np.random.default_rng(B + dim)
+    x = attention_problem(rng, B, 1, 4, 2, 64, 600, 2)
+    lens = rng.integers(1, 3, size=B)
+    ks, vs = (far_apart(dev(x[n]), dim, 2**31 + 64) for n in ("ks", "vs"))
+    out = torch.full((B, 1, 256), 77, dtype=torch.int16, device="cuda")
+    myl.Prefix(ctx, dev(x["k"]), dev(x["v"])).attention_dev(make_plan(ctx, PLAN), dev(x["q"]), ks, vs,
+                                                            dev(lens.astype(np.int32)), out)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    assert np.array_equal(out.cpu().numpy(),
+                          R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **PLAN))
+    del ks, vs
+    torch.cuda.empty_cache()
+
+
+def test_adapter_and_verify_offsets_past_32_bits(ctx):
+    rng = np.random.default_rng(40)
+    p = adapter_problem(rng, 2, 200, 90, 8, 3)
+    x = far_apart(dev(p["x"]), 0, 2**31 + 8)
+    y = far_apart(torch.zeros((2, 90), dtype=torch.int16, device="cuda"), 0, 2**31 + 8)
+    assert np.array_equal(run_adapters(ctx, p, [2, 0], x=x, y=y), adapter_ref(p, [2, 0]))
+    del x, y
+    for V in (700, 20001):
+        v = verify_problem(rng, 2, 2, V)
+        ref = R.verify(v["target"], v["draft"], v["tokens"], None, v["rand"], R.EXP_LUT, 4, 0)
+        got = run_verify(ctx, v, target=far_apart(dev(v["target"]), 0, 2**31 + 5), draft=dev(v["draft"]))
+        assert np.array_equal(got[0], ref[0]) and np.array_equal(got[1], ref[1])
+        got = run_verify(ctx, v, draft=far_apart(dev(v["draft"]), 1, 2**31 + 5))
+        assert np.array_equal(got[0], ref[0]) and np.array_equal(got[1], ref[1])
+        torch.cuda.empty_cache()
