@@ -605,7 +605,8 @@ int myl_attention_int(myl_ctx* ctx, const int16_t* q, int64_t q_len, const int16
  * composed of its primitives, so every result is one exact integer. The device
  * forms may be captured in a CUDA graph once a call of the same size has run (it
  * sizes the context's workspaces; a larger call may move them, after which the
- * graph has to be captured again).
+ * graph has to be captured again). Replays share the workspaces with the context's
+ * other calls: the caller orders them.
  *
  * Attention plan: the constants of attention_int (attention.rs:42-94) and of
  * the rescale to the output projection's input (model.rs:563-567):
@@ -687,7 +688,8 @@ int myl_linear_adapters_dev(myl_ctx* ctx, const myl_weight* w, const myl_requant
  * tokens, the drawn one, then -1. Logits are device int32, row (b, i) at
  * b * seq_stride + i * pos_stride (target: drafted + 1 rows, draft: drafted);
  * tokens [batch][drafted], counts [batch] (NULL: drafted), rand
- * [batch][drafted + 1], out_tokens [batch][drafted + 1] contiguous. A drafted
+ * [batch][drafted + 1], out_tokens [batch][drafted + 1] contiguous; the outputs
+ * overlap none of the inputs. A drafted
  * token outside the vocabulary counts as having no weight, a count outside
  * [0, drafted] is clamped; both are reported as MYL_ERR_DEVICE at the next
  * synchronising call. Limits: vocab times the largest table entry below 2^32,
@@ -702,14 +704,15 @@ int myl_verify_dev(myl_ctx* ctx, const myl_verifier* verifier, const int32_t* ta
                    int64_t drafted, int64_t vocab, const int32_t* tokens, const int32_t* counts,
                    const uint64_t* rand, int32_t* accepted, int32_t* out_tokens, void* stream);
 
-/* Sessions of a served model (world 1). myl_session_fork: `batch` sequences that
+/* Sessions of a served model (world 1). The sequences of a session share one
+ * position: they advance, and are rewound, together. myl_session_fork: `batch` sequences that
  * continue sequence `seq` of `parent`, each for up to max_new more positions.
  * The parent's positions become a shared prefix (laid out once; the parent may
  * go on or be released) and the parent's last logits every sequence's, so that
  * myl_decode_greedy can follow at once, also after myl_session_reset or a rewind to
  * the prefix's end (a parent that was itself rewound has no logits to give: the
  * fork needs a forward first); results equal separate sessions that hold the
- * prompt each. head_dim a multiple of 8 up to 248, prob_frac_bits <= 15; no
+ * prompt each. A fork starts without adapters. head_dim a multiple of 8 up to 248, prob_frac_bits <= 15; no
  * fork of a fork. */
 int myl_session_fork(myl_ctx* ctx, const myl_model* model, const myl_session* parent, int64_t seq,
                      int64_t batch, int64_t max_new, myl_session** out);

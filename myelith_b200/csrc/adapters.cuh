@@ -27,7 +27,7 @@ struct AdapterParams {
   int ldb;
   const int32_t* ids;  // [M]
   int64_t M;
-  int16_t* h;  // [M][ldb], columns rank..ldb-1 zero
+  int16_t* h;  // [M][ldb]; columns rank..ldb-1 and rows without an adapter hold anything
   int* err;
 };
 
@@ -85,7 +85,8 @@ __device__ __forceinline__ void adapter_planes(const int16_t* row, int64_t k, in
 // h: block = 8 TOK rows x 16 RK rank rows, its WARPS warps share the K axis.
 // <1, 1, 16> spreads few rows over many warps; <2, 2, 8> reads x and A half as
 // often (a K step's operands serve four MMA tiles). A warp's share of K is at most
-// 32768 (AD_MAX_K), so its sums stay inside int32: 2^15 * 2^7 * 2^8.
+// 32768 (AD_MAX_K), so its sums stay inside int32: 2^15 * 2^7 * 2^8. Two blocks an
+// SM leave <1, 1, 16> 64 registers a thread, of which it spills 11.
 constexpr int64_t AD_MAX_K = 8 * 32768;
 template <int TOK, int RK, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, 2)
@@ -177,7 +178,7 @@ __device__ __forceinline__ int32_t adapter_add(int32_t y, int acc, int s) {
 // y += clamp16(rescale(B_a[n] . h[m])), |B . h| <= 256 * 2^7 * 2^15 in int32.
 constexpr int AD_ETHREADS = 256;
 
-// One output: y[m][n] of a row with adapter a.
+// One output: y[m][n] of a row with adapter a (h past the rank meets zero weights).
 __device__ __forceinline__ void adapter_one(const AdapterParams& p, int16_t* y, int64_t m, int64_t n, int a) {
   const int16_t y0 = *y;
   const int s = p.sb[int64_t(a) * p.N + n];

@@ -153,7 +153,9 @@ __global__ void __launch_bounds__(256)
 // dot = 256 sum q*kh + sum q*kl, both exact in int32 for hd <= 248.
 // Blocks x < nbp work on the prefix (grid.y: kv head and row group); the rest
 // on a suffix tile of request b = (x - nbp) / tiles (grid.y: kv head and row
-// group of that request's T * G rows).
+// group of that request's T * G rows). The grid is sized for the R rows of the
+// prefix: of a suffix tile's ceil(R / 8) row groups ceil(T G / 8) have rows, one of
+// 7 for 8 requests of 28/4 heads, one of 56 for 64, and the others leave at once.
 template <bool SUFFIX>
 __device__ __forceinline__ void prefix_scores_block(const PrefixParams& p, int g, int row0, int nrow, int b,
                                                     int j0, int nkeys, int n_b, int16_t* s_q,

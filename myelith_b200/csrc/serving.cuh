@@ -76,7 +76,12 @@ void free_handle(myl_ctx* ctx, T* h) {
 // kernels / tensor cores; R rows per KV head, nkv heads, P positions):
 //   R 14, 4 heads, 2048: 22 / 25    R 28, 4, 2048: 29 / 27    R 56, 4, 500: 27 / 25
 //   R 7, 4 heads, 8192: 28 / 34     R 7, 4, 32749: 69 / 63    R 7, 2, 32749: 40 / 46
-//   R 105, 2 heads, 300: 20 / 25
+// Below 512 positions it sends every call to the few-row kernels, which is right
+// for few rows and short suffixes alone (S suffix positions; R 56, 4 heads, 100 + 64:
+// 20 / 24, 300 + 64: 24 / 23; R 112, 2 heads, 511 + 64: 21 / 23) and costs many rows a
+// lot (R 112, 4 heads, 300 + 512: 51 / 32; R 448, 4 heads, 300 + 64: 84 / 34, 300 +
+// 512: 315 / 45; R 2240, 4 heads, 511 + 512: 1524 / 124), most of it in blocks of the
+// suffix part that find no row (prefix_scores_kernel).
 bool prefix_on_tensor_cores(const PrefixParams& p) {
   return p.P >= 512 && int64_t(p.R) * p.R * p.nkv * p.P >= int64_t(1) << 22;
 }
@@ -357,9 +362,12 @@ int run_verify(myl_ctx* ctx, VerifyParams& p, cudaStream_t st) {
   const int64_t units = int64_t(p.B) * (p.D + 1);
   const int64_t logit_bytes = p.draft ? 4 : 2;
   // Slices of at most 40 KB, so that four CTAs share an SM and some load while
-  // others sweep; smaller ones as long as the SMs hold the CTAs at once (us with 4,
-  // 8, 16 CTAs a position: 5 positions of 151936 30 / 20 / 14; 80 of 32000 17 / 13
-  // / 19; 384 of 32000 32 / 37 / 66; 384 of 152064 without draft logits 84 / 59 / 78).
+  // others sweep; smaller ones up to one and a half times the CTAs that the SMs hold
+  // at once, four each (us with 4, 8, 16 CTAs a position: 5 positions of 151936 30 /
+  // 20 / 14; 37 of 152064 without draft logits 29 / 21 / 19, 52 40 / 28 / 25, 74 41 /
+  // 28 / 29, 80 49 / 33 / 32; 52 with draft logits 51 / 35 / 29; 40 of 32000 12 / 11 /
+  // 15; 80 of 32000 17 / 13 / 19; 384 of 32000 32 / 37 / 66; 384 of 152064 without
+  // draft logits 84 / 59 / 78).
   int cl = 1;
   while (cl < VERIFY_MAX_CL && p.V * logit_bytes > int64_t(cl) * 40 * 1024) cl *= 2;
   while (cl < VERIFY_MAX_CL && 2 * units * cl <= 6 * int64_t(ctx->num_sms) && p.V >= cl * 4096) cl *= 2;

@@ -88,7 +88,7 @@ __device__ __forceinline__ int verify_count(const VerifyParams& p, int b) {
 // Positions past the drafted ones are not read. The last position of a request to
 // finish (a counter per request) writes its output. (Clusters that stay and take
 // positions in turn were slower, 132 us: the hardware spreads uneven positions
-// better.)
+// better.) Four CTAs an SM leave 64 registers a thread, of which 6 spill.
 struct VerifyShared {
   int32_t mx[2][VERIFY_MAX_CL];              // slice maxima by CTA: target, draft
   unsigned long long sum[2][VERIFY_MAX_CL];  // slice weight sums

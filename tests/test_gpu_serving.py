@@ -734,6 +734,7 @@ def test_serving_operators_in_a_graph(ctx):
     ctx.synchronize()
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 @pytest.mark.parametrize("B", [2, 70])
 def test_first_calls_are_not_captured(B):
     """The statistics that calls keep at zero have to be zero before the first replay."""
