@@ -153,11 +153,20 @@ int dev_alloc(std::vector<void*>& list, T** p, size_t count) {
   return MYL_OK;
 }
 
+// cudaMemset and cudaMemcpy work on the default stream, behind whatever is queued
+// there, and may return before they are done; the context's stream and most
+// callers' do not wait for that stream by themselves.
+int uploads_done() {
+  CUDA_TRY(cudaStreamSynchronize(nullptr));
+  return MYL_OK;
+}
+
 template <typename T>
 int dev_upload(std::vector<void*>& list, T** p, const T* host, size_t count) {
   TRY(dev_alloc(list, p, count));
-  if (count) CUDA_TRY(cudaMemcpy(*p, host, count * sizeof(T), cudaMemcpyHostToDevice));
-  return MYL_OK;
+  if (!count) return MYL_OK;
+  CUDA_TRY(cudaMemcpy(*p, host, count * sizeof(T), cudaMemcpyHostToDevice));
+  return uploads_done();
 }
 
 // i8 difference and width checks of rescale (width 32) / rescale_i64 (64),
@@ -371,7 +380,7 @@ int session_alloc(myl_ctx* ctx, myl_session* s) {
   CUDA_TRY(cudaMallocHost(&s->h_tokens, size_t(R) * 4));
   CUDA_TRY(cudaMallocHost(&s->h_logits, size_t(B * m->V) * 4));
   (void)ctx;
-  return MYL_OK;
+  return uploads_done();
 }
 
 void release_session(myl_ctx* ctx, myl_session* s) {

@@ -567,7 +567,7 @@ int myl_session_set_adapters(myl_ctx* ctx, myl_session* s, int64_t layer, int pr
   if (!s->d_row_ids) {
     TRY(dev_alloc(s->allocs, &s->d_seq_ids, size_t(s->B)));
     TRY(dev_alloc(s->allocs, &s->d_row_ids, size_t(s->rows_cap)));
-    CUDA_TRY(cudaMemset(s->d_seq_ids, 0xFF, size_t(s->B) * 4));  // -1: none
+    CUDA_TRY(cudaMemsetAsync(s->d_seq_ids, 0xFF, size_t(s->B) * 4, ctx->stream));  // -1: none
   }
   try {
     std::vector<const myl_adapters*>& list = o ? s->ad_o : s->ad_qkv;
@@ -594,8 +594,9 @@ int myl_session_set_adapter_ids(myl_ctx* ctx, myl_session* s, const int32_t* ids
     if (ids[b] < -1 || ids[b] >= num) return fail(MYL_ERR_SHAPE, "adapter id %d", ids[b]);
   }
   CUDA_TRY(cudaSetDevice(ctx->device));
+  // in the order of the session's steps; the caller's array is free on return
+  CUDA_TRY(cudaMemcpyAsync(s->d_seq_ids, ids, size_t(s->B) * 4, cudaMemcpyHostToDevice, ctx->stream));
   CUDA_TRY(cudaStreamSynchronize(ctx->stream));
-  CUDA_TRY(cudaMemcpy(s->d_seq_ids, ids, size_t(s->B) * 4, cudaMemcpyHostToDevice));
   return MYL_OK;
 }
 
@@ -787,7 +788,7 @@ int myl_adapters_register(myl_ctx* ctx, int64_t num, int64_t rank, int64_t in_fe
   int rc = upload(&ad->A, A, num * rank, in_features, ad->lda);
   if (rc == MYL_OK) rc = upload(&ad->B, B, num * out_features, rank, ad->ldb);
   if (rc == MYL_OK) rc = dev_upload(ad->allocs, &ad->sa, sa.data(), sa.size());
-  if (rc == MYL_OK) rc = dev_upload(ad->allocs, &ad->sb, sb.data(), sb.size());
+  if (rc == MYL_OK) rc = dev_upload(ad->allocs, &ad->sb, sb.data(), sb.size());  // waits for all four
   if (rc != MYL_OK) {
     free_handle(ctx, ad);
     return rc;
@@ -857,6 +858,7 @@ int myl_verifier_create(myl_ctx* ctx, const int16_t* exp_lut, int64_t exp_len, u
   if (rc == MYL_OK && (cudaMemcpy(v->d_lut, exp_lut, size_t(v->len) * 2, cudaMemcpyHostToDevice) != cudaSuccess ||
                        cudaMemset(v->d_lut + v->len, 0, 2) != cudaSuccess))
     rc = fail(MYL_ERR_CUDA, "exp table upload");
+  if (rc == MYL_OK) rc = uploads_done();
   if (rc != MYL_OK) {
     free_handle(ctx, v);
     return rc;

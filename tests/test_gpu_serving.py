@@ -996,3 +996,31 @@ def test_adapter_and_verify_offsets_past_32_bits(ctx):
         got = run_verify(ctx, v, draft=far_apart(dev(v["draft"]), 1, 2**31 + 5))
         assert np.array_equal(got[0], ref[0]) and np.array_equal(got[1], ref[1])
         torch.cuda.empty_cache()
+
+
+def test_plans_are_uploaded_when_their_calls_return(ctx):
+    """Plans, adapters and verifiers made while the default stream is busy, used on another at once."""
+    rng = np.random.default_rng(41)
+    x, lens = attention_problem(rng, 2, 1, 4, 2, 64, 30, 8), [3, 8]
+    v, a, ids = verify_problem(rng, 3, 2, 500), adapter_problem(rng, 6, 256, 64, 8, 3), [0, 1, -1, 2, 2, 0]
+    q, ks, vs, n = dev(x["q"]), dev(x["ks"]), dev(x["vs"]), dev(np.array(lens, np.int32))
+    prefix = myl.Prefix(ctx, dev(x["k"]), dev(x["v"]))
+    t, d, tok, rand = dev(v["target"]), dev(v["draft"]), dev(v["tokens"]), dev(v["rand"])
+    w = myl.Weight(ctx, a["W"], 256, a["ws"])
+    rq, ax, ai = w.requant(myl.RQ_SHIFT_I16, 8, 8), dev(a["x"]), dev(np.array(ids, np.int32))
+    out, y = torch.zeros((2, 1, 256), dtype=torch.int16, device="cuda"), torch.zeros((6, 64), dtype=torch.int16, device="cuda")
+    acc, toks = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((3,), (3, 3)))
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    plan, ad = make_plan(ctx, PLAN), myl.Adapters(ctx, a["A"], a["sa"], a["B"], a["sb"], 8, 8, 8)
+    ver = myl.DraftVerifier(ctx, R.EXP_LUT, 4, 0)
+    prefix.attention_dev(plan, q, ks, vs, n, out, stream=s)
+    w.linear_adapters_dev(rq, ad, ax, ai, y, stream=s)
+    ver.verify_dev(t, d, tok, None, rand, acc, toks, stream=s)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    assert np.array_equal(out.cpu().numpy(), R.prefix_attention(x["q"], x["k"], x["v"], x["ks"], x["vs"], lens, **PLAN))
+    assert np.array_equal(y.cpu().numpy(), adapter_ref(a, ids))
+    ref = R.verify(v["target"], v["draft"], v["tokens"], None, v["rand"], R.EXP_LUT, 4, 0)
+    assert np.array_equal(acc.cpu().numpy(), ref[0]) and np.array_equal(toks.cpu().numpy(), ref[1])

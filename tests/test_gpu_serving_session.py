@@ -393,3 +393,48 @@ def test_fork_of_many_sequences_decodes_by_replays(model):
     for half in (both[:B], both[B:]):
         assert np.array_equal(half, np.concatenate((a[0], c), 1))
     assert np.array_equal(plain.decode(5)[0], fork.decode(5)[0])
+
+
+# ---- work that is still queued on the default stream ----------------------------------------
+
+
+def queue_work():
+    torch.cuda._sleep(100_000_000)  # about 50 ms
+
+
+def test_sessions_are_ready_while_the_default_stream_is_busy(ctx, model):
+    """What a session, its fork and its adapters start from is in place when the calls return."""
+    spec, m = model
+    rng = np.random.default_rng(6)
+    tokens = rng.integers(0, spec.vocab, size=(2, 3)).astype(np.int32)
+    plain, prompt = prompted(m, spec)
+    want = plain.forward(tokens), plain.decode(5)[0]
+    ads = adapters(ctx, spec, rng)
+    torch.cuda.synchronize()
+
+    def same(s):
+        assert np.array_equal(s.forward(tokens), want[0]) and np.array_equal(s.decode(5)[0], want[1])
+
+    queue_work()
+    s, _ = prompted(m, spec)
+    same(s)
+    parent = m.session(1, 20)
+    parent.forward(prompt[None])
+    queue_work()
+    same(parent.fork(2, 20))
+    s, _ = prompted(m, spec)
+    queue_work()
+    for l, p, a in ads:  # every sequence without an adapter until ids are set
+        s.set_adapters(l, p, a)
+    same(s)
+    # ids that follow at once
+    ids = [1, -1]
+    ref, late = (parent.fork(2, 20) for _ in range(2))
+    for l, p, a in ads:
+        ref.set_adapters(l, p, a), late.set_adapters(l, p, a)
+    ref.set_adapter_ids(ids)
+    a = ref.forward(tokens)
+    queue_work()
+    late.set_adapter_ids(ids)
+    assert np.array_equal(late.forward(tokens), a)
+    torch.cuda.synchronize()
